@@ -104,6 +104,8 @@ __device__ __forceinline__ void sn_rows(const float* w, const float* t, const fl
   float acc = 0.f;
   if (VEC == 4) {
     for (long c = lane * 4; c < cols; c += 64 * 4) {
+      // every product rounded before it is added: sigma's last bit is part of what seeded runs of a network reproduce
+#pragma clang fp contract(off)
       const f32x4 a = *reinterpret_cast<const f32x4*>(src + c), b = *reinterpret_cast<const f32x4*>(t + c);
       acc += (a[0] * b[0] + a[1] * b[1]) + (a[2] * b[2] + a[3] * b[3]);
     }
