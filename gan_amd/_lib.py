@@ -26,6 +26,8 @@ EXPORTS = (
     "gc_channel_scale", "gc_rowdot_workspace_bytes", "gc_rowdot", "gc_modulated_act_backward_workspace_bytes",
     "gc_modulated_act_backward", "gc_act_concat_fwd", "gc_act_concat_bwd",
     "gc_wgan_mix", "gc_gradient_penalty_workspace_bytes", "gc_gradient_penalty_fwd", "gc_gradient_penalty_bwd", "gc_wgan_critic_loss", "gc_image_batch_prepare", "gc_spectral_norm_workspace_bytes", "gc_spectral_norm_power_iteration", "gc_spectral_norm_multi_plan", "gc_spectral_norm_multi_run",
+    "gc_block_norm_fwd", "gc_block_norm_workspace_bytes", "gc_block_norm_bwd", "gc_axial_rotary", "gc_diff_attention_workspace_bytes",
+    "gc_diff_attention_fwd", "gc_diff_attention_bwd",
 )
 
 
@@ -41,6 +43,31 @@ class Epilogue(ctypes.Structure):
                 ("stat_rows", ctypes.c_void_p), ("stat_rows_capacity", ctypes.c_int32), ("stat_rows_written", ctypes.POINTER(ctypes.c_int32)),
                 ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
                 ("sample_scale", ctypes.c_void_p), ("sample_scale_out", ctypes.c_void_p)]
+
+
+_vp, _i32, _i64, _f32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
+
+
+class BlockNorm(ctypes.Structure):
+    _fields_ = ([(n, _i64) for n in ("batch", "rows")] + [(n, _i32) for n in ("cols", "dtype", "layer", "with_input_norm")] +
+                [("eps", _f32), ("residual_constant", _f32)] + [(n, _i32) for n in ("gate_per_sample", "mod_per_sample", "residual_per_channel", "reserved")] +
+                [(n, _i64) for n in ("x_batch_stride", "x_row_stride", "f_batch_stride", "f_row_stride")] +
+                [(n, _vp) for n in ("x", "f", "out_weight", "out_bias", "gate", "residual_scale", "in_weight", "in_bias", "scale", "shift", "y", "h",
+                                    "stats", "dy", "dh", "dx", "df", "d_out_weight", "d_out_bias", "d_gate", "d_residual_scale", "d_in_weight",
+                                    "d_in_bias", "d_scale", "d_shift")])
+
+
+class Rotary(ctypes.Structure):
+    _fields_ = ([(n, _i64) for n in ("batch", "tokens")] +
+                [(n, _i32) for n in ("q_heads", "k_heads", "dim", "pairs", "axes", "halves", "dtype", "position_dtype", "positions_per_sample", "inverse")] +
+                [("q_stride", _i64 * 3), ("k_stride", _i64 * 3)] +
+                [(n, _vp) for n in ("q", "k", "q_out", "k_out", "positions", "pair_turns", "pair_axis")])
+
+
+class DiffAttention(ctypes.Structure):
+    _fields_ = ([("q_stride", _i64 * 4), ("k_stride", _i64 * 4), ("v_stride", _i64 * 3)] +
+                [(n, _i32) for n in ("B", "NQ", "NK", "H", "HK", "d", "dv", "causal")] + [("scale", _f32), ("reserved", _i32)] +
+                [(n, _vp) for n in ("q", "k", "v", "lam", "key_lengths", "out", "out2", "lse", "dout", "dq", "dk", "dv_out", "dlam")])
 
 
 _lib = None
@@ -152,6 +179,15 @@ def lib():
     L.gc_adam_step.restype = ctypes.c_int
     L.gc_adam_ema_step.argtypes = [i32, vp, vp, vp, vp, vp, f32, vp, vp, f32, f32, f32, f32, vp]
     L.gc_adam_ema_step.restype = ctypes.c_int
+    L.gc_block_norm_fwd.argtypes = [ctypes.POINTER(BlockNorm), vp]
+    L.gc_block_norm_workspace_bytes.argtypes = [i64, i64, i32]
+    L.gc_block_norm_workspace_bytes.restype = sz
+    L.gc_block_norm_bwd.argtypes = [ctypes.POINTER(BlockNorm), vp, sz, vp]
+    L.gc_axial_rotary.argtypes = [ctypes.POINTER(Rotary), vp]
+    L.gc_diff_attention_workspace_bytes.argtypes = [ctypes.POINTER(DiffAttention), ctypes.c_int]
+    L.gc_diff_attention_workspace_bytes.restype = sz
+    L.gc_diff_attention_fwd.argtypes = [ctypes.POINTER(DiffAttention), vp, sz, vp]
+    L.gc_diff_attention_bwd.argtypes = [ctypes.POINTER(DiffAttention), vp, sz, vp]
     L.gc_profile_enable.argtypes = [ctypes.c_int]
     L.gc_profile_collect.argtypes = [ctypes.c_int, vp, vp, vp, vp]
     for fn in ("gc_pack_weight", "gc_conv2d_fprop", "gc_conv2d_dgrad", "gc_conv2d_wgrad", "gc_conv2d_wgrad_noalloc", "gc_dwblur3x3", "gc_dwblur3x3_masked", "gc_profile_enable",

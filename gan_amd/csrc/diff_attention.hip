@@ -1,0 +1,875 @@
+// Differential attention: the difference of two softmax maps over the same values,
+//
+//   out_i = sum_j (p1_ij - lam p2_ij) v_j,      pm_ij = exp(scale <q_m,i , k_m,j>) / sum_j' exp(..)      (visible keys j)
+//
+// with one lam per head.  Nothing of size rows x keys is stored.
+//
+// Forward: one pass over the keys with a running maximum and sum per map and two accumulators (the maps' denominators are known
+// only at the end), which share every value fragment read from LDS: per pair of positions 4 d + 4 dv multiply-adds of which the
+// definition needs 4 d + 2 dv.  Scores are computed TRANSPOSED, S^T = K Q^T on 32x32x16 matrix instructions, so that a lane holds
+// one softmax row i = lane % 32 at keys j = 8 (r / 4) + 4 h + r % 4 (h = lane / 32).  Taking the reduction index of the second
+// product in the order in which those accumulators lie (slot (h, e) of k-step t  <->  j = 16 t + 8 (e / 4) + 4 h + e % 4), the
+// exponentiated scores are its B operand P^T without a trip through LDS, and V^T in that order is what two transposing LDS reads
+// return.  The running maximum moves only when an exponential would exceed 2^8 (the sums are fp32 and keep their precision).
+//
+// Backward from the saved log2-sums L_m (P recomputed, dP = dO V^T shared by both maps, delta_m,i = dO_i . O_m,i):
+//   dV_j = sum_i (p1 - lam p2)_ij dO_i     dS1 = P1 (dP - delta1)     dS2 = -lam P2 (dP - delta2)     dQm = dSm Km, dKm = dSm^T Qm
+//   dlam = -sum_i (delta2_i + sum_j p2_ij (dP_ij - delta2_i)):  the second term vanishes but for the rounding of the stored O, which
+//   it takes out of the sum (an fp32 gradient that is not held to the bf16 rounding of O)
+// in two kernels that own the rows of their outputs (dkv: 128 keys of a key head, summed over the query heads that share them;
+// dq: 128 queries of a head): no atomics, results reproduce.
+//
+// Tiles of 64 rows go from HBM to LDS directly (16 bytes per lane), two stages in turn; the 16-byte chunks of a row are permuted on
+// the SOURCE side so that both the row-wise and the transposing reads spread over the banks.  Rows past the end, and the columns
+// between d and its padded width, are answered with zeros by the buffer's range check, so nothing behind a sample's length is read.
+// Probabilities and score gradients are rounded to bf16 for the second products (the operands' own type; 2^-9 each, independent),
+// everything else is fp32.
+#include "common.h"
+
+namespace gc {
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4_ptr;
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+
+constexpr int kRows = 128;                       // rows of a workgroup: 32 per wave
+constexpr int kBlk = 64;                         // rows staged per step
+constexpr uint32_t kOutOfRange = 0x80000000u;
+constexpr float kLazy = 8.f;                     // log2 units by which a score may exceed the running maximum
+constexpr float kLargeScore = 1048576.f;         // log2 units
+
+struct DiffParams {
+  gc_diff_attention a;
+  int G, tiles, nsplit, blocks_per_split;
+  FastDiv div_nq;
+  float c2, lazy;                                // scale * log2(e); kLazy in units of a score
+  float *part, *ml, *delta, *lampart;
+};
+
+__device__ __forceinline__ bf16x8 zero8() { return __builtin_bit_cast(bf16x8, u32x4{0u, 0u, 0u, 0u}); }
+__device__ __forceinline__ f32x16 zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int r = 0; r < 16; r++) z[r] = 0.f;
+  return z;
+}
+__device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ bf16x8 pack8(const f32x16& v, int r0) {
+  const u32x2 lo = cvt_bf16x4(f32x4{v[r0], v[r0 + 1], v[r0 + 2], v[r0 + 3]}), hi = cvt_bf16x4(f32x4{v[r0 + 4], v[r0 + 5], v[r0 + 6], v[r0 + 7]});
+  return __builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], hi[0], hi[1]});
+}
+// The two half-waves' values of a row, in both (v_permlane32_swap: one result holds the lower half's value, the other the upper's).
+// The results are copied to scalars first: a bit cast of a vector's element itself reads element 0.
+__device__ __forceinline__ void both_halves(float v, float& lo, float& hi) {
+  typedef unsigned int u32pair __attribute__((ext_vector_type(2)));
+  const unsigned int u = __builtin_bit_cast(unsigned int, v);
+  const u32pair r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const unsigned int a = r[0], b = r[1];
+  lo = __builtin_bit_cast(float, a);
+  hi = __builtin_bit_cast(float, b);
+}
+__device__ __forceinline__ float half_max(float v) {
+  float a, b;
+  both_halves(v, a, b);
+  return fmaxf(a, b);
+}
+__device__ __forceinline__ float half_sum(float v) {
+  float a, b;
+  both_halves(v, a, b);
+  return a + b;
+}
+
+// Chunk permutation of a tile row of ROWB bytes.  64 banks of 4 bytes: rows closer than 256 / ROWB apart never collide; among 16
+// rows at one chunk (row-wise reads) and 4 rows x 4 chunks (transposing reads) every 16-byte slot is used once.
+template <int ROWB>
+__device__ __forceinline__ int swz(int row) {
+  if (ROWB == 64) return (row >> 2) & 3;
+  if (ROWB == 128) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+  return ((row & 3) << 2) | ((row >> 2) & 3);
+}
+
+// Every load into LDS that this wave issued has landed, then the workgroup meets: the staged tile is complete and the other stage
+// is no longer read.  (A workgroup barrier alone does not wait for loads that are counted as vector memory.)
+__device__ __forceinline__ void tile_ready() {
+  __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));        // vmcnt(0)
+  __syncthreads();
+}
+
+// One tile of 64 rows of `width` elements (padded to ROWB / 2 columns), from a tensor with row stride `stride` bytes.
+template <int ROWB>
+struct Loader {
+  static constexpr int CPR = ROWB / 16, RPI = 64 / CPR, NI = ROWB / 64, BASES = ROWB >= 512 ? 2 : 1;
+  uint32_t voff[BASES];
+  uint32_t step;
+  int wave;
+  __device__ __forceinline__ void init(int wave_, int lane, uint32_t stride, int width) {
+    wave = wave_;
+#pragma unroll
+    for (int b = 0; b < BASES; b++) {
+      const int row = (wave + 4 * b) * RPI + lane / CPR, chunk = (lane % CPR) ^ swz<ROWB>(row);
+      voff[b] = chunk * 8 < width ? (uint32_t)row * stride + chunk * 16 : kOutOfRange;
+    }
+    step = 4 * RPI * stride;
+  }
+  // rows [row0, row0 + 64) of the tensor at `base`, of which those below `rows` exist
+  __device__ __forceinline__ void load(const uint16_t* base, int64_t row0, int64_t rows, uint32_t stride, int width, char* lds) const {
+    int64_t left = rows - row0;
+    left = left < 0 ? 0 : (left > kBlk ? kBlk : left);
+    const char* p = reinterpret_cast<const char*>(base) + row0 * (int64_t)stride;
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, left > 0 ? (int)((left - 1) * stride + width * 2) : 0, 0x00020000);
+#pragma unroll
+    for (int n = 0; n < NI; n++)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(lds + (wave + 4 * n) * 1024), 16, (int)(voff[n % BASES] + (uint32_t)(n - n % BASES) * step), 0, 0, 0);
+  }
+};
+
+// Row-wise A operand: rows r0 + lane % 32, columns 16 ks + 8 h + {0..7}
+template <int ROWB>
+__device__ __forceinline__ bf16x8 row_frag(const char* tile, int r0, int ks, int lane) {
+  const int row = lane & 31, h = lane >> 5;
+  return *reinterpret_cast<const bf16x8*>(tile + (r0 + row) * ROWB + (((2 * ks + h) ^ swz<ROWB>(row)) << 4));
+}
+// Transposed A operand: columns 32 cb + lane % 32, rows 16 t + {4 h + 0..3, 8 + 4 h + 0..3}
+template <int ROWB>
+__device__ __forceinline__ bf16x8 col_frag(const char* tile, int t, int cb, int lane) {
+  const int h = lane >> 5, rr = 4 * h + ((lane >> 2) & 3), chunk = cb * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), sub = (lane & 1) * 8;
+  const char* lo_p = tile + (16 * t + rr) * ROWB + ((chunk ^ swz<ROWB>(rr)) << 4) + sub;
+  const char* hi_p = tile + (16 * t + 8 + rr) * ROWB + ((chunk ^ swz<ROWB>(8 + rr)) << 4) + sub;
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)lo_p);
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)hi_p);
+  typedef short s16x8 __attribute__((ext_vector_type(8)));
+  const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  return __builtin_bit_cast(bf16x8, v);
+}
+// 8 elements of a global row as a B operand; zero past the row's width
+__device__ __forceinline__ bf16x8 global_frag(const uint16_t* row, bool valid, int col, int width) {
+  if (!valid || col >= width) return zero8();
+  return __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(row + col));
+}
+
+__device__ __forceinline__ int sample_length(const gc_diff_attention& a, int b) {
+  if (a.key_lengths == nullptr) return a.NK;
+  const int n = a.key_lengths[b];
+  return n < 0 ? 0 : (n > a.NK ? a.NK : n);
+}
+// number of visible keys of query i (possibly <= 0)
+__device__ __forceinline__ int visible(const gc_diff_attention& a, int i, int len) {
+  const int n = i + 1 + len - a.NQ;
+  return a.causal ? (n < 0 ? 0 : (n < len ? n : len)) : len;
+}
+
+template <int DK, int DV>
+struct Cfg {
+  static constexpr int KROW = DK * 2, VROW = DV * 2, KB = kBlk * KROW, VB = kBlk * VROW;
+  static constexpr int KS = DK / 16, VS = DV / 16, KC = DK / 32, VC = DV / 32;
+  static constexpr int WAVES = DV > 128 ? 1 : 2;      // per SIMD: the accumulators of the widest form take the registers of two
+};
+
+// ---------------------------------------------------------------------------------------------------------------------------
+// Rows of a workgroup: 128 of the G * NQ rows (head of the group, query) that share a key head.
+template <int DK, int DV>
+__global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_fwd_kernel(const DiffParams P) {
+  typedef Cfg<DK, DV> F;
+  constexpr int STAGE = 2 * F::KB + F::VB;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const gc_diff_attention& a = P.a;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  uint32_t lid = xcd_remap(blockIdx.x, gridDim.x);
+  const int split = (int)(lid % (uint32_t)P.nsplit);
+  lid /= (uint32_t)P.nsplit;
+  int tile = (int)(lid % (uint32_t)P.tiles);
+  const int bh = (int)(lid / (uint32_t)P.tiles), b = bh / a.HK, hk = bh - b * a.HK;
+  if (a.causal) tile = P.tiles - 1 - tile;                 // the longest rows first
+  const int R = P.G * a.NQ, len = sample_length(a, b);
+  const int r0 = tile * kRows, w0 = r0 + wave * 32, r = w0 + (lane & 31);
+  const bool valid = r < R;
+  const int rc = valid ? r : R - 1, g = (int)fd_div((uint32_t)rc, P.div_nq), i = rc - g * a.NQ, head = hk * P.G + g;
+  const int lim = visible(a, i, len);
+  // most and fewest visible keys of this wave's rows, most of the workgroup's
+  int kend = len, wmin = len, wmax = len;
+  if (a.causal) {
+    const int e = (r0 + kRows < R ? r0 + kRows : R) - 1, ge = (int)fd_div((uint32_t)e, P.div_nq), gs = (int)fd_div((uint32_t)r0, P.div_nq);
+    kend = gs == ge ? visible(a, e - ge * a.NQ, len) : len;
+    const int first = w0 < R ? w0 : R - 1, last = w0 + 31 < R ? w0 + 31 : R - 1;
+    const int gf = (int)fd_div((uint32_t)first, P.div_nq), gl = (int)fd_div((uint32_t)last, P.div_nq);
+    wmin = gf == gl ? visible(a, first - gf * a.NQ, len) : visible(a, 0, len);
+    wmax = gf == gl ? visible(a, last - gl * a.NQ, len) : len;
+  }
+  wmin = __builtin_amdgcn_readfirstlane(wmin);
+  wmax = __builtin_amdgcn_readfirstlane(wmax);
+
+  const uint16_t* qrow = static_cast<const uint16_t*>(a.q) + b * a.q_stride[0] + i * a.q_stride[1] + head * a.q_stride[2];
+  bf16x8 qf[2][F::KS];
+#pragma unroll
+  for (int m = 0; m < 2; m++)
+#pragma unroll
+    for (int ks = 0; ks < F::KS; ks++) qf[m][ks] = global_frag(qrow + m * a.q_stride[3], valid, ks * 16 + 8 * h, a.d);
+
+  f32x16 acc[2][F::VC];
+  float mrun[2] = {-INFINITY, -INFINITY}, lsum[2] = {0.f, 0.f};
+#pragma unroll
+  for (int m = 0; m < 2; m++)
+#pragma unroll
+    for (int cb = 0; cb < F::VC; cb++) acc[m][cb] = zero16();
+
+  const uint16_t* kbase = static_cast<const uint16_t*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[2];
+  const uint16_t* vbase = static_cast<const uint16_t*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[2];
+  const uint32_t kst = (uint32_t)(a.k_stride[1] * 2), vst = (uint32_t)(a.v_stride[1] * 2);
+  Loader<F::KROW> lk;
+  Loader<F::VROW> lv;
+  lk.init(wave, lane, kst, a.d);
+  lv.init(wave, lane, vst, a.dv);
+  auto fetch = [&](int blk, char* st) {
+    lk.load(kbase, (int64_t)blk * kBlk, len, kst, a.d, st);
+    lk.load(kbase + a.k_stride[3], (int64_t)blk * kBlk, len, kst, a.d, st + F::KB);
+    lv.load(vbase, (int64_t)blk * kBlk, len, vst, a.dv, st + 2 * F::KB);
+  };
+
+  const int nblk = (kend + kBlk - 1) / kBlk;
+  const int blk0 = split * P.blocks_per_split, blk1 = min(nblk, blk0 + P.blocks_per_split);
+  if (blk0 < blk1) fetch(blk0, smem);
+  for (int blk = blk0; blk < blk1; blk++) {
+    tile_ready();
+    if (blk + 1 < blk1) fetch(blk + 1, smem + ((blk + 1 - blk0) & 1) * STAGE);
+    const char* st = smem + ((blk - blk0) & 1) * STAGE;
+    const int j0 = blk * kBlk;
+    if (j0 >= wmax) continue;                              // (the whole wave; the barrier above is met by every wave in every step)
+    bf16x8 pb[2][4];
+#pragma unroll
+    for (int m = 0; m < 2; m++) {
+      f32x16 s[2];
+#pragma unroll
+      for (int jb = 0; jb < 2; jb++) {
+        s[jb] = zero16();
+#pragma unroll
+        for (int ks = 0; ks < F::KS; ks++) s[jb] = mfma(row_frag<F::KROW>(st + m * F::KB, jb * 32, ks, lane), qf[m][ks], s[jb]);
+      }
+      if (j0 + kBlk > wmin) {
+#pragma unroll
+        for (int jb = 0; jb < 2; jb++)
+#pragma unroll
+          for (int e = 0; e < 16; e++)
+            if (j0 + jb * 32 + 8 * (e >> 2) + 4 * h + (e & 3) >= lim) s[jb][e] = -INFINITY;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int jb = 0; jb < 2; jb++)
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) mx = fmaxf(fmaxf(s[jb][e], s[jb][e + 1]), mx);
+      mx = half_max(mx);
+      if (__builtin_amdgcn_ballot_w64(mx > mrun[m] + P.lazy) != 0) {
+        const float mn = fmaxf(mrun[m], mx);
+        const float alpha = __builtin_amdgcn_exp2f((mrun[m] - (mn == -INFINITY ? 0.f : mn)) * P.c2);
+        mrun[m] = mn;
+        lsum[m] *= alpha;
+#pragma unroll
+        for (int cb = 0; cb < F::VC; cb++) acc[m][cb] *= alpha;
+      }
+      const float top = mrun[m] == -INFINITY ? 0.f : mrun[m], base = top * P.c2;
+      // one multiply-add per score; its constant residue (2^-24 of base, the same for a whole row) cancels in the quotient unless it
+      // is itself an exponent to speak of, as with scores that stand for a mask's lowest value
+      if (__builtin_amdgcn_ballot_w64(fabsf(base) > kLargeScore) == 0) {
+#pragma unroll
+        for (int jb = 0; jb < 2; jb++)
+#pragma unroll
+          for (int e = 0; e < 16; e++) s[jb][e] = __builtin_amdgcn_exp2f(s[jb][e] * P.c2 - base);
+      } else {
+#pragma unroll
+        for (int jb = 0; jb < 2; jb++)
+#pragma unroll
+          for (int e = 0; e < 16; e++) s[jb][e] = __builtin_amdgcn_exp2f((s[jb][e] - top) * P.c2);
+      }
+#pragma unroll
+      for (int jb = 0; jb < 2; jb++) {
+#pragma unroll
+        for (int e = 0; e < 16; e++) lsum[m] += s[jb][e];
+        pb[m][2 * jb] = pack8(s[jb], 0);
+        pb[m][2 * jb + 1] = pack8(s[jb], 8);
+      }
+    }
+#pragma unroll
+    for (int cb = 0; cb < F::VC; cb++)
+#pragma unroll
+      for (int t = 0; t < 4; t++) {
+        const bf16x8 va = col_frag<F::VROW>(st + 2 * F::KB, t, cb, lane);
+        acc[0][cb] = mfma(va, pb[0][t], acc[0][cb]);
+        acc[1][cb] = mfma(va, pb[1][t], acc[1][cb]);
+      }
+  }
+
+  lsum[0] = half_sum(lsum[0]);
+  lsum[1] = half_sum(lsum[1]);
+  if (!valid) return;
+  if (P.nsplit > 1) {
+    const size_t row = ((size_t)split * a.B * a.HK + bh) * R + r;
+    float* ml = P.ml + row * 4;
+    if (h == 0) *reinterpret_cast<f32x4*>(ml) = f32x4{mrun[0], lsum[0], mrun[1], lsum[1]};
+#pragma unroll
+    for (int m = 0; m < 2; m++)
+      if (lsum[m] != 0.f)                                  // an empty share is not read by the joining kernel
+#pragma unroll
+        for (int cb = 0; cb < F::VC; cb++)
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            *reinterpret_cast<f32x4*>(P.part + (row * 2 + m) * DV + cb * 32 + 8 * e + 4 * h) =
+                f32x4{acc[m][cb][4 * e], acc[m][cb][4 * e + 1], acc[m][cb][4 * e + 2], acc[m][cb][4 * e + 3]};
+    return;
+  }
+  const float inv0 = lsum[0] != 0.f ? 1.f / lsum[0] : 0.f, inv1 = lsum[1] != 0.f ? 1.f / lsum[1] : 0.f, lam = a.lam[head];
+  const size_t orow = (((size_t)b * a.NQ + i) * a.H + head) * a.dv;
+#pragma unroll
+  for (int cb = 0; cb < F::VC; cb++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const int c = cb * 32 + 8 * e + 4 * h;
+      if (c >= a.dv) continue;
+      f32x4 o2, o;
+#pragma unroll
+      for (int x = 0; x < 4; x++) {
+        o2[x] = acc[1][cb][4 * e + x] * inv1;
+        o[x] = acc[0][cb][4 * e + x] * inv0 - lam * o2[x];
+      }
+      *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + orow + c) = cvt_bf16x4(o);
+      if (a.out2 != nullptr) *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out2) + orow + c) = cvt_bf16x4(o2);
+    }
+  if (a.lse != nullptr && h == 0) {
+    float* l = a.lse + ((size_t)b * a.H + head) * 2 * a.NQ + i;
+    l[0] = lsum[0] != 0.f ? mrun[0] * P.c2 + __log2f(lsum[0]) : INFINITY;
+    l[a.NQ] = lsum[1] != 0.f ? mrun[1] * P.c2 + __log2f(lsum[1]) : INFINITY;
+  }
+}
+
+// Joins the shares of a row that was split over the keys: one wave per row, lanes along the value columns.
+__global__ __launch_bounds__(kThreads) void diff_join_kernel(const DiffParams P, int DV) {
+  const gc_diff_attention& a = P.a;
+  const int R = P.G * a.NQ, lane = threadIdx.x & 63;
+  const int64_t idx = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+  const size_t rows = (size_t)a.B * a.HK * R;
+  if ((size_t)idx >= rows) return;
+  const int bh = (int)(idx / R), r = (int)(idx - (int64_t)bh * R), b = bh / a.HK, hk = bh - b * a.HK;
+  const int g = r / a.NQ, i = r - g * a.NQ, head = hk * P.G + g;
+  float M[2] = {-INFINITY, -INFINITY}, L[2] = {0.f, 0.f};
+  for (int s = 0; s < P.nsplit; s++) {
+    const float* ml = P.ml + ((size_t)s * rows + idx) * 4;
+    for (int m = 0; m < 2; m++) if (ml[2 * m + 1] != 0.f) M[m] = fmaxf(M[m], ml[2 * m]);
+  }
+  float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  for (int s = 0; s < P.nsplit; s++) {
+    const size_t row = (size_t)s * rows + idx;
+    const float* ml = P.ml + row * 4;
+    for (int m = 0; m < 2; m++) {
+      if (ml[2 * m + 1] == 0.f) continue;
+      const float w = __builtin_amdgcn_exp2f((ml[2 * m] - M[m]) * P.c2);
+      L[m] += w * ml[2 * m + 1];
+      const float* src = P.part + (row * 2 + m) * DV;
+#pragma unroll
+      for (int x = 0; x < 4; x++)
+        if (lane + 64 * x < a.dv) acc[m][x] += w * src[lane + 64 * x];
+    }
+  }
+  const float inv0 = L[0] != 0.f ? 1.f / L[0] : 0.f, inv1 = L[1] != 0.f ? 1.f / L[1] : 0.f, lam = a.lam[head];
+  const size_t orow = (((size_t)b * a.NQ + i) * a.H + head) * a.dv;
+#pragma unroll
+  for (int x = 0; x < 4; x++) {
+    const int c = lane + 64 * x;
+    if (c >= a.dv) continue;
+    const float o2 = acc[1][x] * inv1;
+    static_cast<uint16_t*>(a.out)[orow + c] = float_to_bf16_bits(acc[0][x] * inv0 - lam * o2);
+    if (a.out2 != nullptr) static_cast<uint16_t*>(a.out2)[orow + c] = float_to_bf16_bits(o2);
+  }
+  if (a.lse != nullptr && lane == 0) {
+    float* l = a.lse + ((size_t)b * a.H + head) * 2 * a.NQ + i;
+    l[0] = L[0] != 0.f ? M[0] * P.c2 + __log2f(L[0]) : INFINITY;
+    l[a.NQ] = L[1] != 0.f ? M[1] * P.c2 + __log2f(L[1]) : INFINITY;
+  }
+}
+
+// delta [B][H][2][NQ]: dO . O1 = dO . out + lam dO . O2, and dO . O2; 16 lanes per row
+__global__ __launch_bounds__(kThreads) void diff_delta_kernel(const DiffParams P) {
+  const gc_diff_attention& a = P.a;
+  const size_t rows = (size_t)a.B * a.NQ * a.H, row = ((size_t)blockIdx.x * kThreads + threadIdx.x) >> 4;
+  const int sub = threadIdx.x & 15;
+  float s[2] = {0.f, 0.f};
+  if (row < rows)
+    for (int c = sub * 8; c < a.dv; c += 128) {
+      const size_t o = row * a.dv + c;
+      const u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.dout) + o);
+      const u32x4 x = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.out) + o);
+      const u32x4 y = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.out2) + o);
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const float wl = __builtin_bit_cast(float, w[e] << 16), wh = __builtin_bit_cast(float, w[e] & 0xffff0000u);
+        s[0] += wl * __builtin_bit_cast(float, x[e] << 16) + wh * __builtin_bit_cast(float, x[e] & 0xffff0000u);
+        s[1] += wl * __builtin_bit_cast(float, y[e] << 16) + wh * __builtin_bit_cast(float, y[e] & 0xffff0000u);
+      }
+    }
+#pragma unroll
+  for (int m = 0; m < 2; m++)
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) s[m] += __shfl_xor(s[m], o);
+  if (row < rows && sub == 0) {
+    const int head = (int)(row % a.H);
+    const size_t bi = row / a.H, b = bi / a.NQ, i = bi - b * a.NQ;
+    float* d = P.delta + (b * a.H + head) * 2 * a.NQ + i;
+    d[0] = s[0] + a.lam[head] * s[1];
+    d[a.NQ] = s[1];
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------
+// Owner: 128 queries of a head; walks the keys.  Produces dQ and the workgroup's share of dlam.
+template <int DK, int DV>
+__global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dq_kernel(const DiffParams P) {
+  typedef Cfg<DK, DV> F;
+  constexpr int STAGE = 2 * F::KB + F::VB;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ float red[kThreads / 64];
+  const gc_diff_attention& a = P.a;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const uint32_t lid = xcd_remap(blockIdx.x, gridDim.x);
+  int tile = (int)(lid % (uint32_t)P.tiles);
+  const int bh = (int)(lid / (uint32_t)P.tiles), b = bh / a.H, head = bh - b * a.H, hk = head / P.G;
+  if (a.causal) tile = P.tiles - 1 - tile;
+  const int len = sample_length(a, b), r0 = tile * kRows, w0 = r0 + wave * 32, r = w0 + (lane & 31);
+  const bool valid = r < a.NQ;
+  const int i = valid ? r : a.NQ - 1, lim = visible(a, i, len);
+  const int kend = visible(a, min(r0 + kRows, a.NQ) - 1, len);
+  const int wmin = visible(a, min(w0, a.NQ - 1), len), wmax = visible(a, min(w0 + 31, a.NQ - 1), len);
+
+  const uint16_t* qrow = static_cast<const uint16_t*>(a.q) + b * a.q_stride[0] + i * a.q_stride[1] + head * a.q_stride[2];
+  const size_t orow = (((size_t)b * a.NQ + i) * a.H + head) * a.dv;
+  const uint16_t* grow = static_cast<const uint16_t*>(a.dout) + orow;
+  bf16x8 qf[2][F::KS], gf[F::VS];
+#pragma unroll
+  for (int m = 0; m < 2; m++)
+#pragma unroll
+    for (int ks = 0; ks < F::KS; ks++) qf[m][ks] = global_frag(qrow + m * a.q_stride[3], valid, ks * 16 + 8 * h, a.d);
+#pragma unroll
+  for (int ks = 0; ks < F::VS; ks++) gf[ks] = global_frag(grow, valid, ks * 16 + 8 * h, a.dv);
+  float L[2], D[2];
+#pragma unroll
+  for (int m = 0; m < 2; m++) {
+    const size_t o = ((size_t)(b * a.H + head) * 2 + m) * a.NQ + i;
+    L[m] = a.lse[o];
+    D[m] = P.delta[o];
+  }
+
+  f32x16 acc[2][F::KC];
+#pragma unroll
+  for (int m = 0; m < 2; m++)
+#pragma unroll
+    for (int cb = 0; cb < F::KC; cb++) acc[m][cb] = zero16();
+  float left = 0.f;                                        // sum_j p2 (dP - delta2)
+
+  const uint16_t* kbase = static_cast<const uint16_t*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[2];
+  const uint16_t* vbase = static_cast<const uint16_t*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[2];
+  const uint32_t kst = (uint32_t)(a.k_stride[1] * 2), vst = (uint32_t)(a.v_stride[1] * 2);
+  Loader<F::KROW> lk;
+  Loader<F::VROW> lv;
+  lk.init(wave, lane, kst, a.d);
+  lv.init(wave, lane, vst, a.dv);
+  auto fetch = [&](int blk, char* st) {
+    lk.load(kbase, (int64_t)blk * kBlk, len, kst, a.d, st);
+    lk.load(kbase + a.k_stride[3], (int64_t)blk * kBlk, len, kst, a.d, st + F::KB);
+    lv.load(vbase, (int64_t)blk * kBlk, len, vst, a.dv, st + 2 * F::KB);
+  };
+  const int nblk = (kend + kBlk - 1) / kBlk;
+  if (nblk > 0) fetch(0, smem);
+  for (int blk = 0; blk < nblk; blk++) {
+    tile_ready();
+    if (blk + 1 < nblk) fetch(blk + 1, smem + ((blk + 1) & 1) * STAGE);
+    const char* st = smem + (blk & 1) * STAGE;
+    const int j0 = blk * kBlk;
+    if (j0 >= wmax) continue;
+    const bool masked = j0 + kBlk > wmin;
+#pragma unroll
+    for (int jb = 0; jb < 2; jb++) {
+      f32x16 s[2], dp = zero16();
+#pragma unroll
+      for (int m = 0; m < 2; m++) {
+        s[m] = zero16();
+#pragma unroll
+        for (int ks = 0; ks < F::KS; ks++) s[m] = mfma(row_frag<F::KROW>(st + m * F::KB, jb * 32, ks, lane), qf[m][ks], s[m]);
+      }
+#pragma unroll
+      for (int ks = 0; ks < F::VS; ks++) dp = mfma(row_frag<F::VROW>(st + 2 * F::KB, jb * 32, ks, lane), gf[ks], dp);
+#pragma unroll
+      for (int e = 0; e < 16; e++) {
+        float p0 = __builtin_amdgcn_exp2f(s[0][e] * P.c2 - L[0]), p1 = __builtin_amdgcn_exp2f(s[1][e] * P.c2 - L[1]);
+        if (masked && j0 + jb * 32 + 8 * (e >> 2) + 4 * h + (e & 3) >= lim) { p0 = 0.f; p1 = 0.f; }
+        s[0][e] = p0 * (dp[e] - D[0]);
+        s[1][e] = p1 * (dp[e] - D[1]);
+        left += s[1][e];
+      }
+#pragma unroll
+      for (int m = 0; m < 2; m++) {
+        const bf16x8 d0 = pack8(s[m], 0), d1 = pack8(s[m], 8);
+#pragma unroll
+        for (int cb = 0; cb < F::KC; cb++) {
+          acc[m][cb] = mfma(col_frag<F::KROW>(st + m * F::KB, 2 * jb, cb, lane), d0, acc[m][cb]);
+          acc[m][cb] = mfma(col_frag<F::KROW>(st + m * F::KB, 2 * jb + 1, cb, lane), d1, acc[m][cb]);
+        }
+      }
+    }
+  }
+  const float lam = a.lam[head];
+  if (valid) {
+    const float f[2] = {a.scale, -lam * a.scale};
+    uint16_t* dst = static_cast<uint16_t*>(a.dq) + (((size_t)b * a.NQ + i) * a.H + head) * 2 * a.d;
+#pragma unroll
+    for (int m = 0; m < 2; m++)
+#pragma unroll
+      for (int cb = 0; cb < F::KC; cb++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int c = cb * 32 + 8 * e + 4 * h;
+          if (c >= a.d) continue;
+          *reinterpret_cast<u32x2*>(dst + m * a.d + c) = cvt_bf16x4(f32x4{acc[m][cb][4 * e] * f[m], acc[m][cb][4 * e + 1] * f[m], acc[m][cb][4 * e + 2] * f[m],
+                                                                       acc[m][cb][4 * e + 3] * f[m]});
+        }
+  }
+  float t = valid ? left + (h == 0 ? D[1] : 0.f) : 0.f;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
+  if (lane == 0) red[wave] = t;
+  __syncthreads();
+  if (tid == 0) P.lampart[(size_t)bh * P.tiles + tile] = ((red[0] + red[1]) + red[2]) + red[3];
+}
+
+// dlam[head] = -(the workgroups' shares, added in a fixed order); one workgroup per head
+__global__ __launch_bounds__(kThreads) void diff_dlam_kernel(const DiffParams P) {
+  __shared__ float red[kThreads];
+  const int head = blockIdx.x;
+  const int64_t n = (int64_t)P.a.B * P.tiles;
+  float s = 0.f;
+  for (int64_t i = threadIdx.x; i < n; i += kThreads) {
+    const int64_t b = i / P.tiles, t = i - b * P.tiles;
+    s += P.lampart[(b * P.a.H + head) * P.tiles + t];
+  }
+  red[threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float t = 0.f;
+    for (int i = 0; i < kThreads; i++) t += red[i];
+    P.a.dlam[head] = -t;
+  }
+}
+
+// Owner: 128 keys of a key head; walks the queries of every head that shares them.  Produces dK and dV.  OUT: 1 dK, 2 dV, 3 both
+// (both accumulators of the widest form do not fit the register file: it runs as two launches).
+template <int DK, int DV, int OUT>
+__global__ __launch_bounds__(kThreads, (DV > 64 ? 1 : 2)) void diff_bwd_dkv_kernel(const DiffParams P) {
+  typedef Cfg<DK, DV> F;
+  constexpr int VECB = 4 * kBlk * 4;                       // L1, L2, delta1, delta2 of the staged queries
+  constexpr int STAGE = 2 * F::KB + F::VB + VECB;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const gc_diff_attention& a = P.a;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const uint32_t lid = xcd_remap(blockIdx.x, gridDim.x);
+  const int tile = (int)(lid % (uint32_t)P.tiles), bh = (int)(lid / (uint32_t)P.tiles), b = bh / a.HK, hk = bh - b * a.HK;
+  const int len = sample_length(a, b), j0 = tile * kRows, w0 = j0 + wave * 32, j = w0 + (lane & 31);
+  const bool exists = j < a.NK, valid = j < len;
+
+  const int jc = valid ? j : 0;
+  const uint16_t* krow = static_cast<const uint16_t*>(a.k) + b * a.k_stride[0] + jc * a.k_stride[1] + hk * a.k_stride[2];
+  const uint16_t* vrow = static_cast<const uint16_t*>(a.v) + b * a.v_stride[0] + jc * a.v_stride[1] + hk * a.v_stride[2];
+  bf16x8 kf[2][F::KS], vf[F::VS];
+#pragma unroll
+  for (int m = 0; m < 2; m++)
+#pragma unroll
+    for (int ks = 0; ks < F::KS; ks++) kf[m][ks] = global_frag(krow + m * a.k_stride[3], valid, ks * 16 + 8 * h, a.d);
+  if (OUT & 1)
+#pragma unroll
+    for (int ks = 0; ks < F::VS; ks++) vf[ks] = global_frag(vrow, valid, ks * 16 + 8 * h, a.dv);
+
+  f32x16 adk[2][F::KC], adv[F::VC];
+#pragma unroll
+  for (int cb = 0; cb < F::KC; cb++) { adk[0][cb] = zero16(); adk[1][cb] = zero16(); }
+#pragma unroll
+  for (int cb = 0; cb < F::VC; cb++) adv[cb] = zero16();
+
+  const uint32_t qst = (uint32_t)(a.q_stride[1] * 2), gst = (uint32_t)a.H * a.dv * 2;
+  Loader<F::KROW> lq;
+  Loader<F::VROW> lg;
+  lq.init(wave, lane, qst, a.d);
+  lg.init(wave, lane, gst, a.dv);
+  // first query that sees key j: i >= j + NQ - len
+  const int shift = a.causal ? a.NQ - len : -a.NK - 1;
+  const int imin = j + shift;                              // this lane's (this key's) first query
+  const int first = max(0, (j0 + shift) / kBlk), nblk = (a.NQ + kBlk - 1) / kBlk;
+  const int per_head = j0 < len && nblk > first ? nblk - first : 0, steps = per_head * P.G;
+  auto fetch = [&](int step, char* st) {
+    const int g = step / per_head, blk = first + step - g * per_head, head = hk * P.G + g;
+    const uint16_t* q = static_cast<const uint16_t*>(a.q) + b * a.q_stride[0] + head * a.q_stride[2];
+    const uint16_t* go = static_cast<const uint16_t*>(a.dout) + ((size_t)b * a.NQ * a.H + head) * a.dv;
+    lq.load(q, (int64_t)blk * kBlk, a.NQ, qst, a.d, st);
+    lq.load(q + a.q_stride[3], (int64_t)blk * kBlk, a.NQ, qst, a.d, st + F::KB);
+    lg.load(go, (int64_t)blk * kBlk, a.NQ, gst, a.dv, st + 2 * F::KB);
+    // wave 0, 1: L of the two maps; 2, 3: delta.  64 floats, zeros past the last query
+    const float* v = (wave < 2 ? a.lse : P.delta) + ((size_t)(b * a.H + head) * 2 + (wave & 1)) * a.NQ + (int64_t)blk * kBlk;
+    const int left = min(kBlk, a.NQ - blk * kBlk);
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(v), 0, left * 4, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(st + 2 * F::KB + F::VB + wave * kBlk * 4), 4, lane * 4, 0, 0, 0);
+  };
+  if (steps > 0) fetch(0, smem);
+  for (int step = 0; step < steps; step++) {
+    tile_ready();
+    if (step + 1 < steps) fetch(step + 1, smem + ((step + 1) & 1) * STAGE);
+    const char* st = smem + (step & 1) * STAGE;
+    const float* vec = reinterpret_cast<const float*>(st + 2 * F::KB + F::VB);
+    const int g = step / per_head, i0 = (first + step - g * per_head) * kBlk;
+    const float nlam = -a.lam[hk * P.G + g];
+    if (i0 + kBlk - 1 < w0 + shift) continue;              // no query of the block sees a key of this wave
+    const bool masked = i0 < w0 + 31 + shift;
+#pragma unroll
+    for (int ib = 0; ib < 2; ib++) {
+      f32x16 s[2], dp = zero16();
+#pragma unroll
+      for (int m = 0; m < 2; m++) {
+        s[m] = zero16();
+#pragma unroll
+        for (int ks = 0; ks < F::KS; ks++) s[m] = mfma(row_frag<F::KROW>(st + m * F::KB, ib * 32, ks, lane), kf[m][ks], s[m]);
+      }
+      if (OUT & 1)
+#pragma unroll
+        for (int ks = 0; ks < F::VS; ks++) dp = mfma(row_frag<F::VROW>(st + 2 * F::KB, ib * 32, ks, lane), vf[ks], dp);
+      f32x16 mix;
+#pragma unroll
+      for (int e4 = 0; e4 < 4; e4++) {
+        const int o = ib * 32 + 8 * e4 + 4 * h;
+        const f32x4 L0 = *reinterpret_cast<const f32x4*>(vec + o), L1 = *reinterpret_cast<const f32x4*>(vec + kBlk + o);
+        const f32x4 D0 = *reinterpret_cast<const f32x4*>(vec + 2 * kBlk + o), D1 = *reinterpret_cast<const f32x4*>(vec + 3 * kBlk + o);
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+          const int e = 4 * e4 + x;
+          float p0 = __builtin_amdgcn_exp2f(s[0][e] * P.c2 - L0[x]), p1 = __builtin_amdgcn_exp2f(s[1][e] * P.c2 - L1[x]);
+          if (masked && i0 + o + x < imin) { p0 = 0.f; p1 = 0.f; }
+          p1 *= nlam;
+          mix[e] = p0 + p1;
+          s[0][e] = p0 * (dp[e] - D0[x]);
+          s[1][e] = p1 * (dp[e] - D1[x]);
+        }
+      }
+      if (OUT & 2) {
+        const bf16x8 m0 = pack8(mix, 0), m1 = pack8(mix, 8);
+#pragma unroll
+        for (int cb = 0; cb < F::VC; cb++) {
+          adv[cb] = mfma(col_frag<F::VROW>(st + 2 * F::KB, 2 * ib, cb, lane), m0, adv[cb]);
+          adv[cb] = mfma(col_frag<F::VROW>(st + 2 * F::KB, 2 * ib + 1, cb, lane), m1, adv[cb]);
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < ((OUT & 1) ? 2 : 0); m++) {
+        const bf16x8 d0 = pack8(s[m], 0), d1 = pack8(s[m], 8);
+#pragma unroll
+        for (int cb = 0; cb < F::KC; cb++) {
+          adk[m][cb] = mfma(col_frag<F::KROW>(st + m * F::KB, 2 * ib, cb, lane), d0, adk[m][cb]);
+          adk[m][cb] = mfma(col_frag<F::KROW>(st + m * F::KB, 2 * ib + 1, cb, lane), d1, adk[m][cb]);
+        }
+      }
+    }
+  }
+  if (!exists) return;
+  // keys behind the sample's length: zeros (their columns hold whatever the zero-filled operands gave)
+  uint16_t* dk = static_cast<uint16_t*>(a.dk) + ((size_t)(b * (size_t)a.NK + j) * a.HK + hk) * 2 * a.d;
+  uint16_t* dv = static_cast<uint16_t*>(a.dv_out) + ((size_t)(b * (size_t)a.NK + j) * a.HK + hk) * a.dv;
+  const u32x2 none = {0u, 0u};
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+#pragma unroll
+    for (int m = 0; m < ((OUT & 1) ? 2 : 0); m++)
+#pragma unroll
+      for (int cb = 0; cb < F::KC; cb++) {
+        const int c = cb * 32 + 8 * e + 4 * h;
+        const f32x16& v = adk[m][cb];
+        if (c < a.d)
+          *reinterpret_cast<u32x2*>(dk + m * a.d + c) =
+              valid ? cvt_bf16x4(f32x4{v[4 * e] * a.scale, v[4 * e + 1] * a.scale, v[4 * e + 2] * a.scale, v[4 * e + 3] * a.scale}) : none;
+      }
+#pragma unroll
+    for (int cb = 0; cb < ((OUT & 2) ? F::VC : 0); cb++) {
+      const int c = cb * 32 + 8 * e + 4 * h;
+      const f32x16& v = adv[cb];
+      if (c < a.dv) *reinterpret_cast<u32x2*>(dv + c) = valid ? cvt_bf16x4(f32x4{v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]}) : none;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------
+bool misaligned(const void* p) { return p == nullptr || (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
+
+int form_of(const gc_diff_attention* a) { return a->d <= 32 && a->dv <= 64 ? 0 : (a->d <= 64 && a->dv <= 128 ? 1 : 2); }
+constexpr int kDV[3] = {64, 128, 256};
+
+int check_desc(const gc_diff_attention* a, bool backward) {
+  if (a == nullptr) { set_error("differential attention: null descriptor"); return GC_BAD_ARGUMENT; }
+  if (a->B < 0 || a->NQ < 0 || a->NK < 0 || a->H <= 0 || a->HK <= 0 || a->H % a->HK != 0 || a->d <= 0 || a->d > 128 || a->d % 8 != 0 || a->dv <= 0 ||
+      a->dv > 256 || a->dv % 8 != 0) {
+    set_error("differential attention: supported are d %% 8 == 0 up to 128, dv %% 8 == 0 up to 256, H a multiple of HK (got B=%d NQ=%d NK=%d H=%d HK=%d d=%d dv=%d)",
+              a->B, a->NQ, a->NK, a->H, a->HK, a->d, a->dv);
+    return GC_UNSUPPORTED_GEOMETRY;
+  }
+  const int64_t G = a->H / a->HK;
+  const int64_t tiles = (int64_t)a->B * a->H * (((int64_t)(a->NQ > a->NK ? a->NQ : a->NK) + kRows - 1) / kRows);
+  if (G * a->NQ >= (1ll << 30) || a->NK >= (1 << 30) || tiles * 64 >= (1ll << 31)) {
+    set_error("differential attention: too many rows (B=%d NQ=%d NK=%d H=%d)", a->B, a->NQ, a->NK, a->H);
+    return GC_UNSUPPORTED_GEOMETRY;
+  }
+  if (!(a->scale > 0.f) || a->scale > 1e30f) { set_error("differential attention: scale must be positive and finite"); return GC_BAD_ARGUMENT; }
+  for (int i = 0; i < 4; i++)
+    if (a->q_stride[i] % 8 != 0 || a->k_stride[i] % 8 != 0 || (i < 3 && a->v_stride[i] % 8 != 0)) {
+      set_error("differential attention: strides must be multiples of 8 elements");
+      return GC_BAD_ARGUMENT;
+    }
+  const int64_t widest = 1ll << 23;       // elements: 64 rows stay below 2^30 bytes
+  if (a->q_stride[1] < a->d || a->k_stride[1] < a->d || a->v_stride[1] < a->dv || a->q_stride[1] >= widest || a->k_stride[1] >= widest || a->v_stride[1] >= widest ||
+      (int64_t)a->H * a->dv >= widest) {
+    set_error("differential attention: rows must not overlap and row strides must be below 2^23 elements");
+    return GC_UNSUPPORTED_GEOMETRY;
+  }
+  const void* base[] = {a->q, a->k, a->v, a->out};
+  for (const void* p : base)
+    if (misaligned(p)) { set_error("differential attention: q, k, v and out must be non-null and 16-byte aligned"); return GC_BAD_ARGUMENT; }
+  if (a->lam == nullptr || (a->out2 != nullptr && misaligned(a->out2))) { set_error("differential attention: lam is null or out2 misaligned"); return GC_BAD_ARGUMENT; }
+  if (backward) {
+    const void* more[] = {a->out2, a->dout, a->dq, a->dk, a->dv_out};
+    for (const void* p : more)
+      if (misaligned(p)) { set_error("differential attention backward: out2, dout, dq, dk, dv must be non-null and 16-byte aligned"); return GC_BAD_ARGUMENT; }
+    if (a->lse == nullptr || a->dlam == nullptr) { set_error("differential attention backward: lse and dlam must not be null"); return GC_BAD_ARGUMENT; }
+  }
+  return GC_OK;
+}
+
+// Few rows, long keys: the keys are split so that about two workgroups per CU run, each with at least four blocks.
+void plan_forward(const gc_diff_attention* a, DiffParams& P) {
+  P.a = *a;
+  P.G = a->H / a->HK;
+  const int64_t R = (int64_t)P.G * a->NQ, nblk = ((int64_t)a->NK + kBlk - 1) / kBlk;
+  P.tiles = (int)((R + kRows - 1) / kRows);
+  P.div_nq = make_fastdiv((uint32_t)a->NQ);
+  P.c2 = a->scale * 1.44269504088896340736f;
+  P.lazy = kLazy / P.c2;
+  const int64_t groups = (int64_t)a->B * a->HK * P.tiles, want = 2ll * device_cu_count();
+  int64_t n = groups > 0 && groups < want ? (want + groups - 1) / groups : 1;
+  if (n > nblk / 4) n = nblk / 4;
+  if (n > 256) n = 256;
+  if (n < 1) n = 1;
+  P.blocks_per_split = (int)((nblk + n - 1) / n);
+  if (P.blocks_per_split < 1) P.blocks_per_split = 1;
+  P.nsplit = (int)((nblk + P.blocks_per_split - 1) / P.blocks_per_split);
+  if (P.nsplit < 1) P.nsplit = 1;
+}
+size_t forward_bytes(const DiffParams& P, int DV) {
+  if (P.nsplit <= 1) return 0;
+  const size_t rows = (size_t)P.nsplit * P.a.B * P.a.HK * P.G * P.a.NQ;
+  return rows * (4 + 2 * (size_t)DV) * sizeof(float);
+}
+size_t backward_bytes(const gc_diff_attention* a) {
+  const size_t rows = (size_t)a->B * a->H * a->NQ, tiles = (size_t)a->B * a->H * ((a->NQ + kRows - 1) / kRows);
+  return ((rows * 2 + 3) / 4 * 4 + tiles) * sizeof(float);
+}
+
+template <int DK, int DV>
+int launch_fwd(const DiffParams& P, hipStream_t s) {
+  typedef Cfg<DK, DV> F;
+  constexpr int lds = 2 * (2 * F::KB + F::VB);
+  if (int e = ensure_dynamic_smem(reinterpret_cast<const void*>(diff_fwd_kernel<DK, DV>), lds)) return e;
+  hipLaunchKernelGGL((diff_fwd_kernel<DK, DV>), dim3((unsigned)P.a.B * P.a.HK * P.tiles * P.nsplit), dim3(kThreads), lds, s, P);
+  return check_hip(hipGetLastError(), "diff_fwd launch");
+}
+template <int DK, int DV>
+int launch_dq(const DiffParams& P, hipStream_t s) {
+  typedef Cfg<DK, DV> F;
+  constexpr int lds = 2 * (2 * F::KB + F::VB);
+  if (int e = ensure_dynamic_smem(reinterpret_cast<const void*>(diff_bwd_dq_kernel<DK, DV>), lds)) return e;
+  hipLaunchKernelGGL((diff_bwd_dq_kernel<DK, DV>), dim3((unsigned)P.a.B * P.a.H * P.tiles), dim3(kThreads), lds, s, P);
+  return check_hip(hipGetLastError(), "diff_bwd_dq launch");
+}
+template <int DK, int DV, int OUT>
+int launch_dkv(const DiffParams& P, hipStream_t s) {
+  typedef Cfg<DK, DV> F;
+  constexpr int lds = 2 * (2 * F::KB + F::VB + 4 * kBlk * 4);
+  if (int e = ensure_dynamic_smem(reinterpret_cast<const void*>(diff_bwd_dkv_kernel<DK, DV, OUT>), lds)) return e;
+  hipLaunchKernelGGL((diff_bwd_dkv_kernel<DK, DV, OUT>), dim3((unsigned)P.a.B * P.a.HK * P.tiles), dim3(kThreads), lds, s, P);
+  return check_hip(hipGetLastError(), "diff_bwd_dkv launch");
+}
+
+}  // namespace
+}  // namespace gc
+
+using namespace gc;
+
+extern "C" size_t gc_diff_attention_workspace_bytes(const gc_diff_attention* desc, int backward) {
+  if (desc == nullptr || desc->B <= 0 || desc->NQ <= 0 || desc->H <= 0 || desc->HK <= 0 || desc->H % desc->HK != 0) return 0;
+  if (backward) return backward_bytes(desc);
+  DiffParams P{};
+  plan_forward(desc, P);
+  return forward_bytes(P, kDV[form_of(desc)]);
+}
+
+extern "C" int gc_diff_attention_fwd(const gc_diff_attention* desc, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int e = check_desc(desc, false)) return e;
+  if (desc->B == 0 || desc->NQ == 0) return GC_OK;
+  DiffParams P{};
+  plan_forward(desc, P);
+  const int form = form_of(desc), DV = kDV[form];
+  const size_t need = forward_bytes(P, DV);
+  if (need > 0 && (misaligned(workspace) || workspace_bytes < need)) {
+    set_error("differential attention: a 16-byte aligned workspace of %zu bytes is needed", need);
+    return GC_WORKSPACE_TOO_SMALL;
+  }
+  const size_t rows = (size_t)P.nsplit * desc->B * desc->HK * P.G * desc->NQ;
+  P.ml = static_cast<float*>(workspace);
+  P.part = need > 0 ? P.ml + rows * 4 : nullptr;
+  hipStream_t s = (hipStream_t)stream;
+  {
+    ProfScope ps("gc::diff_fwd_kernel", 4.0 * desc->B * desc->H * (double)desc->NQ * desc->NK * (desc->d + desc->dv), s);
+    const int e = form == 0 ? launch_fwd<32, 64>(P, s) : (form == 1 ? launch_fwd<64, 128>(P, s) : launch_fwd<128, 256>(P, s));
+    if (e) return e;
+  }
+  if (P.nsplit > 1) {
+    const size_t out_rows = (size_t)desc->B * desc->H * desc->NQ;
+    hipLaunchKernelGGL(diff_join_kernel, dim3((unsigned)((out_rows + 3) / 4)), dim3(kThreads), 0, s, P, DV);
+    return check_hip(hipGetLastError(), "diff_join launch");
+  }
+  return GC_OK;
+}
+
+extern "C" int gc_diff_attention_bwd(const gc_diff_attention* desc, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int e = check_desc(desc, true)) return e;
+  if (desc->B == 0 || desc->NQ == 0 || desc->NK == 0) {
+    set_error("differential attention backward: an empty tensor has no gradient to compute");
+    return GC_BAD_ARGUMENT;
+  }
+  const size_t need = backward_bytes(desc);
+  if (misaligned(workspace) || workspace_bytes < need) {
+    set_error("differential attention backward: a 16-byte aligned workspace of %zu bytes is needed", need);
+    return GC_WORKSPACE_TOO_SMALL;
+  }
+  DiffParams P{};
+  plan_forward(desc, P);
+  const size_t rows = (size_t)desc->B * desc->H * desc->NQ;
+  P.delta = static_cast<float*>(workspace);
+  P.lampart = P.delta + (rows * 2 + 3) / 4 * 4;
+  hipStream_t s = (hipStream_t)stream;
+  const int form = form_of(desc);
+  const double pairs = (double)desc->B * desc->H * desc->NQ * desc->NK;
+  hipLaunchKernelGGL(diff_delta_kernel, dim3((unsigned)((rows * 16 + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, P);
+  if (check_hip(hipGetLastError(), "diff_delta launch")) return GC_HIP_ERROR;
+  {
+    P.tiles = (desc->NK + kRows - 1) / kRows;
+    ProfScope ps("gc::diff_bwd_dkv_kernel", pairs * (8.0 * desc->d + 4.0 * desc->dv), s);
+    int e = form == 0 ? launch_dkv<32, 64, 3>(P, s) : (form == 1 ? launch_dkv<64, 128, 3>(P, s) : launch_dkv<128, 256, 1>(P, s));
+    if (e == GC_OK && form == 2) e = launch_dkv<128, 256, 2>(P, s);
+    if (e) return e;
+  }
+  P.tiles = (desc->NQ + kRows - 1) / kRows;
+  {
+    ProfScope ps("gc::diff_bwd_dq_kernel", pairs * (8.0 * desc->d + 2.0 * desc->dv), s);
+    const int e = form == 0 ? launch_dq<32, 64>(P, s) : (form == 1 ? launch_dq<64, 128>(P, s) : launch_dq<128, 256>(P, s));
+    if (e) return e;
+  }
+  hipLaunchKernelGGL(diff_dlam_kernel, dim3(desc->H), dim3(kThreads), 0, s, P);
+  return check_hip(hipGetLastError(), "diff_dlam launch");
+}

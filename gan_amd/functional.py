@@ -13,7 +13,7 @@ import os
 
 import torch
 
-from . import ops
+from . import ops, token_ops
 
 
 def _single(v, name):
@@ -195,3 +195,60 @@ def upsample_nearest2x_add(input, addend):
     if not _FUSED_SUMS or input.shape[1] % 8 or addend.dtype != input.dtype or not input.is_cuda:
         return upsample_nearest2x(input) + addend
     return ops.replicate2x_add(input, addend, 1.0)
+
+
+# ---- image / video transformer blocks ------------------------------------------------------------------------------------
+# EXTENSIONS -- not part of the reference, whose one attention block is BigGAN/model.py:80-105.  Tokens lie in rows: an image
+# [B, C, H, W] in channels-last memory is x.permute(0, 2, 3, 1) = [B, H, W, C] without a copy.
+
+
+def block_input_norm(x, weight=None, bias=None, *, scale=None, shift=None, kind="rms", eps=1e-6):
+    """The norm in front of a transformer block: (norm(x) * weight + bias) * (1 + scale) + shift over the last dimension of
+    x [B, ..., C], fp32 or bf16, at most 8192 channels.  kind: "rms" (root mean square) or "layer" (mean and variance); eps is
+    added to the mean square / variance.  weight, bias: [C]; scale, shift (a condition's modulation): [C], or [B, C] for one per
+    sample; None leaves a part out.  Statistics and sums are fp32, the result is rounded once.  First-order gradients."""
+    return token_ops.block_norm("block_input_norm", x, None, None, None, None, 1.0, weight, bias, scale, shift, kind, eps, True)
+
+
+def block_output_norm(x, f, weight=None, bias=None, *, gate=None, residual_scale=1.0, kind="rms", eps=1e-6):
+    """The norm behind a transformer block, its gate and the residual sum: residual_scale * x + gate * (norm(f) * weight + bias)
+    for the residual stream x and the block's output f, both [B, ..., C].  gate: [C] or [B, C]; residual_scale: a number, or a
+    tensor of one element or [C].  Otherwise as block_input_norm."""
+    token_ops._require(f is not None, "block_output_norm: f must be a tensor")
+    return token_ops.block_norm("block_output_norm", x, f, weight, bias, gate, residual_scale, None, None, None, None, kind, eps, False)
+
+
+def block_boundary_norm(x, f, out_weight=None, in_weight=None, out_bias=None, in_bias=None, *, gate=None, residual_scale=1.0, scale=None,
+                        shift=None, kind="rms", eps=1e-6):
+    """The boundary between two transformer blocks as one sweep: y = block_output_norm(x, f, out_weight, out_bias, ...), the
+    residual stream behind the first, and h = block_input_norm(y, in_weight, in_bias, ...), what the second reads.  Returns
+    (y, h).  h is computed from y before y is rounded to its storage type."""
+    token_ops._require(f is not None, "block_boundary_norm: f must be a tensor")
+    return token_ops.block_norm("block_boundary_norm", x, f, out_weight, out_bias, gate, residual_scale, in_weight, in_bias, scale, shift, kind,
+                                eps, True)
+
+
+def rotary_table(dims, base=10000.0, interleaved=True, device=None):
+    """The frequencies of axial_rotary: dims[a] (even) elements of a head turn with axis a, pair i of them by base ** (-2 i /
+    dims[a]) radians per unit of position.  base: one number, or one per axis.  interleaved: a pair is two neighbouring elements;
+    otherwise pair p is (p, P + p) of the first 2 P elements.  Make it once per layer and device."""
+    return token_ops.rotary_table(dims, base, interleaved, device)
+
+
+def axial_rotary(q, k, positions, table):
+    """q [B, N, HQ, D] and k [B, N, HK, D] (or None) turned by their positions along several axes (time, height, width), in one
+    launch; returns (q, k), or q alone.  positions: [N, axes] shared by the samples or [B, N, axes], int32, int64, float32 or
+    float64 (angles are formed in fp64); table: rotary_table(...).  Elements of a head behind the table's pass through.  fp32 or
+    bf16.  Positions receive no gradient."""
+    return token_ops.axial_rotary(q, k, positions, table)
+
+
+def differential_attention(q, k, v, lam, *, scale=None, causal=False, key_lengths=None):
+    """(softmax(scale q1 k1^T) - lam softmax(scale q2 k2^T)) v without a [NQ, NK] matrix in memory: q [B, NQ, H, 2, d], k
+    [B, NK, HK, 2, d] (index 3: the two maps), v [B, NK, HK, dv], bf16; lam: [H], fp32 or bf16.  Returns [B, NQ, H, dv].  d: a multiple
+    of 8 up to 128, dv: up to 256; H a multiple of HK (head h reads keys h // (H // HK)).  scale: d ** -0.5 by default, positive.
+    key_lengths [B] (integers, clamped to 0 .. NK): keys from there on are not read at all.  causal: query i sees keys
+    j <= i + length - NQ, i.e. the queries are the last NQ positions of a sample; values at keys hidden this way must be finite.
+    A query without a visible key gives zeros and sends no gradient.  Single queries against long keys are split over the
+    keys.  Deterministic; first-order gradients for q, k, v and lam."""
+    return token_ops.differential_attention(q, k, v, lam, scale, causal, key_lengths)

@@ -532,6 +532,84 @@ size_t gc_attention_residual_workspace_bytes(int32_t B, int32_t N, int32_t C);
 int gc_attention_residual_bwd(const void* g, const void* mixed, const float* gamma, void* dmixed, float* dgamma, void* workspace,
                               size_t workspace_bytes, int32_t B, int32_t N, int32_t C, int32_t dtype, void* stream);
 
+/* ---- operators of image / video transformer blocks --------------------------------------------------------------------
+ * Extensions (the reference's only attention is BigGAN/model.py:80-105): tokens in rows, an image [B][H][W][C] being
+ * B samples of H * W rows. */
+
+/* The norms before and after a block, fused with the block's gate and the residual scale:
+ *   y = residual * x + gate * (norm(f) * out_weight + out_bias)                    where f is given
+ *   h = (norm(y) * in_weight + in_bias) * (1 + scale) + shift                      where with_input_norm is set (y = x without f)
+ * norm: over the cols channels of a row, root mean square (layer = 0) or mean and variance (layer = 1).  x, f: rows of cols
+ * contiguous elements with the given strides (elements); y, h, dy, dh, dx, df: contiguous [batch][rows][cols].  Every
+ * parameter is fp32, null for its neutral value, [cols] or (gate: gate_per_sample, scale and shift: mod_per_sample)
+ * [batch][cols]; residual_scale: null (residual_constant is used), one float, or residual_per_channel [cols].
+ * stats: [4][batch * rows] floats written by the forward pass if not null and read by the backward pass.
+ * Backward: any of dy, dh may be null (zero); writes dx, df and every d_* that is not null; the workspace holds partial sums,
+ * added in a fixed order.  cols <= 8192, batch <= 65535. */
+typedef struct gc_block_norm {
+  int64_t batch, rows;
+  int32_t cols, dtype, layer, with_input_norm;
+  float eps, residual_constant;
+  int32_t gate_per_sample, mod_per_sample, residual_per_channel, reserved;
+  int64_t x_batch_stride, x_row_stride, f_batch_stride, f_row_stride;
+  const void *x, *f;
+  const float *out_weight, *out_bias, *gate, *residual_scale, *in_weight, *in_bias, *scale, *shift;
+  void *y, *h;
+  float* stats;
+  const void *dy, *dh;
+  void *dx, *df;
+  float *d_out_weight, *d_out_bias, *d_gate, *d_residual_scale, *d_in_weight, *d_in_bias, *d_scale, *d_shift;
+} gc_block_norm;
+int gc_block_norm_fwd(const gc_block_norm* desc, void* stream);
+size_t gc_block_norm_workspace_bytes(int64_t batch, int64_t rows, int32_t cols);
+int gc_block_norm_bwd(const gc_block_norm* desc, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rotary positions with several axes.  Pair p of a head turns by 2 pi * positions[.., pair_axis[p]] * pair_turns[p]; pairs are
+ * neighbouring elements (2p, 2p + 1), or with `halves` (p, pairs + p); elements from 2 * pairs on are copied.
+ * q, k: [batch][tokens][heads][dim] with strides {batch, token, head} in elements, contiguous heads; k_heads = 0: q alone.
+ * q_out, k_out: contiguous.  positions: [tokens][axes], or [batch][tokens][axes] with positions_per_sample.  pair_turns (fp64)
+ * and pair_axis are device arrays of `pairs` entries.  inverse: the angles are negated (the backward pass). */
+typedef enum gc_position_dtype { GC_POS_I32 = 0, GC_POS_I64 = 1, GC_POS_F32 = 2, GC_POS_F64 = 3 } gc_position_dtype;
+typedef struct gc_rotary {
+  int64_t batch, tokens;
+  int32_t q_heads, k_heads, dim, pairs, axes, halves, dtype, position_dtype, positions_per_sample, inverse;
+  int64_t q_stride[3], k_stride[3];
+  const void *q, *k;
+  void *q_out, *k_out;
+  const void* positions;
+  const double* pair_turns;
+  const int32_t* pair_axis;
+} gc_rotary;
+int gc_axial_rotary(const gc_rotary* desc, void* stream);
+
+/* Differential attention: out_i = sum_j (p1_ij - lam p2_ij) v_j with pm_ij = softmax over the visible keys j of
+ * scale * <q_m,i , k_m,j>, m = 1, 2; lam: one fp32 number per head.  bf16 tensors: q [B][NQ][H][2][d], k [B][NK][HK][2][d],
+ * v [B][NK][HK][dv] with strides {batch, row, head(, map)} in elements (multiples of 8, contiguous innermost, 16-byte aligned),
+ * out / out2 / dout [B][NQ][H][dv], dq, dk, dv_out contiguous.  Heads of q share the keys of head h / (H / HK).
+ * Visible: j < key_lengths[b] (null: NK; clamped to 0 .. NK); with `causal` also j <= i + key_lengths[b] - NQ (the queries are
+ * the sample's last NQ positions).  A row without a visible key gives zeros and sends no gradient.  Keys behind a sample's
+ * length are never read.
+ * out2 (the second map's product with v) and lse [B][H][2][NQ] (log2 of the softmax denominators) may be null unless a backward pass
+ * follows.  d <= 128, dv <= 256, both multiples of 8.  Accumulation and statistics fp32, no atomics.
+ * Workspaces: gc_diff_attention_workspace_bytes(desc, backward); 0 bytes: may be null. */
+typedef struct gc_diff_attention {
+  int64_t q_stride[4], k_stride[4], v_stride[3];
+  int32_t B, NQ, NK, H, HK, d, dv, causal;
+  float scale;
+  int32_t reserved;
+  const void *q, *k, *v;
+  const float* lam;
+  const int32_t* key_lengths;
+  void *out, *out2;
+  float* lse;
+  const void* dout;
+  void *dq, *dk, *dv_out;
+  float* dlam;
+} gc_diff_attention;
+size_t gc_diff_attention_workspace_bytes(const gc_diff_attention* desc, int backward);
+int gc_diff_attention_fwd(const gc_diff_attention* desc, void* workspace, size_t workspace_bytes, void* stream);
+int gc_diff_attention_bwd(const gc_diff_attention* desc, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Split reductions.  A convolution whose output grid cannot fill the chip (few output pixels x channels, long
  * reduction) is split over several workgroups that add fp32 partial tiles into the zeroed output with atomics; the
  * order of those adds, and so the last bit of the result, varies from run to run.  gc_set_split_reduction(0) turns
