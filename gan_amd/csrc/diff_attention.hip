@@ -31,7 +31,6 @@ namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4_ptr;
-typedef __attribute__((address_space(3))) void* lds_ptr_t;
 
 constexpr int kRows = 128;                       // rows of a workgroup: 32 per wave
 constexpr int kBlk = 64;                         // rows staged per step
@@ -59,6 +58,16 @@ __device__ __forceinline__ bf16x8 pack8(const f32x16& v, int r0) {
   const u32x2 lo = cvt_bf16x4(f32x4{v[r0], v[r0 + 1], v[r0 + 2], v[r0 + 3]}), hi = cvt_bf16x4(f32x4{v[r0 + 4], v[r0 + 5], v[r0 + 6], v[r0 + 7]});
   return __builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], hi[0], hi[1]});
 }
+__device__ __forceinline__ bf16x8 pack8_sum(const f32x16& u, const f32x16& v, int r0) {
+  f32x4 a, b;
+#pragma unroll
+  for (int x = 0; x < 4; x++) {
+    a[x] = u[r0 + x] + v[r0 + x];
+    b[x] = u[r0 + 4 + x] + v[r0 + 4 + x];
+  }
+  const u32x2 lo = cvt_bf16x4(a), hi = cvt_bf16x4(b);
+  return __builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], hi[0], hi[1]});
+}
 // The two half-waves' values of a row, in both (v_permlane32_swap: one result holds the lower half's value, the other the upper's).
 // The results are copied to scalars first: a bit cast of a vector's element itself reads element 0.
 __device__ __forceinline__ void both_halves(float v, float& lo, float& hi) {
@@ -80,13 +89,15 @@ __device__ __forceinline__ float half_sum(float v) {
   return a + b;
 }
 
-// Chunk permutation of a tile row of ROWB bytes.  64 banks of 4 bytes: rows closer than 256 / ROWB apart never collide; among 16
-// rows at one chunk (row-wise reads) and 4 rows x 4 chunks (transposing reads) every 16-byte slot is used once.
-template <int ROWB>
+// Chunk permutations of a tile row of ROWB bytes (64 banks of 4 bytes: rows closer than 256 / ROWB apart never collide), by how the
+// tile is read: row-wise (16 rows at one chunk), transposed (4 rows x 4 chunks), or both ways.  Transposed reads of a tile that is
+// only read so depend on two bits of the row, which leaves their addresses to immediate offsets.
+enum Use { kRowWise, kTransposed, kBothWays };
+template <int ROWB, Use U>
 __device__ __forceinline__ int swz(int row) {
-  if (ROWB == 64) return (row >> 2) & 3;
-  if (ROWB == 128) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
-  return ((row & 3) << 2) | ((row >> 2) & 3);
+  if (U == kRowWise) return ROWB == 64 ? (row >> 2) & 3 : (ROWB == 128 ? (row >> 1) & 7 : row & 15);
+  if (U == kTransposed) return ROWB == 64 ? 0 : (ROWB == 128 ? ((row >> 1) & 1) << 2 : (row & 3) << 2);
+  return ROWB == 64 ? (row >> 2) & 3 : (ROWB == 128 ? (((row >> 1) & 1) << 2) | ((row >> 2) & 3) : ((row & 3) << 2) | ((row >> 2) & 3));
 }
 
 // Every load into LDS that this wave issued has landed, then the workgroup meets: the staged tile is complete and the other stage
@@ -96,10 +107,28 @@ __device__ __forceinline__ void tile_ready() {
   __syncthreads();
 }
 
-// One tile of 64 rows of `width` elements (padded to ROWB / 2 columns), from a tensor with row stride `stride` bytes.
-template <int ROWB>
+// 16 (or 4) bytes per lane from a buffer straight into LDS at `lds` + 16 (4) * lane.  Written in assembly because the compiler, which
+// cannot tell the stages apart, would wait for every such load in front of the next transposing LDS read.  No register receives
+// data; tile_ready() waits for the loads.
+typedef uint32_t u32x4s __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void load_to_lds16(u32x4s rsrc, uint32_t voff, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "memory");
+}
+__device__ __forceinline__ void load_to_lds4(u32x4s rsrc, uint32_t voff, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "memory");
+}
+// Raw buffer of `bytes` bytes at p (uniform): loads at or past its end return zeros
+__device__ __forceinline__ u32x4s buffer_at(const void* p, uint32_t bytes) {
+  const uint64_t a = reinterpret_cast<uint64_t>(p);
+  return u32x4s{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a), (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(a >> 32) & 0xffffu)),
+                (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
+}
+
+// One tile of ROWS rows of `width` elements (padded to ROWB / 2 columns), from a tensor with row stride `stride` bytes.
+template <int ROWB, Use U, int ROWS = kBlk>
 struct Loader {
-  static constexpr int CPR = ROWB / 16, RPI = 64 / CPR, NI = ROWB / 64, BASES = ROWB >= 512 ? 2 : 1;
+  static constexpr int CPR = ROWB / 16, RPI = 64 / CPR, NI = ROWS * ROWB / 4096, BASES = ROWB >= 512 ? 2 : 1;
+  static_assert(NI >= 1, "every wave loads part of a tile");
   uint32_t voff[BASES];
   uint32_t step;
   int wave;
@@ -107,41 +136,53 @@ struct Loader {
     wave = wave_;
 #pragma unroll
     for (int b = 0; b < BASES; b++) {
-      const int row = (wave + 4 * b) * RPI + lane / CPR, chunk = (lane % CPR) ^ swz<ROWB>(row);
+      const int row = (wave + 4 * b) * RPI + lane / CPR, chunk = (lane % CPR) ^ swz<ROWB, U>(row);
       voff[b] = chunk * 8 < width ? (uint32_t)row * stride + chunk * 16 : kOutOfRange;
     }
-    step = 4 * RPI * stride;
+    step = 4 * RPI * stride;                               // bytes between a wave's consecutive instructions
   }
-  // rows [row0, row0 + 64) of the tensor at `base`, of which those below `rows` exist
-  __device__ __forceinline__ void load(const uint16_t* base, int64_t row0, int64_t rows, uint32_t stride, int width, char* lds) const {
-    int64_t left = rows - row0;
-    left = left < 0 ? 0 : (left > kBlk ? kBlk : left);
+  // rows [row0, row0 + ROWS) of the tensor at `base`, of which those below `rows` exist, to LDS at `lds`.  The instructions' row offsets
+  // go into the (scalar) buffer base, so that one offset register serves all of them.
+  __device__ __forceinline__ void load(const uint16_t* base, int64_t row0, int64_t rows, uint32_t stride, int width, uint32_t lds) const {
+    const int64_t left = rows - row0;
+    const int n_rows = left < 0 ? 0 : (left > ROWS ? ROWS : (int)left);
     const char* p = reinterpret_cast<const char*>(base) + row0 * (int64_t)stride;
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, left > 0 ? (int)((left - 1) * stride + width * 2) : 0, 0x00020000);
+    const uint32_t bytes = n_rows > 0 ? (uint32_t)(n_rows - 1) * stride + width * 2 : 0u;
 #pragma unroll
-    for (int n = 0; n < NI; n++)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(lds + (wave + 4 * n) * 1024), 16, (int)(voff[n % BASES] + (uint32_t)(n - n % BASES) * step), 0, 0, 0);
+    for (int n = 0; n < NI; n += BASES) {
+      const uint32_t skip = (uint32_t)n * step;
+      const u32x4s rs = buffer_at(p + skip, bytes > skip ? bytes - skip : 0u);
+#pragma unroll
+      for (int b = 0; b < BASES; b++) load_to_lds16(rs, voff[b], lds + (wave + 4 * (n + b)) * 1024);
+    }
   }
 };
 
-// Row-wise A operand: rows r0 + lane % 32, columns 16 ks + 8 h + {0..7}
-template <int ROWB>
-__device__ __forceinline__ bf16x8 row_frag(const char* tile, int r0, int ks, int lane) {
-  const int row = lane & 31, h = lane >> 5;
-  return *reinterpret_cast<const bf16x8*>(tile + (r0 + row) * ROWB + (((2 * ks + h) ^ swz<ROWB>(row)) << 4));
-}
-// Transposed A operand: columns 32 cb + lane % 32, rows 16 t + {4 h + 0..3, 8 + 4 h + 0..3}
-template <int ROWB>
-__device__ __forceinline__ bf16x8 col_frag(const char* tile, int t, int cb, int lane) {
-  const int h = lane >> 5, rr = 4 * h + ((lane >> 2) & 3), chunk = cb * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), sub = (lane & 1) * 8;
-  const char* lo_p = tile + (16 * t + rr) * ROWB + ((chunk ^ swz<ROWB>(rr)) << 4) + sub;
-  const char* hi_p = tile + (16 * t + 8 + rr) * ROWB + ((chunk ^ swz<ROWB>(8 + rr)) << 4) + sub;
-  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)lo_p);
-  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)hi_p);
+typedef __attribute__((address_space(3))) const bf16x8* lds_bf16x8_ptr;
+__device__ __forceinline__ uint32_t lds_offset(const char* p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p; }
+__device__ __forceinline__ bf16x8 read_row(uint32_t addr) { return *(lds_bf16x8_ptr)(uintptr_t)addr; }
+__device__ __forceinline__ bf16x8 read_col(uint32_t lo_addr, uint32_t hi_addr) {
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(uintptr_t)lo_addr);
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(uintptr_t)hi_addr);
   typedef short s16x8 __attribute__((ext_vector_type(8)));
   const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   return __builtin_bit_cast(bf16x8, v);
 }
+// Address of this lane's chunk in row lane % 32 of a tile for k-step 0; k-step ks is at address ^ (ks << 5)
+template <int ROWB, Use U>
+__device__ __forceinline__ uint32_t row_addr(int lane) {
+  const int row = lane & 31, h = lane >> 5;
+  return row * ROWB + ((h ^ swz<ROWB, U>(row)) << 4);
+}
+// Address of this lane's 8 bytes of a transposing read of rows row0 .. row0 + 7 (4 per half-wave), columns 0 .. 31; column block cb is
+// at address ^ (cb << 6), the rows 8 further on at the same offset + 8 rows (read both ways: at that, with bit 5 flipped)
+template <int ROWB, Use U>
+__device__ __forceinline__ uint32_t col_addr(int lane, int row0) {
+  const int h = lane >> 5, rr = row0 + 4 * h + ((lane >> 2) & 3), chunk = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+  return rr * ROWB + ((chunk ^ swz<ROWB, U>(rr)) << 4) + (lane & 1) * 8;
+}
+template <int ROWB>
+__device__ __forceinline__ bf16x8 read_col_both(uint32_t lo_addr) { return read_col(lo_addr, (lo_addr ^ 32) + 8 * ROWB); }
 // 8 elements of a global row as a B operand; zero past the row's width
 __device__ __forceinline__ bf16x8 global_frag(const uint16_t* row, bool valid, int col, int width) {
   if (!valid || col >= width) return zero8();
@@ -172,7 +213,7 @@ template <int DK, int DV>
 __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_fwd_kernel(const DiffParams P) {
   typedef Cfg<DK, DV> F;
   constexpr int STAGE = 2 * F::KB + F::VB;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
   const gc_diff_attention& a = P.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   uint32_t lid = xcd_remap(blockIdx.x, gridDim.x);
@@ -216,86 +257,117 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_fwd_kerne
   const uint16_t* kbase = static_cast<const uint16_t*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[2];
   const uint16_t* vbase = static_cast<const uint16_t*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[2];
   const uint32_t kst = (uint32_t)(a.k_stride[1] * 2), vst = (uint32_t)(a.v_stride[1] * 2);
-  Loader<F::KROW> lk;
-  Loader<F::VROW> lv;
+  Loader<F::KROW, kRowWise> lk;
+  Loader<F::VROW, kTransposed> lv;
   lk.init(wave, lane, kst, a.d);
   lv.init(wave, lane, vst, a.dv);
-  auto fetch = [&](int blk, char* st) {
+  auto fetch = [&](int blk, uint32_t st) {
     lk.load(kbase, (int64_t)blk * kBlk, len, kst, a.d, st);
     lk.load(kbase + a.k_stride[3], (int64_t)blk * kBlk, len, kst, a.d, st + F::KB);
     lv.load(vbase, (int64_t)blk * kBlk, len, vst, a.dv, st + 2 * F::KB);
   };
 
+  const uint32_t base0 = lds_offset(smem);
+  const uint32_t kaddr = base0 + row_addr<F::KROW, kRowWise>(lane), vaddr = base0 + 2 * F::KB + col_addr<F::VROW, kTransposed>(lane, 0);
   const int nblk = (kend + kBlk - 1) / kBlk;
   const int blk0 = split * P.blocks_per_split, blk1 = min(nblk, blk0 + P.blocks_per_split);
-  if (blk0 < blk1) fetch(blk0, smem);
+  if (blk0 < blk1) fetch(blk0, base0);
   for (int blk = blk0; blk < blk1; blk++) {
     tile_ready();
-    if (blk + 1 < blk1) fetch(blk + 1, smem + ((blk + 1 - blk0) & 1) * STAGE);
-    const char* st = smem + ((blk - blk0) & 1) * STAGE;
-    const int j0 = blk * kBlk;
-    if (j0 >= wmax) continue;                              // (the whole wave; the barrier above is met by every wave in every step)
-    bf16x8 pb[2][4];
-#pragma unroll
-    for (int m = 0; m < 2; m++) {
+    if (blk + 1 < blk1) fetch(blk + 1, base0 + ((blk + 1 - blk0) & 1) * STAGE);
+    const uint32_t stage = ((blk - blk0) & 1) * STAGE;
+    // (the whole wave; the barrier above is met by every wave in every step)
+    if (blk * kBlk >= wmax) continue;
+#pragma unroll 1
+    for (int jb = 0; jb < 2; jb++) {
+      const int j0 = blk * kBlk + jb * 32;
+      const uint32_t ka = kaddr + stage + jb * 32 * F::KROW, va = vaddr + stage + jb * 32 * F::VROW;
+      // LDS reads are issued well in front of the matrix instructions that use them, all K fragments first, the first half of the V
+      // fragments in front of the exponentials; the fences keep the compiler from moving them back down
+      bf16x8 kf[2][F::KS], vf[F::VC];
       f32x16 s[2];
 #pragma unroll
-      for (int jb = 0; jb < 2; jb++) {
-        s[jb] = zero16();
+      for (int ks = 0; ks < F::KS; ks++)
 #pragma unroll
-        for (int ks = 0; ks < F::KS; ks++) s[jb] = mfma(row_frag<F::KROW>(st + m * F::KB, jb * 32, ks, lane), qf[m][ks], s[jb]);
+        for (int m = 0; m < 2; m++) kf[m][ks] = read_row((ka ^ (ks << 5)) + m * F::KB);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int ks = 0; ks < F::KS; ks++)
+#pragma unroll
+        for (int m = 0; m < 2; m++) s[m] = mfma(kf[m][ks], qf[m][ks], ks == 0 ? zero16() : s[m]);
+      if (j0 + 32 > wmin) {
+        const int room = lim - j0 - 4 * h;
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          s[0][e] = 8 * (e >> 2) + (e & 3) >= room ? -INFINITY : s[0][e];
+          s[1][e] = 8 * (e >> 2) + (e & 3) >= room ? -INFINITY : s[1][e];
+        }
       }
-      if (j0 + kBlk > wmin) {
+      float mx[2], top[2], base[2];
 #pragma unroll
-        for (int jb = 0; jb < 2; jb++)
+      for (int m = 0; m < 2; m++) {
+        mx[m] = -INFINITY;
 #pragma unroll
-          for (int e = 0; e < 16; e++)
-            if (j0 + jb * 32 + 8 * (e >> 2) + 4 * h + (e & 3) >= lim) s[jb][e] = -INFINITY;
+        for (int e = 0; e < 16; e += 2) mx[m] = fmaxf(fmaxf(s[m][e], s[m][e + 1]), mx[m]);
+        mx[m] = half_max(mx[m]);
       }
-      float mx = -INFINITY;
+      if (__builtin_amdgcn_ballot_w64(mx[0] > mrun[0] + P.lazy || mx[1] > mrun[1] + P.lazy) != 0) {
 #pragma unroll
-      for (int jb = 0; jb < 2; jb++)
+        for (int m = 0; m < 2; m++) {
+          const float mn = fmaxf(mrun[m], mx[m]);
+          const float alpha = __builtin_amdgcn_exp2f((mrun[m] - (mn == -INFINITY ? 0.f : mn)) * P.c2);
+          mrun[m] = mn;
+          lsum[m] *= alpha;
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) mx = fmaxf(fmaxf(s[jb][e], s[jb][e + 1]), mx);
-      mx = half_max(mx);
-      if (__builtin_amdgcn_ballot_w64(mx > mrun[m] + P.lazy) != 0) {
-        const float mn = fmaxf(mrun[m], mx);
-        const float alpha = __builtin_amdgcn_exp2f((mrun[m] - (mn == -INFINITY ? 0.f : mn)) * P.c2);
-        mrun[m] = mn;
-        lsum[m] *= alpha;
-#pragma unroll
-        for (int cb = 0; cb < F::VC; cb++) acc[m][cb] *= alpha;
-      }
-      const float top = mrun[m] == -INFINITY ? 0.f : mrun[m], base = top * P.c2;
-      // one multiply-add per score; its constant residue (2^-24 of base, the same for a whole row) cancels in the quotient unless it
-      // is itself an exponent to speak of, as with scores that stand for a mask's lowest value
-      if (__builtin_amdgcn_ballot_w64(fabsf(base) > kLargeScore) == 0) {
-#pragma unroll
-        for (int jb = 0; jb < 2; jb++)
-#pragma unroll
-          for (int e = 0; e < 16; e++) s[jb][e] = __builtin_amdgcn_exp2f(s[jb][e] * P.c2 - base);
-      } else {
-#pragma unroll
-        for (int jb = 0; jb < 2; jb++)
-#pragma unroll
-          for (int e = 0; e < 16; e++) s[jb][e] = __builtin_amdgcn_exp2f((s[jb][e] - top) * P.c2);
+          for (int cb = 0; cb < F::VC; cb++) acc[m][cb] *= alpha;
+        }
       }
 #pragma unroll
-      for (int jb = 0; jb < 2; jb++) {
+      for (int m = 0; m < 2; m++) {
+        top[m] = mrun[m] == -INFINITY ? 0.f : mrun[m];
+        base[m] = top[m] * P.c2;
+      }
+      // one multiply-add per score; its constant residue (2^-24 of base, the same for a whole row) cancels in the quotient unless
+      // it is itself an exponent to speak of, as with scores that stand for a mask's lowest value
+      if (__builtin_amdgcn_ballot_w64(fmaxf(fabsf(base[0]), fabsf(base[1])) > kLargeScore) != 0) {
 #pragma unroll
-        for (int e = 0; e < 16; e++) lsum[m] += s[jb][e];
-        pb[m][2 * jb] = pack8(s[jb], 0);
-        pb[m][2 * jb + 1] = pack8(s[jb], 8);
+        for (int m = 0; m < 2; m++) {
+#pragma unroll
+          for (int e = 0; e < 16; e++) s[m][e] -= top[m];
+          base[m] = 0.f;
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int cb = 0; cb < F::VC; cb++) vf[cb] = read_col(va ^ (cb << 6), (va ^ (cb << 6)) + 8 * F::VROW);
+      __builtin_amdgcn_sched_barrier(0);
+      bf16x8 pb[2][2];
+#pragma unroll
+      for (int m = 0; m < 2; m++) {
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          s[m][e] = __builtin_amdgcn_exp2f(s[m][e] * P.c2 - base[m]);
+          lsum[m] += s[m][e];
+        }
+        pb[m][0] = pack8(s[m], 0);
+        pb[m][1] = pack8(s[m], 8);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      bf16x8 vg[F::VC];
+#pragma unroll
+      for (int cb = 0; cb < F::VC; cb++) vg[cb] = read_col((va ^ (cb << 6)) + 16 * F::VROW, (va ^ (cb << 6)) + 24 * F::VROW);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int cb = 0; cb < F::VC; cb++) {
+        acc[0][cb] = mfma(vf[cb], pb[0][0], acc[0][cb]);
+        acc[1][cb] = mfma(vf[cb], pb[1][0], acc[1][cb]);
+      }
+#pragma unroll
+      for (int cb = 0; cb < F::VC; cb++) {
+        acc[0][cb] = mfma(vg[cb], pb[0][1], acc[0][cb]);
+        acc[1][cb] = mfma(vg[cb], pb[1][1], acc[1][cb]);
       }
     }
-#pragma unroll
-    for (int cb = 0; cb < F::VC; cb++)
-#pragma unroll
-      for (int t = 0; t < 4; t++) {
-        const bf16x8 va = col_frag<F::VROW>(st + 2 * F::KB, t, cb, lane);
-        acc[0][cb] = mfma(va, pb[0][t], acc[0][cb]);
-        acc[1][cb] = mfma(va, pb[1][t], acc[1][cb]);
-      }
   }
 
   lsum[0] = half_sum(lsum[0]);
@@ -423,7 +495,7 @@ template <int DK, int DV>
 __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dq_kernel(const DiffParams P) {
   typedef Cfg<DK, DV> F;
   constexpr int STAGE = 2 * F::KB + F::VB;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
   __shared__ float red[kThreads / 64];
   const gc_diff_attention& a = P.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
@@ -465,52 +537,61 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dq_ke
   const uint16_t* kbase = static_cast<const uint16_t*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[2];
   const uint16_t* vbase = static_cast<const uint16_t*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[2];
   const uint32_t kst = (uint32_t)(a.k_stride[1] * 2), vst = (uint32_t)(a.v_stride[1] * 2);
-  Loader<F::KROW> lk;
-  Loader<F::VROW> lv;
+  Loader<F::KROW, kBothWays> lk;
+  Loader<F::VROW, kRowWise> lv;
   lk.init(wave, lane, kst, a.d);
   lv.init(wave, lane, vst, a.dv);
-  auto fetch = [&](int blk, char* st) {
+  auto fetch = [&](int blk, uint32_t st) {
     lk.load(kbase, (int64_t)blk * kBlk, len, kst, a.d, st);
     lk.load(kbase + a.k_stride[3], (int64_t)blk * kBlk, len, kst, a.d, st + F::KB);
     lv.load(vbase, (int64_t)blk * kBlk, len, vst, a.dv, st + 2 * F::KB);
   };
+  const uint32_t base0 = lds_offset(smem);
+  const uint32_t kra = base0 + row_addr<F::KROW, kBothWays>(lane), kca = base0 + col_addr<F::KROW, kBothWays>(lane, 0);
+  const uint32_t vra = base0 + 2 * F::KB + row_addr<F::VROW, kRowWise>(lane);
   const int nblk = (kend + kBlk - 1) / kBlk;
-  if (nblk > 0) fetch(0, smem);
+  if (nblk > 0) fetch(0, base0);
   for (int blk = 0; blk < nblk; blk++) {
     tile_ready();
-    if (blk + 1 < nblk) fetch(blk + 1, smem + ((blk + 1) & 1) * STAGE);
-    const char* st = smem + (blk & 1) * STAGE;
-    const int j0 = blk * kBlk;
-    if (j0 >= wmax) continue;
-    const bool masked = j0 + kBlk > wmin;
-#pragma unroll
+    if (blk + 1 < nblk) fetch(blk + 1, base0 + ((blk + 1) & 1) * STAGE);
+    const uint32_t stage = (blk & 1) * STAGE;
+    if (blk * kBlk >= wmax) continue;
+#pragma unroll 1
     for (int jb = 0; jb < 2; jb++) {
+      const int j0 = blk * kBlk + jb * 32;
+      const uint32_t ka = kra + stage + jb * 32 * F::KROW, va = vra + stage + jb * 32 * F::VROW, kc = kca + stage + jb * 32 * F::KROW;
       f32x16 s[2], dp = zero16();
 #pragma unroll
       for (int m = 0; m < 2; m++) {
         s[m] = zero16();
 #pragma unroll
-        for (int ks = 0; ks < F::KS; ks++) s[m] = mfma(row_frag<F::KROW>(st + m * F::KB, jb * 32, ks, lane), qf[m][ks], s[m]);
+        for (int ks = 0; ks < F::KS; ks++) s[m] = mfma(read_row((ka ^ (ks << 5)) + m * F::KB), qf[m][ks], s[m]);
       }
 #pragma unroll
-      for (int ks = 0; ks < F::VS; ks++) dp = mfma(row_frag<F::VROW>(st + 2 * F::KB, jb * 32, ks, lane), gf[ks], dp);
+      for (int ks = 0; ks < F::VS; ks++) dp = mfma(read_row(va ^ (ks << 5)), gf[ks], dp);
+      if (j0 + 32 > wmin) {
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          const bool hidden = 8 * (e >> 2) + (e & 3) >= lim - j0 - 4 * h;
+          s[0][e] = hidden ? -INFINITY : s[0][e];
+          s[1][e] = hidden ? -INFINITY : s[1][e];
+        }
+      }
 #pragma unroll
       for (int e = 0; e < 16; e++) {
-        float p0 = __builtin_amdgcn_exp2f(s[0][e] * P.c2 - L[0]), p1 = __builtin_amdgcn_exp2f(s[1][e] * P.c2 - L[1]);
-        if (masked && j0 + jb * 32 + 8 * (e >> 2) + 4 * h + (e & 3) >= lim) { p0 = 0.f; p1 = 0.f; }
+        const float p0 = __builtin_amdgcn_exp2f(s[0][e] * P.c2 - L[0]), p1 = __builtin_amdgcn_exp2f(s[1][e] * P.c2 - L[1]);
         s[0][e] = p0 * (dp[e] - D[0]);
         s[1][e] = p1 * (dp[e] - D[1]);
         left += s[1][e];
       }
 #pragma unroll
-      for (int m = 0; m < 2; m++) {
-        const bf16x8 d0 = pack8(s[m], 0), d1 = pack8(s[m], 8);
+      for (int m = 0; m < 2; m++)
 #pragma unroll
-        for (int cb = 0; cb < F::KC; cb++) {
-          acc[m][cb] = mfma(col_frag<F::KROW>(st + m * F::KB, 2 * jb, cb, lane), d0, acc[m][cb]);
-          acc[m][cb] = mfma(col_frag<F::KROW>(st + m * F::KB, 2 * jb + 1, cb, lane), d1, acc[m][cb]);
+        for (int t = 0; t < 2; t++) {
+          const bf16x8 d = pack8(s[m], 8 * t);
+#pragma unroll
+          for (int cb = 0; cb < F::KC; cb++) acc[m][cb] = mfma(read_col_both<F::KROW>((kc ^ (cb << 6)) + m * F::KB + t * 16 * F::KROW), d, acc[m][cb]);
         }
-      }
     }
   }
   const float lam = a.lam[head];
@@ -557,31 +638,48 @@ __global__ __launch_bounds__(kThreads) void diff_dlam_kernel(const DiffParams P)
 }
 
 // Owner: 128 keys of a key head; walks the queries of every head that shares them.  Produces dK and dV.  OUT: 1 dK, 2 dV, 3 both
-// (both accumulators of the widest form do not fit the register file: it runs as two launches).
+// (both accumulators of the widest form do not fit the register file: it runs as two launches).  VLDS: the owned values, an operand of
+// dP, stay in LDS instead of registers, and the queries are staged 32 rows at a time to make room: with 64 keys' worth of accumulators
+// per wave that is what lets two waves share a SIMD without spilling.
 template <int DK, int DV, int OUT>
-__global__ __launch_bounds__(kThreads, (DV > 64 ? 1 : 2)) void diff_bwd_dkv_kernel(const DiffParams P) {
+struct DkvCfg {
+  static constexpr bool VLDS = DV == 128 && (OUT & 1);
+  static constexpr int ROWS = VLDS ? 32 : kBlk, KB = ROWS * DK * 2, VB = ROWS * DV * 2;
+  static constexpr int STAGE = 2 * KB + VB + 4 * kBlk * 4;                  // with L1, L2, delta1, delta2 of the staged queries
+  static constexpr int LDS = 2 * STAGE + (VLDS ? kRows * DV * 2 : 0);
+};
+template <int DK, int DV, int OUT>
+__global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dkv_kernel(const DiffParams P) {
   typedef Cfg<DK, DV> F;
-  constexpr int VECB = 4 * kBlk * 4;                       // L1, L2, delta1, delta2 of the staged queries
-  constexpr int STAGE = 2 * F::KB + F::VB + VECB;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+  typedef DkvCfg<DK, DV, OUT> X;
+  constexpr int ROWS = X::ROWS, STAGE = X::STAGE;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
   const gc_diff_attention& a = P.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const uint32_t lid = xcd_remap(blockIdx.x, gridDim.x);
   const int tile = (int)(lid % (uint32_t)P.tiles), bh = (int)(lid / (uint32_t)P.tiles), b = bh / a.HK, hk = bh - b * a.HK;
   const int len = sample_length(a, b), j0 = tile * kRows, w0 = j0 + wave * 32, j = w0 + (lane & 31);
-  const bool exists = j < a.NK, valid = j < len;
+  const bool valid = j < len;
 
   const int jc = valid ? j : 0;
-  const uint16_t* krow = static_cast<const uint16_t*>(a.k) + b * a.k_stride[0] + jc * a.k_stride[1] + hk * a.k_stride[2];
-  const uint16_t* vrow = static_cast<const uint16_t*>(a.v) + b * a.v_stride[0] + jc * a.v_stride[1] + hk * a.v_stride[2];
-  bf16x8 kf[2][F::KS], vf[F::VS];
+  const uint16_t* kbase = static_cast<const uint16_t*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[2];
+  const uint16_t* vbase = static_cast<const uint16_t*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[2];
+  const uint32_t base0 = lds_offset(smem);
+  bf16x8 kf[2][F::KS], vf[X::VLDS ? 1 : F::VS];
 #pragma unroll
   for (int m = 0; m < 2; m++)
 #pragma unroll
-    for (int ks = 0; ks < F::KS; ks++) kf[m][ks] = global_frag(krow + m * a.k_stride[3], valid, ks * 16 + 8 * h, a.d);
-  if (OUT & 1)
+    for (int ks = 0; ks < F::KS; ks++) kf[m][ks] = global_frag(kbase + jc * a.k_stride[1] + m * a.k_stride[3], valid, ks * 16 + 8 * h, a.d);
+  if (X::VLDS) {
+    Loader<F::VROW, kRowWise> lv;
+    const uint32_t vst = (uint32_t)(a.v_stride[1] * 2);
+    lv.init(wave, lane, vst, a.dv);
 #pragma unroll
-    for (int ks = 0; ks < F::VS; ks++) vf[ks] = global_frag(vrow, valid, ks * 16 + 8 * h, a.dv);
+    for (int x = 0; x < kRows / kBlk; x++) lv.load(vbase, (int64_t)j0 + x * kBlk, len, vst, a.dv, base0 + 2 * STAGE + x * kBlk * F::VROW);
+  } else if (OUT & 1) {
+#pragma unroll
+    for (int ks = 0; ks < F::VS; ks++) vf[ks] = global_frag(vbase + jc * a.v_stride[1], valid, ks * 16 + 8 * h, a.dv);
+  }
 
   f32x16 adk[2][F::KC], adv[F::VC];
 #pragma unroll
@@ -590,87 +688,103 @@ __global__ __launch_bounds__(kThreads, (DV > 64 ? 1 : 2)) void diff_bwd_dkv_kern
   for (int cb = 0; cb < F::VC; cb++) adv[cb] = zero16();
 
   const uint32_t qst = (uint32_t)(a.q_stride[1] * 2), gst = (uint32_t)a.H * a.dv * 2;
-  Loader<F::KROW> lq;
-  Loader<F::VROW> lg;
+  Loader<F::KROW, kBothWays, ROWS> lq;
+  Loader<F::VROW, kBothWays, ROWS> lg;
   lq.init(wave, lane, qst, a.d);
   lg.init(wave, lane, gst, a.dv);
   // first query that sees key j: i >= j + NQ - len
   const int shift = a.causal ? a.NQ - len : -a.NK - 1;
-  const int imin = j + shift;                              // this lane's (this key's) first query
-  const int first = max(0, (j0 + shift) / kBlk), nblk = (a.NQ + kBlk - 1) / kBlk;
-  const int per_head = j0 < len && nblk > first ? nblk - first : 0, steps = per_head * P.G;
-  auto fetch = [&](int step, char* st) {
-    const int g = step / per_head, blk = first + step - g * per_head, head = hk * P.G + g;
+  const int first = max(0, (j0 + shift) / ROWS), nblk = j0 < len ? (a.NQ + ROWS - 1) / ROWS : 0;
+  // staged step: query block `blk` of the group's head `g`
+  auto fetch = [&](int g, int blk, uint32_t st) {
+    const int head = hk * P.G + g;
     const uint16_t* q = static_cast<const uint16_t*>(a.q) + b * a.q_stride[0] + head * a.q_stride[2];
     const uint16_t* go = static_cast<const uint16_t*>(a.dout) + ((size_t)b * a.NQ * a.H + head) * a.dv;
-    lq.load(q, (int64_t)blk * kBlk, a.NQ, qst, a.d, st);
-    lq.load(q + a.q_stride[3], (int64_t)blk * kBlk, a.NQ, qst, a.d, st + F::KB);
-    lg.load(go, (int64_t)blk * kBlk, a.NQ, gst, a.dv, st + 2 * F::KB);
-    // wave 0, 1: L of the two maps; 2, 3: delta.  64 floats, zeros past the last query
-    const float* v = (wave < 2 ? a.lse : P.delta) + ((size_t)(b * a.H + head) * 2 + (wave & 1)) * a.NQ + (int64_t)blk * kBlk;
-    const int left = min(kBlk, a.NQ - blk * kBlk);
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(v), 0, left * 4, 0x00020000);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(st + 2 * F::KB + F::VB + wave * kBlk * 4), 4, lane * 4, 0, 0, 0);
+    lq.load(q, (int64_t)blk * ROWS, a.NQ, qst, a.d, st);
+    lq.load(q + a.q_stride[3], (int64_t)blk * ROWS, a.NQ, qst, a.d, st + X::KB);
+    lg.load(go, (int64_t)blk * ROWS, a.NQ, gst, a.dv, st + 2 * X::KB);
+    // wave 0, 1: L of the two maps; 2, 3: delta.  ROWS floats, then zeros (also past the last query), 64 in all
+    const float* v = (wave < 2 ? a.lse : P.delta) + ((size_t)(b * a.H + head) * 2 + (wave & 1)) * a.NQ + (int64_t)blk * ROWS;
+    load_to_lds4(buffer_at(v, min(ROWS, a.NQ - blk * ROWS) * 4), lane * 4, st + 2 * X::KB + X::VB + wave * kBlk * 4);
   };
-  if (steps > 0) fetch(0, smem);
-  for (int step = 0; step < steps; step++) {
+  const uint32_t qra = base0 + row_addr<F::KROW, kBothWays>(lane), qca = base0 + col_addr<F::KROW, kBothWays>(lane, 0);
+  const uint32_t gra = base0 + 2 * X::KB + row_addr<F::VROW, kBothWays>(lane), gca = base0 + 2 * X::KB + col_addr<F::VROW, kBothWays>(lane, 0);
+  const uint32_t vra = base0 + 2 * STAGE + wave * 32 * F::VROW + row_addr<F::VROW, kRowWise>(lane);
+  int g = 0, blk = first, odd = 0;
+  if (first < nblk) fetch(0, first, base0);
+  while (first < nblk && g < P.G) {
+    const float nlam = -a.lam[hk * P.G + g];               // (asked for in front of the next step's loads, which it would wait for)
     tile_ready();
-    if (step + 1 < steps) fetch(step + 1, smem + ((step + 1) & 1) * STAGE);
-    const char* st = smem + (step & 1) * STAGE;
-    const float* vec = reinterpret_cast<const float*>(st + 2 * F::KB + F::VB);
-    const int g = step / per_head, i0 = (first + step - g * per_head) * kBlk;
-    const float nlam = -a.lam[hk * P.G + g];
-    if (i0 + kBlk - 1 < w0 + shift) continue;              // no query of the block sees a key of this wave
-    const bool masked = i0 < w0 + 31 + shift;
-#pragma unroll
-    for (int ib = 0; ib < 2; ib++) {
-      f32x16 s[2], dp = zero16();
+    const int i_blk = blk * ROWS;
+    if (++blk == nblk) { blk = first; g++; }
+    if (g < P.G) fetch(g, blk, base0 + (odd ^ 1) * STAGE);
+    const uint32_t stage = odd * STAGE;
+    odd ^= 1;
+    if (i_blk + ROWS - 1 < w0 + shift) continue;           // no query of the block sees a key of this wave
+#pragma unroll 1
+    for (int ib = 0; ib < ROWS / 32; ib++) {
+      const int i0 = i_blk + ib * 32;
+      const uint32_t qr = qra + stage + ib * 32 * F::KROW, qc = qca + stage + ib * 32 * F::KROW;
+      const uint32_t gr = gra + stage + ib * 32 * F::VROW, gc = gca + stage + ib * 32 * F::VROW;
+      const float* vec = reinterpret_cast<const float*>(smem + stage + 2 * X::KB + X::VB) + ib * 32 + 4 * h;
+      // the order keeps few values alive at once: scores and probabilities, their mix and dV, then dP, the score gradients and dK
+      f32x16 s[2];
 #pragma unroll
       for (int m = 0; m < 2; m++) {
         s[m] = zero16();
 #pragma unroll
-        for (int ks = 0; ks < F::KS; ks++) s[m] = mfma(row_frag<F::KROW>(st + m * F::KB, ib * 32, ks, lane), kf[m][ks], s[m]);
+        for (int ks = 0; ks < F::KS; ks++) s[m] = mfma(read_row((qr ^ (ks << 5)) + m * X::KB), kf[m][ks], s[m]);
       }
-      if (OUT & 1)
+      if (i0 < w0 + 31 + shift) {
+        const int hidden = w0 + (lane & 31) + shift - i0 - 4 * h;      // this lane's key is seen from there on
 #pragma unroll
-        for (int ks = 0; ks < F::VS; ks++) dp = mfma(row_frag<F::VROW>(st + 2 * F::KB, ib * 32, ks, lane), vf[ks], dp);
-      f32x16 mix;
+        for (int e = 0; e < 16; e++) {
+          s[0][e] = 8 * (e >> 2) + (e & 3) < hidden ? -INFINITY : s[0][e];
+          s[1][e] = 8 * (e >> 2) + (e & 3) < hidden ? -INFINITY : s[1][e];
+        }
+      }
 #pragma unroll
       for (int e4 = 0; e4 < 4; e4++) {
-        const int o = ib * 32 + 8 * e4 + 4 * h;
-        const f32x4 L0 = *reinterpret_cast<const f32x4*>(vec + o), L1 = *reinterpret_cast<const f32x4*>(vec + kBlk + o);
-        const f32x4 D0 = *reinterpret_cast<const f32x4*>(vec + 2 * kBlk + o), D1 = *reinterpret_cast<const f32x4*>(vec + 3 * kBlk + o);
+        const f32x4 L0 = *reinterpret_cast<const f32x4*>(vec + 8 * e4), L1 = *reinterpret_cast<const f32x4*>(vec + kBlk + 8 * e4);
 #pragma unroll
         for (int x = 0; x < 4; x++) {
-          const int e = 4 * e4 + x;
-          float p0 = __builtin_amdgcn_exp2f(s[0][e] * P.c2 - L0[x]), p1 = __builtin_amdgcn_exp2f(s[1][e] * P.c2 - L1[x]);
-          if (masked && i0 + o + x < imin) { p0 = 0.f; p1 = 0.f; }
-          p1 *= nlam;
-          mix[e] = p0 + p1;
-          s[0][e] = p0 * (dp[e] - D0[x]);
-          s[1][e] = p1 * (dp[e] - D1[x]);
+          s[0][4 * e4 + x] = __builtin_amdgcn_exp2f(s[0][4 * e4 + x] * P.c2 - L0[x]);
+          s[1][4 * e4 + x] = __builtin_amdgcn_exp2f(s[1][4 * e4 + x] * P.c2 - L1[x]) * nlam;
         }
       }
       if (OUT & 2) {
-        const bf16x8 m0 = pack8(mix, 0), m1 = pack8(mix, 8);
 #pragma unroll
-        for (int cb = 0; cb < F::VC; cb++) {
-          adv[cb] = mfma(col_frag<F::VROW>(st + 2 * F::KB, 2 * ib, cb, lane), m0, adv[cb]);
-          adv[cb] = mfma(col_frag<F::VROW>(st + 2 * F::KB, 2 * ib + 1, cb, lane), m1, adv[cb]);
+        for (int t = 0; t < 2; t++) {
+          const bf16x8 d = pack8_sum(s[0], s[1], 8 * t);
+#pragma unroll
+          for (int cb = 0; cb < F::VC; cb++) adv[cb] = mfma(read_col_both<F::VROW>((gc ^ (cb << 6)) + t * 16 * F::VROW), d, adv[cb]);
         }
       }
+      if (OUT & 1) {
+        f32x16 dp = zero16();
 #pragma unroll
-      for (int m = 0; m < ((OUT & 1) ? 2 : 0); m++) {
-        const bf16x8 d0 = pack8(s[m], 0), d1 = pack8(s[m], 8);
+        for (int ks = 0; ks < F::VS; ks++) dp = mfma(read_row(gr ^ (ks << 5)), X::VLDS ? read_row(vra ^ (ks << 5)) : vf[X::VLDS ? 0 : ks], dp);
 #pragma unroll
-        for (int cb = 0; cb < F::KC; cb++) {
-          adk[m][cb] = mfma(col_frag<F::KROW>(st + m * F::KB, 2 * ib, cb, lane), d0, adk[m][cb]);
-          adk[m][cb] = mfma(col_frag<F::KROW>(st + m * F::KB, 2 * ib + 1, cb, lane), d1, adk[m][cb]);
+        for (int e4 = 0; e4 < 4; e4++) {
+          const f32x4 D0 = *reinterpret_cast<const f32x4*>(vec + 2 * kBlk + 8 * e4), D1 = *reinterpret_cast<const f32x4*>(vec + 3 * kBlk + 8 * e4);
+#pragma unroll
+          for (int x = 0; x < 4; x++) {
+            s[0][4 * e4 + x] *= dp[4 * e4 + x] - D0[x];
+            s[1][4 * e4 + x] *= dp[4 * e4 + x] - D1[x];
+          }
         }
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+#pragma unroll
+          for (int t = 0; t < 2; t++) {
+            const bf16x8 d = pack8(s[m], 8 * t);
+#pragma unroll
+            for (int cb = 0; cb < F::KC; cb++) adk[m][cb] = mfma(read_col_both<F::KROW>((qc ^ (cb << 6)) + m * X::KB + t * 16 * F::KROW), d, adk[m][cb]);
+          }
       }
     }
   }
-  if (!exists) return;
+  if (j >= a.NK) return;
   // keys behind the sample's length: zeros (their columns hold whatever the zero-filled operands gave)
   uint16_t* dk = static_cast<uint16_t*>(a.dk) + ((size_t)(b * (size_t)a.NK + j) * a.HK + hk) * 2 * a.d;
   uint16_t* dv = static_cast<uint16_t*>(a.dv_out) + ((size_t)(b * (size_t)a.NK + j) * a.HK + hk) * a.dv;
@@ -789,7 +903,7 @@ int launch_dq(const DiffParams& P, hipStream_t s) {
 template <int DK, int DV, int OUT>
 int launch_dkv(const DiffParams& P, hipStream_t s) {
   typedef Cfg<DK, DV> F;
-  constexpr int lds = 2 * (2 * F::KB + F::VB + 4 * kBlk * 4);
+  constexpr int lds = DkvCfg<DK, DV, OUT>::LDS;
   if (int e = ensure_dynamic_smem(reinterpret_cast<const void*>(diff_bwd_dkv_kernel<DK, DV, OUT>), lds)) return e;
   hipLaunchKernelGGL((diff_bwd_dkv_kernel<DK, DV, OUT>), dim3((unsigned)P.a.B * P.a.HK * P.tiles), dim3(kThreads), lds, s, P);
   return check_hip(hipGetLastError(), "diff_bwd_dkv launch");
