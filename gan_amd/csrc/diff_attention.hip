@@ -40,7 +40,7 @@ constexpr float kLargeScore = 1048576.f;         // log2 units
 
 struct DiffParams {
   gc_diff_attention a;
-  int G, tiles, nsplit, blocks_per_split;
+  int G, tiles, nsplit, blocks_per_split, few;     // few: at most 32 rows per key head (diff_few_rows_kernel; shares in tiles of 32 keys)
   FastDiv div_nq;
   float c2, lazy;                                // scale * log2(e); kLazy in units of a score
   float *part, *ml, *delta, *lampart;
@@ -125,10 +125,11 @@ __device__ __forceinline__ u32x4s buffer_at(const void* p, uint32_t bytes) {
 }
 
 // One tile of ROWS rows of `width` elements (padded to ROWB / 2 columns), from a tensor with row stride `stride` bytes.
-template <int ROWB, Use U, int ROWS = kBlk>
+template <int ROWB, Use U, int ROWS = kBlk, int NW = kThreads / 64>
 struct Loader {
-  static constexpr int CPR = ROWB / 16, RPI = 64 / CPR, NI = ROWS * ROWB / 4096, BASES = ROWB >= 512 ? 2 : 1;
-  static_assert(NI >= 1, "every wave loads part of a tile");
+  // a wave's instructions repeat their chunk permutation every 16 rows: BASES of them differ
+  static constexpr int CPR = ROWB / 16, RPI = 64 / CPR, NI = ROWS * ROWB / (1024 * NW), BASES = RPI * NW >= 16 ? 1 : 16 / (RPI * NW);
+  static_assert(NI >= 1 && NI % BASES == 0, "every wave loads whole periods of a tile");
   uint32_t voff[BASES];
   uint32_t step;
   int wave;
@@ -136,10 +137,10 @@ struct Loader {
     wave = wave_;
 #pragma unroll
     for (int b = 0; b < BASES; b++) {
-      const int row = (wave + 4 * b) * RPI + lane / CPR, chunk = (lane % CPR) ^ swz<ROWB, U>(row);
+      const int row = (wave + NW * b) * RPI + lane / CPR, chunk = (lane % CPR) ^ swz<ROWB, U>(row);
       voff[b] = chunk * 8 < width ? (uint32_t)row * stride + chunk * 16 : kOutOfRange;
     }
-    step = 4 * RPI * stride;                               // bytes between a wave's consecutive instructions
+    step = NW * RPI * stride;                              // bytes between a wave's consecutive instructions
   }
   // rows [row0, row0 + ROWS) of the tensor at `base`, of which those below `rows` exist, to LDS at `lds`.  The instructions' row offsets
   // go into the (scalar) buffer base, so that one offset register serves all of them.
@@ -153,7 +154,7 @@ struct Loader {
       const uint32_t skip = (uint32_t)n * step;
       const u32x4s rs = buffer_at(p + skip, bytes > skip ? bytes - skip : 0u);
 #pragma unroll
-      for (int b = 0; b < BASES; b++) load_to_lds16(rs, voff[b], lds + (wave + 4 * (n + b)) * 1024);
+      for (int b = 0; b < BASES; b++) load_to_lds16(rs, voff[b], lds + (wave + NW * (n + b)) * 1024);
     }
   }
 };
@@ -200,12 +201,97 @@ __device__ __forceinline__ int visible(const gc_diff_attention& a, int i, int le
   return a.causal ? (n < 0 ? 0 : (n < len ? n : len)) : len;
 }
 
+// Which (sample and head, tile, share) a workgroup owns.  Workgroup n runs on XCD n % 8, each with an L2 of its own: an XCD gets a
+// contiguous run of the work, so that the workgroups that walk one head's keys (queries) at the same time meet in one L2.  Causal
+// tiles differ in length.  `runs` runs of tiles from short to long (the heads of a group) follow each other in a head's tiles, or, with
+// runs = 0, one run from long to short.  Where every XCD gets whole runs, they go one after the other, long tiles first; otherwise the
+// longest tiles of all heads start first on all XCDs (16 heads, 4 key heads, N 8192: 455 against 508 us forward).
+struct WorkId { int bh, tile, share; };
+__device__ __forceinline__ WorkId work_id(const DiffParams& P, uint32_t heads, uint32_t runs) {
+  const uint32_t n = P.nsplit, T = P.tiles;
+  if (!P.a.causal) {
+    const uint32_t lid = xcd_remap(blockIdx.x, gridDim.x);
+    return WorkId{(int)(lid / n / T), (int)(lid / n % T), (int)(lid % n)};
+  }
+  if (runs == 0) return WorkId{(int)(blockIdx.x % (heads * n) / n), (int)(blockIdx.x / (heads * n)), (int)(blockIdx.x % n)};
+  if (T % runs != 0) runs = 1;
+  const uint32_t per = T / runs;
+  if (heads * runs % 8 == 0) {
+    const uint32_t lid = xcd_remap(blockIdx.x, gridDim.x), t = lid / n % T;
+    return WorkId{(int)(lid / n / T), (int)(t - t % per + per - 1 - t % per), (int)(lid % n)};
+  }
+  const uint32_t in = blockIdx.x % (heads * n), t = blockIdx.x / (heads * n);
+  return WorkId{(int)(in / n), (int)((t % runs) * per + per - 1 - t / runs), (int)(in % n)};
+}
+
 template <int DK, int DV>
 struct Cfg {
   static constexpr int KROW = DK * 2, VROW = DV * 2, KB = kBlk * KROW, VB = kBlk * VROW;
   static constexpr int KS = DK / 16, VS = DV / 16, KC = DK / 32, VC = DV / 32;
   static constexpr int WAVES = DV > 128 ? 1 : 2;      // per SIMD: the accumulators of the widest form take the registers of two
 };
+
+// One step of the running softmax of both maps over 32 keys: masks (room: this lane's first hidden key, relative to its first), moves
+// the running maxima, and leaves s[m] and base[m] so that the exponential of a score is exp2(s c2 - base).
+template <int VC>
+__device__ __forceinline__ void softmax_step(f32x16 (&s)[2], f32x16 (&acc)[2][VC], float (&mrun)[2], float (&lsum)[2], float (&base)[2], bool masked,
+                                             int room, float c2, float lazy) {
+  if (masked) {
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+      s[0][e] = 8 * (e >> 2) + (e & 3) >= room ? -INFINITY : s[0][e];
+      s[1][e] = 8 * (e >> 2) + (e & 3) >= room ? -INFINITY : s[1][e];
+    }
+  }
+  float mx[2], top[2];
+#pragma unroll
+  for (int m = 0; m < 2; m++) {
+    mx[m] = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) mx[m] = fmaxf(fmaxf(s[m][e], s[m][e + 1]), mx[m]);
+    mx[m] = half_max(mx[m]);
+  }
+  if (__builtin_amdgcn_ballot_w64(mx[0] > mrun[0] + lazy || mx[1] > mrun[1] + lazy) != 0) {
+#pragma unroll
+    for (int m = 0; m < 2; m++) {
+      const float mn = fmaxf(mrun[m], mx[m]);
+      const float alpha = __builtin_amdgcn_exp2f((mrun[m] - (mn == -INFINITY ? 0.f : mn)) * c2);
+      mrun[m] = mn;
+      lsum[m] *= alpha;
+#pragma unroll
+      for (int cb = 0; cb < VC; cb++) acc[m][cb] *= alpha;
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < 2; m++) {
+    top[m] = mrun[m] == -INFINITY ? 0.f : mrun[m];
+    base[m] = top[m] * c2;
+  }
+  // one multiply-add per score; its constant residue (2^-24 of base, the same for a whole row) cancels in the quotient unless it is
+  // itself an exponent to speak of, as with scores that stand for a mask's lowest value
+  if (__builtin_amdgcn_ballot_w64(fmaxf(fabsf(base[0]), fabsf(base[1])) > kLargeScore) != 0) {
+#pragma unroll
+    for (int m = 0; m < 2; m++) {
+#pragma unroll
+      for (int e = 0; e < 16; e++) s[m][e] -= top[m];
+      base[m] = 0.f;
+    }
+  }
+}
+
+// A row's share of the keys, for the joining kernel: running maxima, sums and unnormalised accumulators
+template <int VC>
+__device__ __forceinline__ void store_share(const DiffParams& P, size_t row, int h, const f32x16 (&acc)[2][VC], const float (&mrun)[2], const float (&lsum)[2]) {
+  if (h == 0) *reinterpret_cast<f32x4*>(P.ml + row * 4) = f32x4{mrun[0], lsum[0], mrun[1], lsum[1]};
+#pragma unroll
+  for (int m = 0; m < 2; m++)
+#pragma unroll
+    for (int cb = 0; cb < VC; cb++)
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        *reinterpret_cast<f32x4*>(P.part + (row * 2 + m) * (VC * 32) + cb * 32 + 8 * e + 4 * h) =
+            f32x4{acc[m][cb][4 * e], acc[m][cb][4 * e + 1], acc[m][cb][4 * e + 2], acc[m][cb][4 * e + 3]};
+}
 
 // ---------------------------------------------------------------------------------------------------------------------------
 // Rows of a workgroup: 128 of the G * NQ rows (head of the group, query) that share a key head.
@@ -216,12 +302,8 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_fwd_kerne
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const gc_diff_attention& a = P.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-  uint32_t lid = xcd_remap(blockIdx.x, gridDim.x);
-  const int split = (int)(lid % (uint32_t)P.nsplit);
-  lid /= (uint32_t)P.nsplit;
-  int tile = (int)(lid % (uint32_t)P.tiles);
-  const int bh = (int)(lid / (uint32_t)P.tiles), b = bh / a.HK, hk = bh - b * a.HK;
-  if (a.causal) tile = P.tiles - 1 - tile;                 // the longest rows first
+  const WorkId id = work_id(P, (uint32_t)a.B * a.HK, (uint32_t)P.G);
+  const int split = id.share, tile = id.tile, bh = id.bh, b = bh / a.HK, hk = bh - b * a.HK;
   const int R = P.G * a.NQ, len = sample_length(a, b);
   const int r0 = tile * kRows, w0 = r0 + wave * 32, r = w0 + (lane & 31);
   const bool valid = r < R;
@@ -295,48 +377,8 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_fwd_kerne
       for (int ks = 0; ks < F::KS; ks++)
 #pragma unroll
         for (int m = 0; m < 2; m++) s[m] = mfma(kf[m][ks], qf[m][ks], ks == 0 ? zero16() : s[m]);
-      if (j0 + 32 > wmin) {
-        const int room = lim - j0 - 4 * h;
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-          s[0][e] = 8 * (e >> 2) + (e & 3) >= room ? -INFINITY : s[0][e];
-          s[1][e] = 8 * (e >> 2) + (e & 3) >= room ? -INFINITY : s[1][e];
-        }
-      }
-      float mx[2], top[2], base[2];
-#pragma unroll
-      for (int m = 0; m < 2; m++) {
-        mx[m] = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) mx[m] = fmaxf(fmaxf(s[m][e], s[m][e + 1]), mx[m]);
-        mx[m] = half_max(mx[m]);
-      }
-      if (__builtin_amdgcn_ballot_w64(mx[0] > mrun[0] + P.lazy || mx[1] > mrun[1] + P.lazy) != 0) {
-#pragma unroll
-        for (int m = 0; m < 2; m++) {
-          const float mn = fmaxf(mrun[m], mx[m]);
-          const float alpha = __builtin_amdgcn_exp2f((mrun[m] - (mn == -INFINITY ? 0.f : mn)) * P.c2);
-          mrun[m] = mn;
-          lsum[m] *= alpha;
-#pragma unroll
-          for (int cb = 0; cb < F::VC; cb++) acc[m][cb] *= alpha;
-        }
-      }
-#pragma unroll
-      for (int m = 0; m < 2; m++) {
-        top[m] = mrun[m] == -INFINITY ? 0.f : mrun[m];
-        base[m] = top[m] * P.c2;
-      }
-      // one multiply-add per score; its constant residue (2^-24 of base, the same for a whole row) cancels in the quotient unless
-      // it is itself an exponent to speak of, as with scores that stand for a mask's lowest value
-      if (__builtin_amdgcn_ballot_w64(fmaxf(fabsf(base[0]), fabsf(base[1])) > kLargeScore) != 0) {
-#pragma unroll
-        for (int m = 0; m < 2; m++) {
-#pragma unroll
-          for (int e = 0; e < 16; e++) s[m][e] -= top[m];
-          base[m] = 0.f;
-        }
-      }
+      float base[2];
+      softmax_step<F::VC>(s, acc, mrun, lsum, base, j0 + 32 > wmin, lim - j0 - 4 * h, P.c2, P.lazy);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int cb = 0; cb < F::VC; cb++) vf[cb] = read_col(va ^ (cb << 6), (va ^ (cb << 6)) + 8 * F::VROW);
@@ -374,18 +416,7 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_fwd_kerne
   lsum[1] = half_sum(lsum[1]);
   if (!valid) return;
   if (P.nsplit > 1) {
-    const size_t row = ((size_t)split * a.B * a.HK + bh) * R + r;
-    float* ml = P.ml + row * 4;
-    if (h == 0) *reinterpret_cast<f32x4*>(ml) = f32x4{mrun[0], lsum[0], mrun[1], lsum[1]};
-#pragma unroll
-    for (int m = 0; m < 2; m++)
-      if (lsum[m] != 0.f)                                  // an empty share is not read by the joining kernel
-#pragma unroll
-        for (int cb = 0; cb < F::VC; cb++)
-#pragma unroll
-          for (int e = 0; e < 4; e++)
-            *reinterpret_cast<f32x4*>(P.part + (row * 2 + m) * DV + cb * 32 + 8 * e + 4 * h) =
-                f32x4{acc[m][cb][4 * e], acc[m][cb][4 * e + 1], acc[m][cb][4 * e + 2], acc[m][cb][4 * e + 3]};
+    store_share<F::VC>(P, ((size_t)split * a.B * a.HK + bh) * R + r, h, acc, mrun, lsum);
     return;
   }
   const float inv0 = lsum[0] != 0.f ? 1.f / lsum[0] : 0.f, inv1 = lsum[1] != 0.f ? 1.f / lsum[1] : 0.f, lam = a.lam[head];
@@ -412,49 +443,189 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_fwd_kerne
   }
 }
 
-// Joins the shares of a row that was split over the keys: one wave per row, lanes along the value columns.
-__global__ __launch_bounds__(kThreads) void diff_join_kernel(const DiffParams P, int DV) {
-  const gc_diff_attention& a = P.a;
-  const int R = P.G * a.NQ, lane = threadIdx.x & 63;
-  const int64_t idx = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
-  const size_t rows = (size_t)a.B * a.HK * R;
-  if ((size_t)idx >= rows) return;
-  const int bh = (int)(idx / R), r = (int)(idx - (int64_t)bh * R), b = bh / a.HK, hk = bh - b * a.HK;
-  const int g = r / a.NQ, i = r - g * a.NQ, head = hk * P.G + g;
-  float M[2] = {-INFINITY, -INFINITY}, L[2] = {0.f, 0.f};
-  for (int s = 0; s < P.nsplit; s++) {
-    const float* ml = P.ml + ((size_t)s * rows + idx) * 4;
-    for (int m = 0; m < 2; m++) if (ml[2 * m + 1] != 0.f) M[m] = fmaxf(M[m], ml[2 * m]);
-  }
-  float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-  for (int s = 0; s < P.nsplit; s++) {
-    const size_t row = (size_t)s * rows + idx;
-    const float* ml = P.ml + row * 4;
-    for (int m = 0; m < 2; m++) {
-      if (ml[2 * m + 1] == 0.f) continue;
-      const float w = __builtin_amdgcn_exp2f((ml[2 * m] - M[m]) * P.c2);
-      L[m] += w * ml[2 * m + 1];
-      const float* src = P.part + (row * 2 + m) * DV;
-#pragma unroll
-      for (int x = 0; x < 4; x++)
-        if (lane + 64 * x < a.dv) acc[m][x] += w * src[lane + 64 * x];
-    }
-  }
-  const float inv0 = L[0] != 0.f ? 1.f / L[0] : 0.f, inv1 = L[1] != 0.f ? 1.f / L[1] : 0.f, lam = a.lam[head];
-  const size_t orow = (((size_t)b * a.NQ + i) * a.H + head) * a.dv;
+// At most 32 rows per key head (single queries and short runs of them against long keys): bound by reading the keys and values once.
+// Every wave walks a share of the keys of its own in tiles of 32, staged privately (no barriers; the loads of the next tile are in
+// flight while one is worked on), so that a CU keeps 64 KiB of loads under way; the shares are joined by diff_join_kernel.  The matrix
+// instructions are idle most of the time here, which pays for probabilities held to 16 bits: their bf16 rounding and its remainder
+// are multiplied with the values separately.
+template <int DK, int DV>
+struct FewCfg {
+  static constexpr int NW = DV > 128 ? 2 : 4;              // waves
+  static constexpr int KB = 32 * DK * 2, VB = 32 * DV * 2, STAGE = 2 * KB + VB, LOADS = STAGE / 1024;
+};
+template <int N>
+__device__ __forceinline__ void wait_loads() {             // all but the N youngest loads of this wave have landed
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+}
+__device__ __forceinline__ bf16x8 pack8_rest(const f32x16& v, int r0, bf16x8 hi) {
+  const u32x4 b = __builtin_bit_cast(u32x4, hi);
+  f32x16 d;
 #pragma unroll
   for (int x = 0; x < 4; x++) {
-    const int c = lane + 64 * x;
-    if (c >= a.dv) continue;
-    const float o2 = acc[1][x] * inv1;
-    static_cast<uint16_t*>(a.out)[orow + c] = float_to_bf16_bits(acc[0][x] * inv0 - lam * o2);
-    if (a.out2 != nullptr) static_cast<uint16_t*>(a.out2)[orow + c] = float_to_bf16_bits(o2);
+    d[2 * x] = v[r0 + 2 * x] - __builtin_bit_cast(float, b[x] << 16);
+    d[2 * x + 1] = v[r0 + 2 * x + 1] - __builtin_bit_cast(float, b[x] & 0xffff0000u);
   }
-  if (a.lse != nullptr && lane == 0) {
-    float* l = a.lse + ((size_t)b * a.H + head) * 2 * a.NQ + i;
-    l[0] = L[0] != 0.f ? M[0] * P.c2 + __log2f(L[0]) : INFINITY;
-    l[a.NQ] = L[1] != 0.f ? M[1] * P.c2 + __log2f(L[1]) : INFINITY;
+  return pack8(d, 0);
+}
+template <int DK, int DV>
+__global__ __launch_bounds__((FewCfg<DK, DV>::NW * 64), 1) void diff_few_rows_kernel(const DiffParams P) {
+  typedef Cfg<DK, DV> F;
+  typedef FewCfg<DK, DV> X;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const gc_diff_attention& a = P.a;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), h = lane >> 5;
+  const int bh = (int)(blockIdx.x / ((uint32_t)P.nsplit / X::NW)), share = (int)(blockIdx.x % ((uint32_t)P.nsplit / X::NW)) * X::NW + wave;
+  const int b = bh / a.HK, hk = bh - b * a.HK, R = P.G * a.NQ, len = sample_length(a, b), r = lane & 31;
+  const bool valid = r < R;
+  const int rc = valid ? r : R - 1, g = (int)fd_div((uint32_t)rc, P.div_nq), i = rc - g * a.NQ, head = hk * P.G + g;
+  const int lim = visible(a, i, len), wmin = visible(a, 0, len), wmax = visible(a, a.NQ - 1, len);
+
+  const uint16_t* qrow = static_cast<const uint16_t*>(a.q) + b * a.q_stride[0] + i * a.q_stride[1] + head * a.q_stride[2];
+  bf16x8 qf[2][F::KS];
+#pragma unroll
+  for (int m = 0; m < 2; m++)
+#pragma unroll
+    for (int ks = 0; ks < F::KS; ks++) qf[m][ks] = global_frag(qrow + m * a.q_stride[3], valid, ks * 16 + 8 * h, a.d);
+  f32x16 acc[2][F::VC];
+  float mrun[2] = {-INFINITY, -INFINITY}, lsum[2] = {0.f, 0.f};
+#pragma unroll
+  for (int m = 0; m < 2; m++)
+#pragma unroll
+    for (int cb = 0; cb < F::VC; cb++) acc[m][cb] = zero16();
+
+  const uint16_t* kbase = static_cast<const uint16_t*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[2];
+  const uint16_t* vbase = static_cast<const uint16_t*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[2];
+  const uint32_t kst = (uint32_t)(a.k_stride[1] * 2), vst = (uint32_t)(a.v_stride[1] * 2);
+  Loader<F::KROW, kRowWise, 32, 1> lk;
+  Loader<F::VROW, kTransposed, 32, 1> lv;
+  lk.init(0, lane, kst, a.d);
+  lv.init(0, lane, vst, a.dv);
+  auto fetch = [&](int t, int rows, uint32_t st) {
+    lk.load(kbase, (int64_t)t * 32, rows, kst, a.d, st);
+    lk.load(kbase + a.k_stride[3], (int64_t)t * 32, rows, kst, a.d, st + X::KB);
+    lv.load(vbase, (int64_t)t * 32, rows, vst, a.dv, st + 2 * X::KB);
+  };
+  const uint32_t base0 = lds_offset(smem) + wave * 2 * X::STAGE;
+  const uint32_t kaddr = base0 + row_addr<F::KROW, kRowWise>(lane), vaddr = base0 + 2 * X::KB + col_addr<F::VROW, kTransposed>(lane, 0);
+  const int t0 = share * P.blocks_per_split, t1 = min((wmax + 31) / 32, t0 + P.blocks_per_split);
+  if (t0 < t1) fetch(t0, len, base0);
+  for (int t = t0; t < t1; t++) {
+    // (behind the last tile: loads of no rows, which read nothing; the count of loads in flight stays the same)
+    fetch(t + 1, t + 1 < t1 ? len : 0, base0 + ((t + 1 - t0) & 1) * X::STAGE);
+    wait_loads<X::LOADS>();
+    const int j0 = t * 32;
+    const uint32_t ka = kaddr + ((t - t0) & 1) * X::STAGE, va = vaddr + ((t - t0) & 1) * X::STAGE;
+    f32x16 s[2];
+#pragma unroll
+    for (int ks = 0; ks < F::KS; ks++)
+#pragma unroll
+      for (int m = 0; m < 2; m++) s[m] = mfma(read_row((ka ^ (ks << 5)) + m * X::KB), qf[m][ks], ks == 0 ? zero16() : s[m]);
+    float base[2];
+    softmax_step<F::VC>(s, acc, mrun, lsum, base, j0 + 32 > wmin, lim - j0 - 4 * h, P.c2, P.lazy);
+    bf16x8 hi[2][2], lo[2][2];
+#pragma unroll
+    for (int m = 0; m < 2; m++) {
+#pragma unroll
+      for (int e = 0; e < 16; e++) {
+        s[m][e] = __builtin_amdgcn_exp2f(s[m][e] * P.c2 - base[m]);
+        lsum[m] += s[m][e];
+      }
+#pragma unroll
+      for (int x = 0; x < 2; x++) {
+        hi[m][x] = pack8(s[m], 8 * x);
+        lo[m][x] = pack8_rest(s[m], 8 * x, hi[m][x]);
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < 2; x++)
+#pragma unroll
+      for (int cb = 0; cb < F::VC; cb++) {
+        const uint32_t y = (va ^ (cb << 6)) + x * 16 * F::VROW;
+        const bf16x8 vf = read_col(y, y + 8 * F::VROW);
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+          acc[m][cb] = mfma(vf, hi[m][x], acc[m][cb]);
+          acc[m][cb] = mfma(vf, lo[m][x], acc[m][cb]);
+        }
+      }
   }
+  wait_loads<0>();                                         // (nothing of this wave is still writing LDS when the workgroup ends)
+  lsum[0] = half_sum(lsum[0]);
+  lsum[1] = half_sum(lsum[1]);
+  if (valid) store_share<F::VC>(P, ((size_t)share * a.B * a.HK + bh) * R + r, h, acc, mrun, lsum);
+}
+
+// Joins the shares of a row that was split over the keys: one workgroup per row.  The shares' weights are worked out first (a thread
+// per share), then every thread adds one value column of one map over every 4th or 8th share, all its loads independent: latency is
+// what this kernel is made of.
+constexpr int kMaxShares = 512, kJoinThreads = 1024;
+__global__ __launch_bounds__(kJoinThreads) void diff_join_kernel(const DiffParams P, int DV) {
+  __shared__ float wt[2][kMaxShares], red[4][kMaxShares / 64], cols[kJoinThreads];
+  const gc_diff_attention& a = P.a;
+  const int R = P.G * a.NQ, tid = threadIdx.x;
+  const int64_t idx = blockIdx.x;
+  const size_t rows = (size_t)a.B * a.HK * R;
+  const int bh = (int)(idx / R), r = (int)(idx - (int64_t)bh * R), b = bh / a.HK, hk = bh - b * a.HK;
+  const int g = r / a.NQ, i = r - g * a.NQ, head = hk * P.G + g;
+  float top[2] = {-INFINITY, -INFINITY}, own[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  if (tid < P.nsplit) {
+    const f32x4 ml = *reinterpret_cast<const f32x4*>(P.ml + ((size_t)tid * rows + idx) * 4);
+#pragma unroll
+    for (int m = 0; m < 2; m++) {
+      own[m] = ml[2 * m];
+      l[m] = ml[2 * m + 1];
+      if (l[m] != 0.f) top[m] = own[m];
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < 2; m++) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top[m] = fmaxf(top[m], __shfl_xor(top[m], o, 64));
+    if (tid < kMaxShares && (tid & 63) == 0) red[m][tid >> 6] = top[m];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int m = 0; m < 2; m++) {
+#pragma unroll
+    for (int w = 0; w < kMaxShares / 64; w++) top[m] = fmaxf(top[m], red[m][w]);
+    // an empty share has no weight; a sum that is not a number has to reach the result
+    const float w = l[m] == 0.f ? 0.f : (l[m] != l[m] ? l[m] : __builtin_amdgcn_exp2f((own[m] - top[m]) * P.c2));
+    if (tid < P.nsplit) wt[m][tid] = w;
+    float t = l[m] == 0.f ? 0.f : w * l[m];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
+    if (tid < kMaxShares && (tid & 63) == 0) red[2 + m][tid >> 6] = t;
+  }
+  __syncthreads();
+  float L[2] = {0.f, 0.f};
+#pragma unroll
+  for (int m = 0; m < 2; m++)
+#pragma unroll
+    for (int w = 0; w < kMaxShares / 64; w++) L[m] += red[2 + m][w];
+  const float inv0 = L[0] != 0.f ? 1.f / L[0] : 0.f, inv1 = L[1] != 0.f ? 1.f / L[1] : 0.f, lam = a.lam[head];
+  const size_t orow = (((size_t)b * a.NQ + i) * a.H + head) * a.dv;
+  const int width = DV < 128 ? DV : 128, per = 2 * width, groups = kJoinThreads / per, grp = tid / per, m = (tid % per) / width;
+  for (int c0 = 0; c0 < a.dv; c0 += width) {
+    const float* src = P.part + ((size_t)idx * 2 + m) * DV + c0 + tid % width;
+    float acc = 0.f;
+#pragma unroll 16
+    for (int s = grp; s < P.nsplit; s += groups) acc += wt[m][s] * src[(size_t)s * rows * 2 * DV];
+    cols[tid] = acc;
+    __syncthreads();
+    const int c = c0 + tid;
+    if (tid < width && c < a.dv) {
+      float t[2] = {0.f, 0.f};
+      for (int q = 0; q < groups; q++)
+#pragma unroll
+        for (int x = 0; x < 2; x++) t[x] += cols[q * per + x * width + tid];
+      const float o2 = t[1] * inv1;
+      static_cast<uint16_t*>(a.out)[orow + c] = float_to_bf16_bits(t[0] * inv0 - lam * o2);
+      if (a.out2 != nullptr) static_cast<uint16_t*>(a.out2)[orow + c] = float_to_bf16_bits(o2);
+    }
+    __syncthreads();
+  }
+  if (a.lse != nullptr && tid < 2)
+    a.lse[((size_t)b * a.H + head) * 2 * a.NQ + (size_t)tid * a.NQ + i] = (tid == 0 ? L[0] : L[1]) != 0.f ? (tid == 0 ? top[0] : top[1]) * P.c2 + __log2f(tid == 0 ? L[0] : L[1]) : INFINITY;
 }
 
 // delta [B][H][2][NQ]: dO . O1 = dO . out + lam dO . O2, and dO . O2; 16 lanes per row
@@ -499,10 +670,8 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dq_ke
   __shared__ float red[kThreads / 64];
   const gc_diff_attention& a = P.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-  const uint32_t lid = xcd_remap(blockIdx.x, gridDim.x);
-  int tile = (int)(lid % (uint32_t)P.tiles);
-  const int bh = (int)(lid / (uint32_t)P.tiles), b = bh / a.H, head = bh - b * a.H, hk = head / P.G;
-  if (a.causal) tile = P.tiles - 1 - tile;
+  const WorkId id = work_id(P, (uint32_t)a.B * a.H, 1);
+  const int share = id.share, tile = id.tile, bh = id.bh, b = bh / a.H, head = bh - b * a.H, hk = head / P.G;
   const int len = sample_length(a, b), r0 = tile * kRows, w0 = r0 + wave * 32, r = w0 + (lane & 31);
   const bool valid = r < a.NQ;
   const int i = valid ? r : a.NQ - 1, lim = visible(a, i, len);
@@ -549,12 +718,12 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dq_ke
   const uint32_t base0 = lds_offset(smem);
   const uint32_t kra = base0 + row_addr<F::KROW, kBothWays>(lane), kca = base0 + col_addr<F::KROW, kBothWays>(lane, 0);
   const uint32_t vra = base0 + 2 * F::KB + row_addr<F::VROW, kRowWise>(lane);
-  const int nblk = (kend + kBlk - 1) / kBlk;
-  if (nblk > 0) fetch(0, base0);
-  for (int blk = 0; blk < nblk; blk++) {
+  const int blk0 = share * P.blocks_per_split, blk1 = min((kend + kBlk - 1) / kBlk, blk0 + P.blocks_per_split);
+  if (blk0 < blk1) fetch(blk0, base0);
+  for (int blk = blk0; blk < blk1; blk++) {
     tile_ready();
-    if (blk + 1 < nblk) fetch(blk + 1, base0 + ((blk + 1) & 1) * STAGE);
-    const uint32_t stage = (blk & 1) * STAGE;
+    if (blk + 1 < blk1) fetch(blk + 1, base0 + ((blk + 1 - blk0) & 1) * STAGE);
+    const uint32_t stage = ((blk - blk0) & 1) * STAGE;
     if (blk * kBlk >= wmax) continue;
 #pragma unroll 1
     for (int jb = 0; jb < 2; jb++) {
@@ -597,7 +766,9 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dq_ke
   const float lam = a.lam[head];
   if (valid) {
     const float f[2] = {a.scale, -lam * a.scale};
-    uint16_t* dst = static_cast<uint16_t*>(a.dq) + (((size_t)b * a.NQ + i) * a.H + head) * 2 * a.d;
+    const size_t row = (((size_t)b * a.NQ + i) * a.H + head) * 2 * a.d;
+    uint16_t* dst = static_cast<uint16_t*>(a.dq) + row;
+    float* part = P.part + (size_t)share * a.B * a.NQ * a.H * 2 * a.d + row;
 #pragma unroll
     for (int m = 0; m < 2; m++)
 #pragma unroll
@@ -606,27 +777,28 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dq_ke
         for (int e = 0; e < 4; e++) {
           const int c = cb * 32 + 8 * e + 4 * h;
           if (c >= a.d) continue;
-          *reinterpret_cast<u32x2*>(dst + m * a.d + c) = cvt_bf16x4(f32x4{acc[m][cb][4 * e] * f[m], acc[m][cb][4 * e + 1] * f[m], acc[m][cb][4 * e + 2] * f[m],
-                                                                       acc[m][cb][4 * e + 3] * f[m]});
+          const f32x4 v = {acc[m][cb][4 * e] * f[m], acc[m][cb][4 * e + 1] * f[m], acc[m][cb][4 * e + 2] * f[m], acc[m][cb][4 * e + 3] * f[m]};
+          if (P.nsplit > 1) *reinterpret_cast<f32x4*>(part + m * a.d + c) = v;
+          else *reinterpret_cast<u32x2*>(dst + m * a.d + c) = cvt_bf16x4(v);
         }
   }
-  float t = valid ? left + (h == 0 ? D[1] : 0.f) : 0.f;
+  float t = valid ? left + (h == 0 && share == 0 ? D[1] : 0.f) : 0.f;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
   if (lane == 0) red[wave] = t;
   __syncthreads();
-  if (tid == 0) P.lampart[(size_t)bh * P.tiles + tile] = ((red[0] + red[1]) + red[2]) + red[3];
+  if (tid == 0) P.lampart[((size_t)bh * P.tiles + tile) * P.nsplit + share] = ((red[0] + red[1]) + red[2]) + red[3];
 }
 
 // dlam[head] = -(the workgroups' shares, added in a fixed order); one workgroup per head
 __global__ __launch_bounds__(kThreads) void diff_dlam_kernel(const DiffParams P) {
   __shared__ float red[kThreads];
   const int head = blockIdx.x;
-  const int64_t n = (int64_t)P.a.B * P.tiles;
+  const int64_t per = (int64_t)P.tiles * P.nsplit, n = P.a.B * per;
   float s = 0.f;
   for (int64_t i = threadIdx.x; i < n; i += kThreads) {
-    const int64_t b = i / P.tiles, t = i - b * P.tiles;
-    s += P.lampart[(b * P.a.H + head) * P.tiles + t];
+    const int64_t b = i / per, t = i - b * per;
+    s += P.lampart[(b * P.a.H + head) * per + t];
   }
   red[threadIdx.x] = s;
   __syncthreads();
@@ -635,6 +807,24 @@ __global__ __launch_bounds__(kThreads) void diff_dlam_kernel(const DiffParams P)
     for (int i = 0; i < kThreads; i++) t += red[i];
     P.a.dlam[head] = -t;
   }
+}
+
+// out = the sum of `shares` fp32 partial results, added in order; two tensors back to back in part: [shares][n0], [shares][n1]
+__global__ __launch_bounds__(kThreads) void diff_sum_kernel(const float* part, int shares, uint16_t* out0, size_t n0, uint16_t* out1, size_t n1) {
+  size_t i = ((size_t)blockIdx.x * kThreads + threadIdx.x) * 4, n = n0;
+  const float* src = part;
+  uint16_t* out = out0;
+  if (i >= n0) {
+    src += (size_t)shares * n0;
+    i -= n0;
+    n = n1;
+    out = out1;
+  }
+  if (i >= n) return;
+  f32x4 t = *reinterpret_cast<const f32x4*>(src + i);
+#pragma unroll 4
+  for (int s = 1; s < shares; s++) t += *reinterpret_cast<const f32x4*>(src + (size_t)s * n + i);
+  *reinterpret_cast<u32x2*>(out + i) = cvt_bf16x4(t);
 }
 
 // Owner: 128 keys of a key head; walks the queries of every head that shares them.  Produces dK and dV.  OUT: 1 dK, 2 dV, 3 both
@@ -656,8 +846,8 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dkv_k
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const gc_diff_attention& a = P.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-  const uint32_t lid = xcd_remap(blockIdx.x, gridDim.x);
-  const int tile = (int)(lid % (uint32_t)P.tiles), bh = (int)(lid / (uint32_t)P.tiles), b = bh / a.HK, hk = bh - b * a.HK;
+  const WorkId id = work_id(P, (uint32_t)a.B * a.HK, 0);
+  const int share = id.share, tile = id.tile, bh = id.bh, b = bh / a.HK, hk = bh - b * a.HK;
   const int len = sample_length(a, b), j0 = tile * kRows, w0 = j0 + wave * 32, j = w0 + (lane & 31);
   const bool valid = j < len;
 
@@ -710,14 +900,17 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dkv_k
   const uint32_t qra = base0 + row_addr<F::KROW, kBothWays>(lane), qca = base0 + col_addr<F::KROW, kBothWays>(lane, 0);
   const uint32_t gra = base0 + 2 * X::KB + row_addr<F::VROW, kBothWays>(lane), gca = base0 + 2 * X::KB + col_addr<F::VROW, kBothWays>(lane, 0);
   const uint32_t vra = base0 + 2 * STAGE + wave * 32 * F::VROW + row_addr<F::VROW, kRowWise>(lane);
-  int g = 0, blk = first, odd = 0;
-  if (first < nblk) fetch(0, first, base0);
-  while (first < nblk && g < P.G) {
+  // this workgroup's share of the (head, block) steps
+  const int per_head = nblk > first ? nblk - first : 0, steps = per_head * P.G;
+  const int step0 = (int)((int64_t)steps * share / P.nsplit), step1 = (int)((int64_t)steps * (share + 1) / P.nsplit);
+  int g = per_head > 0 ? step0 / per_head : 0, blk = first + step0 - g * per_head, odd = 0;
+  if (step0 < step1) fetch(g, blk, base0);
+  for (int step = step0; step < step1; step++) {
     const float nlam = -a.lam[hk * P.G + g];               // (asked for in front of the next step's loads, which it would wait for)
     tile_ready();
     const int i_blk = blk * ROWS;
     if (++blk == nblk) { blk = first; g++; }
-    if (g < P.G) fetch(g, blk, base0 + (odd ^ 1) * STAGE);
+    if (step + 1 < step1) fetch(g, blk, base0 + (odd ^ 1) * STAGE);
     const uint32_t stage = odd * STAGE;
     odd ^= 1;
     if (i_blk + ROWS - 1 < w0 + shift) continue;           // no query of the block sees a key of this wave
@@ -786,27 +979,27 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dkv_k
   }
   if (j >= a.NK) return;
   // keys behind the sample's length: zeros (their columns hold whatever the zero-filled operands gave)
-  uint16_t* dk = static_cast<uint16_t*>(a.dk) + ((size_t)(b * (size_t)a.NK + j) * a.HK + hk) * 2 * a.d;
-  uint16_t* dv = static_cast<uint16_t*>(a.dv_out) + ((size_t)(b * (size_t)a.NK + j) * a.HK + hk) * a.dv;
-  const u32x2 none = {0u, 0u};
+  const size_t key = ((size_t)b * a.NK + j) * a.HK + hk, keys = (size_t)a.B * a.NK * a.HK;
+  auto put = [&](void* out, float* part, int c, const f32x16& v, int e, float f) {
+    f32x4 x = {v[4 * e] * f, v[4 * e + 1] * f, v[4 * e + 2] * f, v[4 * e + 3] * f};
+    if (!valid) x = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (P.nsplit > 1) *reinterpret_cast<f32x4*>(part + c) = x;
+    else *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(out) + c) = cvt_bf16x4(x);
+  };
+  uint16_t* dk = static_cast<uint16_t*>(a.dk) + key * 2 * a.d;
+  uint16_t* dv = static_cast<uint16_t*>(a.dv_out) + key * a.dv;
+  float* pk = P.part + ((size_t)share * keys + key) * 2 * a.d;
+  float* pv = P.part + (size_t)P.nsplit * keys * 2 * a.d + ((size_t)share * keys + key) * a.dv;
 #pragma unroll
   for (int e = 0; e < 4; e++) {
 #pragma unroll
     for (int m = 0; m < ((OUT & 1) ? 2 : 0); m++)
 #pragma unroll
-      for (int cb = 0; cb < F::KC; cb++) {
-        const int c = cb * 32 + 8 * e + 4 * h;
-        const f32x16& v = adk[m][cb];
-        if (c < a.d)
-          *reinterpret_cast<u32x2*>(dk + m * a.d + c) =
-              valid ? cvt_bf16x4(f32x4{v[4 * e] * a.scale, v[4 * e + 1] * a.scale, v[4 * e + 2] * a.scale, v[4 * e + 3] * a.scale}) : none;
-      }
+      for (int cb = 0; cb < F::KC; cb++)
+        if (cb * 32 + 8 * e + 4 * h < a.d) put(dk + m * a.d, pk + m * a.d, cb * 32 + 8 * e + 4 * h, adk[m][cb], e, a.scale);
 #pragma unroll
-    for (int cb = 0; cb < ((OUT & 2) ? F::VC : 0); cb++) {
-      const int c = cb * 32 + 8 * e + 4 * h;
-      const f32x16& v = adv[cb];
-      if (c < a.dv) *reinterpret_cast<u32x2*>(dv + c) = valid ? cvt_bf16x4(f32x4{v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]}) : none;
-    }
+    for (int cb = 0; cb < ((OUT & 2) ? F::VC : 0); cb++)
+      if (cb * 32 + 8 * e + 4 * h < a.dv) put(dv, pv, cb * 32 + 8 * e + 4 * h, adv[cb], e, 1.f);
   }
 }
 
@@ -855,17 +1048,33 @@ int check_desc(const gc_diff_attention* a, bool backward) {
   return GC_OK;
 }
 
-// Few rows, long keys: the keys are split so that about two workgroups per CU run, each with at least four blocks.
+// Whether and how far the keys of a row are split.
 void plan_forward(const gc_diff_attention* a, DiffParams& P) {
   P.a = *a;
   P.G = a->H / a->HK;
-  const int64_t R = (int64_t)P.G * a->NQ, nblk = ((int64_t)a->NK + kBlk - 1) / kBlk;
+  const int64_t R = (int64_t)P.G * a->NQ, cus = device_cu_count(), heads = (int64_t)a->B * a->HK;
   P.tiles = (int)((R + kRows - 1) / kRows);
   P.div_nq = make_fastdiv((uint32_t)a->NQ);
   P.c2 = a->scale * 1.44269504088896340736f;
   P.lazy = kLazy / P.c2;
-  const int64_t groups = (int64_t)a->B * a->HK * P.tiles, want = 2ll * device_cu_count();
-  int64_t n = groups > 0 && groups < want ? (want + groups - 1) / groups : 1;
+  P.few = R <= 32 && a->NK >= 256;
+  int64_t n = 1;
+  if (P.few) {
+    // one workgroup per CU (two of the narrow form, whose stages are half as large), every wave a share of at least two tiles
+    const int form = form_of(a), nw = form == 2 ? 2 : 4;
+    const int64_t tiles32 = ((int64_t)a->NK + 31) / 32;
+    n = cus * (form == 0 ? 2 : 1) / (heads > 0 ? heads : 1);
+    if (n > kMaxShares / nw) n = kMaxShares / nw;
+    if (n > tiles32 / 2 / nw) n = tiles32 / 2 / nw;
+    if (n < 1) n = 1;
+    P.nsplit = (int)n * nw;
+    P.blocks_per_split = (int)((tiles32 + P.nsplit - 1) / P.nsplit);
+    return;
+  }
+  // a grid that leaves three quarters of the workgroup slots (two per CU) empty: split, each share at least four blocks
+  const int64_t nblk = ((int64_t)a->NK + kBlk - 1) / kBlk, groups = heads * P.tiles;
+  n = groups > 0 ? 2 * cus / groups : 1;
+  if (n < 4) n = 1;
   if (n > nblk / 4) n = nblk / 4;
   if (n > 256) n = 256;
   if (n < 1) n = 1;
@@ -879,10 +1088,35 @@ size_t forward_bytes(const DiffParams& P, int DV) {
   const size_t rows = (size_t)P.nsplit * P.a.B * P.a.HK * P.G * P.a.NQ;
   return rows * (4 + 2 * (size_t)DV) * sizeof(float);
 }
-size_t backward_bytes(const gc_diff_attention* a) {
-  const size_t rows = (size_t)a->B * a->H * a->NQ, tiles = (size_t)a->B * a->H * ((a->NQ + kRows - 1) / kRows);
-  return ((rows * 2 + 3) / 4 * 4 + tiles) * sizeof(float);
+// The backward kernels' shares: of the keys of a query tile (dq), of the queries of a key tile (dkv).  A grid that fills the chip takes
+// one share and stores its result; otherwise the shares' fp32 partial results are added by diff_sum_kernel.  Causal key tiles differ in
+// length, so dkv wants twice as many workgroups as run at a time.
+struct BackwardPlan {
+  int dq_tiles, dq_shares, dq_blocks, dkv_tiles, dkv_shares;
+  size_t delta, lampart, part;                             // floats
+};
+BackwardPlan plan_backward(const gc_diff_attention* a) {
+  BackwardPlan p{};
+  const int64_t cus = device_cu_count(), nkb = ((int64_t)a->NK + kBlk - 1) / kBlk, nqb = ((int64_t)a->NQ + kBlk - 1) / kBlk, G = a->H / a->HK;
+  p.dq_tiles = (a->NQ + kRows - 1) / kRows;
+  p.dkv_tiles = (a->NK + kRows - 1) / kRows;
+  int64_t n = 2 * cus / ((int64_t)a->B * a->H * p.dq_tiles);
+  if (n > nkb / 4) n = nkb / 4;
+  if (n < 4) n = 1;
+  p.dq_blocks = (int)((nkb + n - 1) / n);
+  p.dq_shares = (int)((nkb + p.dq_blocks - 1) / p.dq_blocks);
+  n = (a->causal ? 4 : 2) * cus / ((int64_t)a->B * a->HK * p.dkv_tiles);
+  if (n > G * nqb / 4) n = G * nqb / 4;
+  if (n > 64) n = 64;
+  p.dkv_shares = n < 2 ? 1 : (int)n;
+  const size_t rows = (size_t)a->B * a->H * a->NQ, keys = (size_t)a->B * a->HK * a->NK;
+  p.delta = (rows * 2 + 3) / 4 * 4;
+  p.lampart = ((size_t)a->B * a->H * p.dq_tiles * p.dq_shares + 3) / 4 * 4;
+  const size_t dq = p.dq_shares > 1 ? (size_t)p.dq_shares * rows * 2 * a->d : 0, dkv = p.dkv_shares > 1 ? (size_t)p.dkv_shares * keys * (2 * a->d + a->dv) : 0;
+  p.part = dq > dkv ? dq : dkv;                            // (used one after the other)
+  return p;
 }
+size_t backward_bytes(const BackwardPlan& p) { return (p.delta + p.lampart + p.part) * sizeof(float); }
 
 template <int DK, int DV>
 int launch_fwd(const DiffParams& P, hipStream_t s) {
@@ -893,19 +1127,32 @@ int launch_fwd(const DiffParams& P, hipStream_t s) {
   return check_hip(hipGetLastError(), "diff_fwd launch");
 }
 template <int DK, int DV>
+int launch_few(const DiffParams& P, hipStream_t s) {
+  typedef FewCfg<DK, DV> X;
+  constexpr int lds = X::NW * 2 * X::STAGE;
+  if (int e = ensure_dynamic_smem(reinterpret_cast<const void*>(diff_few_rows_kernel<DK, DV>), lds)) return e;
+  hipLaunchKernelGGL((diff_few_rows_kernel<DK, DV>), dim3((unsigned)P.a.B * P.a.HK * (P.nsplit / X::NW)), dim3(X::NW * 64), lds, s, P);
+  return check_hip(hipGetLastError(), "diff_few_rows launch");
+}
+template <int DK, int DV>
 int launch_dq(const DiffParams& P, hipStream_t s) {
   typedef Cfg<DK, DV> F;
   constexpr int lds = 2 * (2 * F::KB + F::VB);
   if (int e = ensure_dynamic_smem(reinterpret_cast<const void*>(diff_bwd_dq_kernel<DK, DV>), lds)) return e;
-  hipLaunchKernelGGL((diff_bwd_dq_kernel<DK, DV>), dim3((unsigned)P.a.B * P.a.H * P.tiles), dim3(kThreads), lds, s, P);
+  hipLaunchKernelGGL((diff_bwd_dq_kernel<DK, DV>), dim3((unsigned)P.a.B * P.a.H * P.tiles * P.nsplit), dim3(kThreads), lds, s, P);
   return check_hip(hipGetLastError(), "diff_bwd_dq launch");
+}
+int launch_sum(const float* part, int shares, void* out0, size_t n0, void* out1, size_t n1, hipStream_t s) {
+  hipLaunchKernelGGL(diff_sum_kernel, dim3((unsigned)(((n0 + n1) / 4 + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, part, shares, (uint16_t*)out0, n0,
+                     (uint16_t*)out1, n1);
+  return check_hip(hipGetLastError(), "diff_sum launch");
 }
 template <int DK, int DV, int OUT>
 int launch_dkv(const DiffParams& P, hipStream_t s) {
   typedef Cfg<DK, DV> F;
   constexpr int lds = DkvCfg<DK, DV, OUT>::LDS;
   if (int e = ensure_dynamic_smem(reinterpret_cast<const void*>(diff_bwd_dkv_kernel<DK, DV, OUT>), lds)) return e;
-  hipLaunchKernelGGL((diff_bwd_dkv_kernel<DK, DV, OUT>), dim3((unsigned)P.a.B * P.a.HK * P.tiles), dim3(kThreads), lds, s, P);
+  hipLaunchKernelGGL((diff_bwd_dkv_kernel<DK, DV, OUT>), dim3((unsigned)P.a.B * P.a.HK * P.tiles * P.nsplit), dim3(kThreads), lds, s, P);
   return check_hip(hipGetLastError(), "diff_bwd_dkv launch");
 }
 
@@ -916,7 +1163,7 @@ using namespace gc;
 
 extern "C" size_t gc_diff_attention_workspace_bytes(const gc_diff_attention* desc, int backward) {
   if (desc == nullptr || desc->B <= 0 || desc->NQ <= 0 || desc->H <= 0 || desc->HK <= 0 || desc->H % desc->HK != 0) return 0;
-  if (backward) return backward_bytes(desc);
+  if (backward) return desc->NK > 0 ? backward_bytes(plan_backward(desc)) : 0;
   DiffParams P{};
   plan_forward(desc, P);
   return forward_bytes(P, kDV[form_of(desc)]);
@@ -938,13 +1185,15 @@ extern "C" int gc_diff_attention_fwd(const gc_diff_attention* desc, void* worksp
   P.part = need > 0 ? P.ml + rows * 4 : nullptr;
   hipStream_t s = (hipStream_t)stream;
   {
-    ProfScope ps("gc::diff_fwd_kernel", 4.0 * desc->B * desc->H * (double)desc->NQ * desc->NK * (desc->d + desc->dv), s);
-    const int e = form == 0 ? launch_fwd<32, 64>(P, s) : (form == 1 ? launch_fwd<64, 128>(P, s) : launch_fwd<128, 256>(P, s));
+    ProfScope ps(P.few ? "gc::diff_few_rows_kernel" : "gc::diff_fwd_kernel", 4.0 * desc->B * desc->H * (double)desc->NQ * desc->NK * (desc->d + desc->dv), s);
+    int e;
+    if (P.few) e = form == 0 ? launch_few<32, 64>(P, s) : (form == 1 ? launch_few<64, 128>(P, s) : launch_few<128, 256>(P, s));
+    else e = form == 0 ? launch_fwd<32, 64>(P, s) : (form == 1 ? launch_fwd<64, 128>(P, s) : launch_fwd<128, 256>(P, s));
     if (e) return e;
   }
   if (P.nsplit > 1) {
     const size_t out_rows = (size_t)desc->B * desc->H * desc->NQ;
-    hipLaunchKernelGGL(diff_join_kernel, dim3((unsigned)((out_rows + 3) / 4)), dim3(kThreads), 0, s, P, DV);
+    hipLaunchKernelGGL(diff_join_kernel, dim3((unsigned)out_rows), dim3(kJoinThreads), 0, s, P, DV);
     return check_hip(hipGetLastError(), "diff_join launch");
   }
   return GC_OK;
@@ -956,34 +1205,43 @@ extern "C" int gc_diff_attention_bwd(const gc_diff_attention* desc, void* worksp
     set_error("differential attention backward: an empty tensor has no gradient to compute");
     return GC_BAD_ARGUMENT;
   }
-  const size_t need = backward_bytes(desc);
+  const BackwardPlan plan = plan_backward(desc);
+  const size_t need = backward_bytes(plan);
   if (misaligned(workspace) || workspace_bytes < need) {
     set_error("differential attention backward: a 16-byte aligned workspace of %zu bytes is needed", need);
     return GC_WORKSPACE_TOO_SMALL;
   }
   DiffParams P{};
   plan_forward(desc, P);
-  const size_t rows = (size_t)desc->B * desc->H * desc->NQ;
+  const size_t rows = (size_t)desc->B * desc->H * desc->NQ, keys = (size_t)desc->B * desc->HK * desc->NK;
   P.delta = static_cast<float*>(workspace);
-  P.lampart = P.delta + (rows * 2 + 3) / 4 * 4;
+  P.lampart = P.delta + plan.delta;
+  P.part = P.lampart + plan.lampart;
   hipStream_t s = (hipStream_t)stream;
   const int form = form_of(desc);
   const double pairs = (double)desc->B * desc->H * desc->NQ * desc->NK;
   hipLaunchKernelGGL(diff_delta_kernel, dim3((unsigned)((rows * 16 + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, P);
   if (check_hip(hipGetLastError(), "diff_delta launch")) return GC_HIP_ERROR;
+  P.tiles = plan.dkv_tiles;
+  P.nsplit = plan.dkv_shares;
   {
-    P.tiles = (desc->NK + kRows - 1) / kRows;
     ProfScope ps("gc::diff_bwd_dkv_kernel", pairs * (8.0 * desc->d + 4.0 * desc->dv), s);
     int e = form == 0 ? launch_dkv<32, 64, 3>(P, s) : (form == 1 ? launch_dkv<64, 128, 3>(P, s) : launch_dkv<128, 256, 1>(P, s));
     if (e == GC_OK && form == 2) e = launch_dkv<128, 256, 2>(P, s);
     if (e) return e;
   }
-  P.tiles = (desc->NQ + kRows - 1) / kRows;
+  if (P.nsplit > 1)
+    if (int e = launch_sum(P.part, P.nsplit, desc->dk, keys * 2 * desc->d, desc->dv_out, keys * desc->dv, s)) return e;
+  P.tiles = plan.dq_tiles;
+  P.nsplit = plan.dq_shares;
+  P.blocks_per_split = plan.dq_blocks;
   {
     ProfScope ps("gc::diff_bwd_dq_kernel", pairs * (8.0 * desc->d + 2.0 * desc->dv), s);
     const int e = form == 0 ? launch_dq<32, 64>(P, s) : (form == 1 ? launch_dq<64, 128>(P, s) : launch_dq<128, 256>(P, s));
     if (e) return e;
   }
+  if (P.nsplit > 1)
+    if (int e = launch_sum(P.part, P.nsplit, desc->dq, rows * 2 * desc->d, nullptr, 0, s)) return e;
   hipLaunchKernelGGL(diff_dlam_kernel, dim3(desc->H), dim3(kThreads), 0, s, P);
   return check_hip(hipGetLastError(), "diff_dlam launch");
 }

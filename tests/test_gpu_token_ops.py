@@ -394,6 +394,12 @@ ATTENTION_CASES = [
     (1, 190, 190, 3, 1, 24, 48, True, None, 0.5),
     (1, 320, 320, 2, 2, 64, 128, True, None, 3.0),
     (1, 129, 129, 1, 1, 64, 64, True, (-3,), 1.0),
+    (1, 8, 3000, 4, 1, 64, 128, True, (2990,), 1.0),
+    (2, 4, 900, 2, 1, 32, 64, False, (900, 31), 1.0),
+    (1, 40, 2100, 1, 1, 32, 64, True, None, 1.0),
+    (1, 700, 700, 3, 1, 32, 64, True, None, 1.0),
+    (1, 520, 300, 2, 1, 64, 128, False, None, 1.0),
+    (1, 300, 520, 2, 2, 128, 256, False, (500,), 1.0),
 ]
 
 
