@@ -179,15 +179,15 @@ def lib():
     L.gc_adam_step.restype = ctypes.c_int
     L.gc_adam_ema_step.argtypes = [i32, vp, vp, vp, vp, vp, f32, vp, vp, f32, f32, f32, f32, vp]
     L.gc_adam_ema_step.restype = ctypes.c_int
-    L.gc_block_norm_fwd.argtypes = [ctypes.POINTER(BlockNorm), vp]
+    L.gc_block_norm_fwd.argtypes = [vp, vp]         # descriptors: a structure by reference, or its packed bytes
     L.gc_block_norm_workspace_bytes.argtypes = [i64, i64, i32]
     L.gc_block_norm_workspace_bytes.restype = sz
-    L.gc_block_norm_bwd.argtypes = [ctypes.POINTER(BlockNorm), vp, sz, vp]
-    L.gc_axial_rotary.argtypes = [ctypes.POINTER(Rotary), vp]
-    L.gc_diff_attention_workspace_bytes.argtypes = [ctypes.POINTER(DiffAttention), ctypes.c_int]
+    L.gc_block_norm_bwd.argtypes = [vp, vp, sz, vp]
+    L.gc_axial_rotary.argtypes = [vp, vp]
+    L.gc_diff_attention_workspace_bytes.argtypes = [vp, ctypes.c_int]
     L.gc_diff_attention_workspace_bytes.restype = sz
-    L.gc_diff_attention_fwd.argtypes = [ctypes.POINTER(DiffAttention), vp, sz, vp]
-    L.gc_diff_attention_bwd.argtypes = [ctypes.POINTER(DiffAttention), vp, sz, vp]
+    L.gc_diff_attention_fwd.argtypes = [vp, vp, sz, vp]
+    L.gc_diff_attention_bwd.argtypes = [vp, vp, sz, vp]
     L.gc_profile_enable.argtypes = [ctypes.c_int]
     L.gc_profile_collect.argtypes = [ctypes.c_int, vp, vp, vp, vp]
     for fn in ("gc_pack_weight", "gc_conv2d_fprop", "gc_conv2d_dgrad", "gc_conv2d_wgrad", "gc_conv2d_wgrad_noalloc", "gc_dwblur3x3", "gc_dwblur3x3_masked", "gc_profile_enable",

@@ -19,6 +19,8 @@
 // workgroup.  A thread keeps its channels for all its rows, so the parameters are read once per workgroup and the sums S
 // live in registers; they leave as one partial row per workgroup and are added in a fixed order (no atomics).  Statistics
 // and sums are fp32; y enters the second norm before it is rounded to its storage type.
+#include <mutex>
+
 #include "common.h"
 
 namespace gc {
@@ -36,71 +38,122 @@ struct NormParams {
   int vec;                        // 16-byte loads and stores are possible
   int slabs;                      // workgroups per sample
   float* part;                    // backward: [batch][slabs][kSums][cols]
+  float* rho_part;                // [batch][slabs], or null (no scalar residual scale asked for)
 };
 
-template <typename T>
-__device__ __forceinline__ void load8(const void* base, int64_t off, int c0, int C, bool vec, float (&v)[kE]) {
-  if (vec) {
-    const f32x4 a = load4<T>(base, (size_t)(off + c0)), b = load4<T>(base, (size_t)(off + c0 + 4));
+// A thread's 8 channels lie in 8 / W runs of W neighbours, a run of all threads of the row behind the other, so that every load
+// instruction of a wave covers one contiguous stretch: W = 8 (bf16) or 4 (fp32) for 16-byte accesses, 1 where the row length, a stride
+// or an address does not allow them.
+template <int W>
+struct Lane {
+  int first, step, C;
+  __device__ __forceinline__ Lane(int t, int tpr, int C_) : first(t * W), step(tpr * W), C(C_) {}
+  __device__ __forceinline__ int ch(int e) const { return (e / W) * step + first + e % W; }
+  __device__ __forceinline__ bool has(int e) const { return ch(e) < C; }       // (a run is there as a whole)
+};
+
+template <typename T> struct Raw { uint32_t w[kE * sizeof(T) / 4]; };           // 8 values as stored
+
+template <typename T, int W>
+__device__ __forceinline__ Raw<T> load_raw(const void* base, int64_t off, const Lane<W>& L, bool live) {
+  Raw<T> r;
 #pragma unroll
-    for (int e = 0; e < 4; e++) { v[e] = a[e]; v[4 + e] = b[e]; }
-  } else {
+  for (int i = 0; i < (int)(kE * sizeof(T) / 4); i++) r.w[i] = 0u;
+  if (!live) return r;
+  const T* p = static_cast<const T*>(base) + off;
+  if constexpr (W > 1) {
+    constexpr int words = W * sizeof(T) / 4;                                    // 4: one 16-byte access per run
 #pragma unroll
-    for (int e = 0; e < kE; e++) {
-      v[e] = 0.f;
-      if (c0 + e < C) {
-        if constexpr (sizeof(T) == 4) v[e] = static_cast<const float*>(base)[off + c0 + e];
-        else v[e] = bf16_bits_to_float(static_cast<const uint16_t*>(base)[off + c0 + e]);
+    for (int k = 0; k < kE / W; k++)
+      if (L.has(k * W)) {
+        const u32x4 q = *reinterpret_cast<const u32x4*>(p + L.ch(k * W));
+#pragma unroll
+        for (int i = 0; i < words; i++) r.w[k * words + i] = q[i];
       }
-    }
-  }
-}
-template <>
-__device__ __forceinline__ void load8<uint16_t>(const void* base, int64_t off, int c0, int C, bool vec, float (&v)[kE]) {
-  const uint16_t* p = static_cast<const uint16_t*>(base) + off + c0;
-  if (vec) {
-    const u32x4 q = *reinterpret_cast<const u32x4*>(p);
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      v[2 * e] = __builtin_bit_cast(float, q[e] << 16);
-      v[2 * e + 1] = __builtin_bit_cast(float, q[e] & 0xffff0000u);
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < kE; e++) v[e] = c0 + e < C ? bf16_bits_to_float(p[e]) : 0.f;
-  }
-}
-template <typename T>
-__device__ __forceinline__ void store8(void* base, int64_t off, int c0, int C, bool vec, const float (&v)[kE]) {
-  if (vec) {
-    const f32x4 a = {v[0], v[1], v[2], v[3]}, b = {v[4], v[5], v[6], v[7]};
-    if constexpr (sizeof(T) == 4) {
-      float* p = static_cast<float*>(base) + off + c0;
-      *reinterpret_cast<f32x4*>(p) = a;
-      *reinterpret_cast<f32x4*>(p + 4) = b;
-    } else {
-      const u32x2 lo = cvt_bf16x4(a), hi = cvt_bf16x4(b);
-      *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(base) + off + c0) = u32x4{lo[0], lo[1], hi[0], hi[1]};
-    }
   } else {
 #pragma unroll
     for (int e = 0; e < kE; e++)
-      if (c0 + e < C) {
-        if constexpr (sizeof(T) == 4) static_cast<float*>(base)[off + c0 + e] = v[e];
-        else static_cast<uint16_t*>(base)[off + c0 + e] = float_to_bf16_bits(v[e]);
+      if (L.has(e)) {
+        if constexpr (sizeof(T) == 4) r.w[e] = __builtin_bit_cast(uint32_t, p[L.ch(e)]);
+        else r.w[e / 2] |= (uint32_t)p[L.ch(e)] << (16 * (e & 1));
+      }
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void widen(const Raw<T>& r, float (&v)[kE]) {
+#pragma unroll
+  for (int e = 0; e < kE; e++) {
+    if constexpr (sizeof(T) == 4) { const uint32_t u = r.w[e]; v[e] = __builtin_bit_cast(float, u); }
+    else v[e] = __builtin_bit_cast(float, (e & 1) ? (r.w[e / 2] & 0xffff0000u) : (r.w[e / 2] << 16));
+  }
+}
+template <typename T, int W>
+__device__ __forceinline__ void store_row(void* base, int64_t off, const Lane<W>& L, const float (&v)[kE]) {
+  T* p = static_cast<T*>(base) + off;
+  if constexpr (W > 1) {
+#pragma unroll
+    for (int k = 0; k < kE / W; k++)
+      if (L.has(k * W)) {
+        if constexpr (sizeof(T) == 4) {
+          *reinterpret_cast<f32x4*>(p + L.ch(k * W)) = f32x4{v[k * W], v[k * W + 1], v[k * W + 2], v[k * W + 3]};
+        } else {
+          const u32x2 lo = cvt_bf16x4(f32x4{v[0], v[1], v[2], v[3]}), hi = cvt_bf16x4(f32x4{v[4], v[5], v[6], v[7]});
+          *reinterpret_cast<u32x4*>(p + L.ch(0)) = u32x4{lo[0], lo[1], hi[0], hi[1]};
+        }
+      }
+  } else {
+#pragma unroll
+    for (int e = 0; e < kE; e++)
+      if (L.has(e)) {
+        if constexpr (sizeof(T) == 4) p[L.ch(e)] = v[e];
+        else p[L.ch(e)] = float_to_bf16_bits(v[e]);
       }
   }
 }
 
 // fp32 parameter: null -> `neutral`; one value per channel, or per (sample, channel)
-__device__ __forceinline__ void load_param(const float* p, int per_sample, int64_t sample, int c0, int C, float neutral, float (&v)[kE]) {
+template <int W>
+__device__ __forceinline__ void load_param(const float* p, int per_sample, int64_t sample, const Lane<W>& L, float neutral, float (&v)[kE]) {
 #pragma unroll
   for (int e = 0; e < kE; e++) v[e] = neutral;
   if (p == nullptr) return;
-  p += (per_sample ? sample * C : 0) + c0;
+  p += per_sample ? sample * L.C : 0;
 #pragma unroll
   for (int e = 0; e < kE; e++)
-    if (c0 + e < C) v[e] = p[e];
+    if (L.has(e)) v[e] = p[L.ch(e)];
+}
+template <int W>
+__device__ __forceinline__ void load_rho(const gc_block_norm& a, const Lane<W>& L, float (&v)[kE]) {
+  if (a.residual_per_channel) { load_param<W>(a.residual_scale, 0, 0, L, 1.f, v); return; }
+  const float r = a.residual_scale != nullptr ? a.residual_scale[0] : a.residual_constant;
+#pragma unroll
+  for (int e = 0; e < kE; e++) v[e] = r;
+}
+
+// v + the value of the lane whose number differs in one bit, in the vector unit: within 16 lanes by data-parallel-primitive moves (the
+// sums of a quad / of 8 lanes are already equal when lanes are mirrored within 8 / 16), beyond by the row and half-wave swaps.
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+template <bool HALVES>
+__device__ __forceinline__ float swap_add(float v) {
+  typedef unsigned int u32pair __attribute__((ext_vector_type(2)));
+  const unsigned int u = __builtin_bit_cast(unsigned int, v);
+  const u32pair r = HALVES ? __builtin_amdgcn_permlane32_swap(u, u, false, false) : __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const unsigned int x = r[0], y = r[1];                   // (scalars first: a bit cast of a vector's element itself reads element 0)
+  return __builtin_bit_cast(float, x) + __builtin_bit_cast(float, y);
+}
+// Sum over groups of n (a power of two up to 64) neighbouring lanes, in all of them
+__device__ __forceinline__ float lanes_sum(float v, int n) {
+  if (n >= 2) v = dpp_add<0xb1>(v);                        // quad_perm 1 0 3 2
+  if (n >= 4) v = dpp_add<0x4e>(v);                        // quad_perm 2 3 0 1
+  if (n >= 8) v = dpp_add<0x141>(v);                       // mirrored within 8
+  if (n >= 16) v = dpp_add<0x140>(v);                      // mirrored within 16
+  if (n >= 32) v = swap_add<false>(v);
+  if (n >= 64) v = swap_add<true>(v);
+  return v;
 }
 
 // Sums of N values over a row's threads, in all of them.  WIDE: the workgroup is the row; `red` holds two sets of
@@ -109,8 +162,7 @@ __device__ __forceinline__ void load_param(const float* p, int per_sample, int64
 template <bool WIDE, int N>
 __device__ __forceinline__ void row_sum(float (&v)[N], int tpr, float* red, int& turn) {
 #pragma unroll
-  for (int n = 0; n < N; n++)
-    for (int o = (WIDE ? 32 : tpr >> 1); o > 0; o >>= 1) v[n] += __shfl_xor(v[n], o, 64);
+  for (int n = 0; n < N; n++) v[n] = lanes_sum(v[n], WIDE ? 64 : tpr);
   if (WIDE) {
     const int nw = blockDim.x >> 6;
     float* r = red + turn * (2 * (kMaxThreads / 64));
@@ -129,10 +181,9 @@ __device__ __forceinline__ void row_sum(float (&v)[N], int tpr, float* red, int&
 }
 
 // mean (0 for the root-mean-square norm) and 1 / standard deviation of a row held as 8 values per thread
-template <bool WIDE>
-__device__ __forceinline__ void row_stats(const float (&v)[kE], int c0, int C, bool layer, float eps, int tpr, float* red, int& turn, float& mu,
-                                          float& r) {
-  const float inv = 1.f / (float)C;
+template <bool WIDE, int W>
+__device__ __forceinline__ void row_stats(const float (&v)[kE], const Lane<W>& L, bool layer, float eps, int tpr, float* red, int& turn, float& mu, float& r) {
+  const float inv = 1.f / (float)L.C;
   mu = 0.f;
   if (layer) {
     float s[1] = {0.f};
@@ -144,76 +195,82 @@ __device__ __forceinline__ void row_stats(const float (&v)[kE], int c0, int C, b
   float q[1] = {0.f};
 #pragma unroll
   for (int e = 0; e < kE; e++) {
-    const float t = c0 + e < C ? v[e] - mu : 0.f;
+    const float t = L.has(e) ? v[e] - mu : 0.f;
     q[0] += t * t;
   }
   row_sum<WIDE, 1>(q, tpr, red, turn);
   r = 1.f / sqrtf(q[0] * inv + eps);
 }
 
-template <typename T, bool WIDE, int PART>
-__global__ __launch_bounds__(WIDE ? kMaxThreads : kThreads) void block_norm_fwd_kernel(const NormParams P) {
+// The rows of a workgroup: side by side (narrow rows) and one after the other.  The next rows are asked for before the current ones are
+// worked on: the two reductions of a row leave no other work to hide the loads behind.
+// MAXT: 256 (narrow rows), or the most threads a wide row takes: 512 leave the backward pass the registers it needs, 1024 do not.
+template <typename T, int MAXT, int PART, int W>
+__global__ __launch_bounds__(MAXT) void block_norm_fwd_kernel(const NormParams P) {
+  constexpr bool WIDE = MAXT > kThreads;
   __shared__ float red[WIDE ? 4 * (kMaxThreads / 64) : 1];
   const gc_block_norm& a = P.a;
   const int C = a.cols, tpr = P.tpr, rpw = WIDE ? 1 : kThreads / tpr;
-  const int c0 = (WIDE ? (int)threadIdx.x : (int)threadIdx.x & (tpr - 1)) * kE, sub = WIDE ? 0 : (int)threadIdx.x / tpr;
-  const bool mine = c0 < C, layer = a.layer != 0;
-  const int64_t sample = blockIdx.y, nstat = a.batch * a.rows;
+  const int t = WIDE ? (int)threadIdx.x : (int)threadIdx.x & (tpr - 1), sub = WIDE ? 0 : (int)threadIdx.x / tpr;
+  const Lane<W> L(t, tpr, C);
+  const bool layer = a.layer != 0;
+  const int64_t sample = blockIdx.y, nstat = a.batch * a.rows, hop = (int64_t)gridDim.x * rpw;
   int turn = 0;
+  // a thread past the last row takes part in the sums with zeros
+  int64_t row = (int64_t)blockIdx.x * rpw + sub;
+  Raw<T> rx = load_raw<T, W>(a.x, sample * a.x_batch_stride + row * a.x_row_stride, L, row < a.rows), rf;
+  if (PART != kIn) rf = load_raw<T, W>(a.f, sample * a.f_batch_stride + row * a.f_row_stride, L, row < a.rows);
   float A[kE], B[kE], Cw[kE], D[kE], rho[kE];
   if (PART != kIn) {
     float g[kE];
-    load_param(a.gate, a.gate_per_sample, sample, c0, C, 1.f, g);
-    load_param(a.out_weight, 0, 0, c0, C, 1.f, A);
-    load_param(a.out_bias, 0, 0, c0, C, 0.f, B);
-    load_param(a.residual_scale, 0, 0, a.residual_per_channel ? c0 : 0, a.residual_per_channel ? C : 1, a.residual_constant, rho);
+    load_param<W>(a.gate, a.gate_per_sample, sample, L, 1.f, g);
+    load_param<W>(a.out_weight, 0, 0, L, 1.f, A);
+    load_param<W>(a.out_bias, 0, 0, L, 0.f, B);
+    load_rho<W>(a, L, rho);
 #pragma unroll
     for (int e = 0; e < kE; e++) {
       A[e] *= g[e];
       B[e] *= g[e];
-      if (a.residual_scale != nullptr && !a.residual_per_channel) rho[e] = rho[0];
     }
   }
   if (PART != kOut) {
-    float s[kE], t[kE];
-    load_param(a.in_weight, 0, 0, c0, C, 1.f, Cw);
-    load_param(a.in_bias, 0, 0, c0, C, 0.f, D);
-    load_param(a.scale, a.mod_per_sample, sample, c0, C, 0.f, s);
-    load_param(a.shift, a.mod_per_sample, sample, c0, C, 0.f, t);
+    float s[kE], sh[kE];
+    load_param<W>(a.in_weight, 0, 0, L, 1.f, Cw);
+    load_param<W>(a.in_bias, 0, 0, L, 0.f, D);
+    load_param<W>(a.scale, a.mod_per_sample, sample, L, 0.f, s);
+    load_param<W>(a.shift, a.mod_per_sample, sample, L, 0.f, sh);
 #pragma unroll
     for (int e = 0; e < kE; e++) {
       Cw[e] *= 1.f + s[e];
-      D[e] = D[e] * (1.f + s[e]) + t[e];
+      D[e] = D[e] * (1.f + s[e]) + sh[e];
     }
   }
-  for (int64_t row0 = (int64_t)blockIdx.x * rpw; row0 < a.rows; row0 += (int64_t)gridDim.x * rpw) {
-    const int64_t row = row0 + sub;
-    const bool live = mine && row < a.rows;
+  for (int64_t row0 = (int64_t)blockIdx.x * rpw; row0 < a.rows; row0 += hop, row += hop) {
+    const bool live = row < a.rows;
     float y[kE], f[kE];
-    // a dead thread (past the last channel or row) takes part in the sums with zeros
-    const bool vec = P.vec != 0;
-#pragma unroll
-    for (int e = 0; e < kE; e++) { y[e] = 0.f; f[e] = 0.f; }
-    if (live) {
-      load8<T>(a.x, sample * a.x_batch_stride + row * a.x_row_stride, c0, C, vec, y);
-      if (PART != kIn) load8<T>(a.f, sample * a.f_batch_stride + row * a.f_row_stride, c0, C, vec, f);
+    widen<T>(rx, y);
+    if (PART != kIn) widen<T>(rf, f);
+    if (row0 + hop < a.rows) {
+      const int64_t next = row + hop;
+      rx = load_raw<T, W>(a.x, sample * a.x_batch_stride + next * a.x_row_stride, L, next < a.rows);
+      if (PART != kIn) rf = load_raw<T, W>(a.f, sample * a.f_batch_stride + next * a.f_row_stride, L, next < a.rows);
     }
     const int64_t out = (sample * a.rows + row) * C;
     float mu_f = 0.f, r_f = 0.f, mu_y = 0.f, r_y = 0.f;
     if (PART != kIn) {
-      row_stats<WIDE>(f, c0, C, layer, a.eps, tpr, red, turn, mu_f, r_f);
+      row_stats<WIDE, W>(f, L, layer, a.eps, tpr, red, turn, mu_f, r_f);
 #pragma unroll
-      for (int e = 0; e < kE; e++) y[e] = c0 + e < C ? rho[e] * y[e] + (A[e] * ((f[e] - mu_f) * r_f) + B[e]) : 0.f;
-      if (live) store8<T>(a.y, out, c0, C, vec, y);
+      for (int e = 0; e < kE; e++) y[e] = L.has(e) ? rho[e] * y[e] + (A[e] * ((f[e] - mu_f) * r_f) + B[e]) : 0.f;
+      if (live) store_row<T, W>(a.y, out, L, y);
     }
     if (PART != kOut) {
-      row_stats<WIDE>(y, c0, C, layer, a.eps, tpr, red, turn, mu_y, r_y);
+      row_stats<WIDE, W>(y, L, layer, a.eps, tpr, red, turn, mu_y, r_y);
       float h[kE];
 #pragma unroll
       for (int e = 0; e < kE; e++) h[e] = Cw[e] * ((y[e] - mu_y) * r_y) + D[e];
-      if (live) store8<T>(a.h, out, c0, C, vec, h);
+      if (live) store_row<T, W>(a.h, out, L, h);
     }
-    if (a.stats != nullptr && c0 == 0 && live) {       // [4][batch * rows]: r_f, r_y, mu_f, mu_y (those the parts have)
+    if (a.stats != nullptr && t == 0 && live) {            // [4][batch * rows]: r_f, r_y, mu_f, mu_y (those the parts have)
       const int64_t i = sample * a.rows + row;
       if (PART != kIn) { a.stats[i] = r_f; if (layer) a.stats[2 * nstat + i] = mu_f; }
       if (PART != kOut) { a.stats[nstat + i] = r_y; if (layer) a.stats[3 * nstat + i] = mu_y; }
@@ -221,36 +278,53 @@ __global__ __launch_bounds__(WIDE ? kMaxThreads : kThreads) void block_norm_fwd_
   }
 }
 
-template <typename T, bool WIDE, int PART>
-__global__ __launch_bounds__(WIDE ? kMaxThreads : kThreads) void block_norm_bwd_kernel(const NormParams P) {
+template <typename T, int MAXT, int PART, int W>
+__global__ __launch_bounds__(MAXT) void block_norm_bwd_kernel(const NormParams P) {
+  constexpr bool WIDE = MAXT > kThreads;
   __shared__ float red[WIDE ? 4 * (kMaxThreads / 64) : 1];
-  __shared__ float fold[WIDE ? 1 : kThreads * kE];
+  __shared__ float fold[WIDE ? 1 : kThreads * kE], scalar[MAXT / 64];
   const gc_block_norm& a = P.a;
   const int C = a.cols, tpr = P.tpr, rpw = WIDE ? 1 : kThreads / tpr;
-  const int lane_in_row = WIDE ? (int)threadIdx.x : (int)threadIdx.x & (tpr - 1);
-  const int c0 = lane_in_row * kE, sub = WIDE ? 0 : (int)threadIdx.x / tpr;
-  const bool mine = c0 < C, layer = a.layer != 0, vec = P.vec != 0;
-  const int64_t sample = blockIdx.y, nstat = a.batch * a.rows;
+  const int t = WIDE ? (int)threadIdx.x : (int)threadIdx.x & (tpr - 1), sub = WIDE ? 0 : (int)threadIdx.x / tpr;
+  const Lane<W> L(t, tpr, C);
+  const bool layer = a.layer != 0;
+  const int64_t sample = blockIdx.y, nstat = a.batch * a.rows, hop = (int64_t)gridDim.x * rpw;
   const float inv = 1.f / (float)C;
   int turn = 0;
+  struct Row { Raw<T> x, f, dy, dh; float st[4]; } next;
+  auto ask = [&](int64_t row) {
+    const bool live = row < a.rows;
+    const int64_t out = (sample * a.rows + row) * C, i = sample * a.rows + row;
+    next.x = load_raw<T, W>(a.x, sample * a.x_batch_stride + row * a.x_row_stride, L, live);
+    if (PART != kIn) next.f = load_raw<T, W>(a.f, sample * a.f_batch_stride + row * a.f_row_stride, L, live);
+    if (PART != kIn) next.dy = load_raw<T, W>(a.dy, out, L, live && a.dy != nullptr);
+    if (PART != kOut) next.dh = load_raw<T, W>(a.dh, out, L, live && a.dh != nullptr);
+#pragma unroll
+    for (int k = 0; k < 4; k++) next.st[k] = 0.f;
+    if (live) {
+      if (PART != kIn) { next.st[0] = a.stats[i]; if (layer) next.st[2] = a.stats[2 * nstat + i]; }
+      if (PART != kOut) { next.st[1] = a.stats[nstat + i]; if (layer) next.st[3] = a.stats[3 * nstat + i]; }
+    }
+  };
+  int64_t row = (int64_t)blockIdx.x * rpw + sub;
+  ask(row);
   float A[kE], B[kE], Cw[kE], rho[kE];
   if (PART != kIn) {
     float g[kE];
-    load_param(a.gate, a.gate_per_sample, sample, c0, C, 1.f, g);
-    load_param(a.out_weight, 0, 0, c0, C, 1.f, A);
-    load_param(a.out_bias, 0, 0, c0, C, 0.f, B);
-    load_param(a.residual_scale, 0, 0, a.residual_per_channel ? c0 : 0, a.residual_per_channel ? C : 1, a.residual_constant, rho);
+    load_param<W>(a.gate, a.gate_per_sample, sample, L, 1.f, g);
+    load_param<W>(a.out_weight, 0, 0, L, 1.f, A);
+    load_param<W>(a.out_bias, 0, 0, L, 0.f, B);
+    load_rho<W>(a, L, rho);
 #pragma unroll
     for (int e = 0; e < kE; e++) {
       A[e] *= g[e];
       B[e] *= g[e];
-      if (a.residual_scale != nullptr && !a.residual_per_channel) rho[e] = rho[0];
     }
   }
   if (PART != kOut) {
     float s[kE];
-    load_param(a.in_weight, 0, 0, c0, C, 1.f, Cw);
-    load_param(a.scale, a.mod_per_sample, sample, c0, C, 0.f, s);
+    load_param<W>(a.in_weight, 0, 0, L, 1.f, Cw);
+    load_param<W>(a.scale, a.mod_per_sample, sample, L, 0.f, s);
 #pragma unroll
     for (int e = 0; e < kE; e++) Cw[e] *= 1.f + s[e];
   }
@@ -260,32 +334,27 @@ __global__ __launch_bounds__(WIDE ? kMaxThreads : kThreads) void block_norm_bwd_
 #pragma unroll
     for (int e = 0; e < kE; e++) S[k][e] = 0.f;
 
-  for (int64_t row0 = (int64_t)blockIdx.x * rpw; row0 < a.rows; row0 += (int64_t)gridDim.x * rpw) {
-    const int64_t row = row0 + sub;
-    const bool live = mine && row < a.rows;
+  for (int64_t row0 = (int64_t)blockIdx.x * rpw; row0 < a.rows; row0 += hop, row += hop) {
+    const bool live = row < a.rows;
     float x[kE], f[kE], g[kE], dh[kE];
+    widen<T>(next.x, x);
+    if (PART != kIn) { widen<T>(next.f, f); widen<T>(next.dy, g); }
+    else
 #pragma unroll
-    for (int e = 0; e < kE; e++) { x[e] = 0.f; f[e] = 0.f; g[e] = 0.f; dh[e] = 0.f; }
+      for (int e = 0; e < kE; e++) g[e] = 0.f;
+    if (PART != kOut) widen<T>(next.dh, dh);
+    const float r_f = next.st[0], r_y = next.st[1], mu_f = next.st[2], mu_y = next.st[3];
+    if (row0 + hop < a.rows) ask(row + hop);
     const int64_t out = (sample * a.rows + row) * C;
-    float r_f = 0.f, r_y = 0.f, mu_f = 0.f, mu_y = 0.f;
-    if (live) {
-      load8<T>(a.x, sample * a.x_batch_stride + row * a.x_row_stride, c0, C, vec, x);
-      if (PART != kIn) load8<T>(a.f, sample * a.f_batch_stride + row * a.f_row_stride, c0, C, vec, f);
-      if (PART != kIn && a.dy != nullptr) load8<T>(a.dy, out, c0, C, vec, g);
-      if (PART != kOut && a.dh != nullptr) load8<T>(a.dh, out, c0, C, vec, dh);
-      const int64_t i = sample * a.rows + row;
-      if (PART != kIn) { r_f = a.stats[i]; if (layer) mu_f = a.stats[2 * nstat + i]; }
-      if (PART != kOut) { r_y = a.stats[nstat + i]; if (layer) mu_y = a.stats[3 * nstat + i]; }
-    }
     if (PART != kIn)
 #pragma unroll
-      for (int e = 0; e < kE; e++) f[e] = c0 + e < C ? (f[e] - mu_f) * r_f : 0.f;          // fh from here on
+      for (int e = 0; e < kE; e++) f[e] = L.has(e) ? (f[e] - mu_f) * r_f : 0.f;            // fh from here on
     if (PART != kOut) {
       float yh[kE], m[2] = {0.f, 0.f};
 #pragma unroll
       for (int e = 0; e < kE; e++) {
         const float y = PART == kIn ? x[e] : rho[e] * x[e] + (A[e] * f[e] + B[e]);
-        yh[e] = c0 + e < C ? (y - mu_y) * r_y : 0.f;
+        yh[e] = L.has(e) ? (y - mu_y) * r_y : 0.f;
         S[2][e] += dh[e] * yh[e];
         S[3][e] += dh[e];
         const float q = Cw[e] * dh[e];
@@ -298,12 +367,12 @@ __global__ __launch_bounds__(WIDE ? kMaxThreads : kThreads) void block_norm_bwd_
       for (int e = 0; e < kE; e++) g[e] += r_y * (Cw[e] * dh[e] - yh[e] * mq - m1);
     }
     if (PART == kIn) {
-      if (live) store8<T>(a.dx, out, c0, C, vec, g);
+      if (live) store_row<T, W>(a.dx, out, L, g);
     } else {
       float p[kE], m[2] = {0.f, 0.f};
 #pragma unroll
       for (int e = 0; e < kE; e++) {
-        if (c0 + e >= C) g[e] = 0.f;
+        if (!L.has(e)) g[e] = 0.f;
         S[0][e] += g[e] * f[e];
         S[1][e] += g[e];
         S[4][e] += g[e] * x[e];
@@ -312,94 +381,162 @@ __global__ __launch_bounds__(WIDE ? kMaxThreads : kThreads) void block_norm_bwd_
         m[1] += p[e];
         x[e] = rho[e] * g[e];
       }
-      if (live) store8<T>(a.dx, out, c0, C, vec, x);
+      if (live) store_row<T, W>(a.dx, out, L, x);
       row_sum<WIDE, 2>(m, tpr, red, turn);
       const float mp = m[0] * inv, m1 = layer ? m[1] * inv : 0.f;
 #pragma unroll
       for (int e = 0; e < kE; e++) p[e] = r_f * (p[e] - f[e] * mp - m1);
-      if (live) store8<T>(a.df, out, c0, C, vec, p);
+      if (live) store_row<T, W>(a.df, out, L, p);
     }
   }
 
   // the workgroup's sums: rows handled side by side are folded in a fixed order, one sum at a time
   float* dst = P.part + ((size_t)sample * gridDim.x + blockIdx.x) * kSums * C;
+  if (PART != kIn && P.rho_part != nullptr) {              // a scalar residual scale: its sum runs over the channels too
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < kE; e++) s += S[4][e];
+    s = lanes_sum(s, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) scalar[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 1; w < (int)(blockDim.x >> 6); w++) s += scalar[w];
+      P.rho_part[sample * gridDim.x + blockIdx.x] = s;
+    }
+  }
 #pragma unroll
   for (int k = 0; k < kSums; k++) {
     if ((PART == kIn && k != 2 && k != 3) || (PART == kOut && (k == 2 || k == 3))) continue;
+    if (k == 4 && !a.residual_per_channel) continue;
     if (!WIDE) {
       __syncthreads();
 #pragma unroll
-      for (int e = 0; e < kE; e++) fold[threadIdx.x * kE + e] = S[k][e];
+      for (int e = 0; e < kE; e++) fold[e * kThreads + threadIdx.x] = S[k][e];
       __syncthreads();
       for (int i = threadIdx.x; i < tpr * kE; i += kThreads) {
+        const int e = i / tpr, l = i - e * tpr, c = (e / W) * (tpr * W) + l * W + e % W;
         float s = 0.f;
-        for (int r = 0; r < rpw; r++) s += fold[r * tpr * kE + i];
-        if (i < C) dst[(size_t)k * C + i] = s;
+        for (int r = 0; r < rpw; r++) s += fold[e * kThreads + r * tpr + l];
+        if (c < C) dst[(size_t)k * C + c] = s;
       }
     } else {
 #pragma unroll
       for (int e = 0; e < kE; e++)
-        if (c0 + e < C) dst[(size_t)k * C + c0 + e] = S[k][e];
+        if (L.has(e)) dst[(size_t)k * C + L.ch(e)] = S[k][e];
     }
   }
 }
 
-// part [batch][slabs][kSums][C] -> sums [batch][kSums][C].  grid (C / 16, kSums, batch), 1024 threads: 16 channels x 64 rows
-__global__ __launch_bounds__(1024) void block_norm_sums_kernel(const float* part, float* sums, int slabs, int C, int parts) {
-  const int k = blockIdx.y;
-  if (((parts == kIn) && k != 2 && k != 3) || (parts == kOut && (k == 2 || k == 3))) return;
-  __shared__ float red[64][17];
-  const int c = blockIdx.x * 16 + (threadIdx.x & 15), r0 = threadIdx.x >> 4;
-  const int64_t sample = blockIdx.z;
-  float s = 0.f;
-  if (c < C)
-    for (int r = r0; r < slabs; r += 64) s += part[((sample * slabs + r) * kSums + k) * C + c];
-  red[r0][threadIdx.x & 15] = s;
-  __syncthreads();
-  if (threadIdx.x < 16 && c < C) {
-    float t = 0.f;
+__device__ __forceinline__ bool sum_used(int k, int parts, const gc_block_norm& a) {
+  return (k < 2 && parts != kIn) || ((k == 2 || k == 3) && parts != kOut) || (k == 4 && parts != kIn && a.residual_per_channel);
+}
+// N sums' column c of a sample's partials over its rows: 64 threads per column, every load independent (also of the sums that the parts
+// do not have, whose memory is there but was not written: nothing uses those totals)
+template <int N>
+__device__ __forceinline__ void column_sums(const float* part, int slabs, int C, int c, float (&total)[N], float (*red)[64][17]) {
+  const int r0 = threadIdx.x >> 4, lc = threadIdx.x & 15;
+  float s[N];
 #pragma unroll
-    for (int r = 0; r < 64; r++) t += red[r][threadIdx.x];
-    sums[(sample * kSums + k) * C + c] = t;
+  for (int k = 0; k < N; k++) s[k] = 0.f;
+  if (c < C) {
+#pragma unroll 4
+    for (int r = r0; r < slabs; r += 64)
+#pragma unroll
+      for (int k = 0; k < N; k++) s[k] += part[((size_t)r * kSums + k) * C + c];
+  }
+#pragma unroll
+  for (int k = 0; k < N; k++) red[k][r0][lc] = s[k];
+  __syncthreads();
+  for (int o = 32; o > 0; o >>= 1) {
+    if (r0 < o)
+#pragma unroll
+      for (int k = 0; k < N; k++) red[k][r0][lc] += red[k][r0 + o][lc];
+    __syncthreads();
+  }
+#pragma unroll
+  for (int k = 0; k < N; k++) total[k] = red[k][0][lc];
+}
+// the gradient of a scalar residual scale: the workgroups' shares in order
+__device__ __forceinline__ void scalar_rho(const gc_block_norm& a, const float* rho_part, int64_t n, float* red, int threads) {
+  float s = 0.f;
+  for (int64_t i = threadIdx.x; i < n; i += threads) s += rho_part[i];
+  s = lanes_sum(s, 64);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < threads / 64; w++) s += red[w];
+    a.d_residual_scale[0] = s;
+  }
+}
+
+// part [batch][slabs][kSums][C] -> sums [batch][kSums][C].  grid (C / 16, kSums, batch), 1024 threads: 16 channels x 64 rows
+__global__ __launch_bounds__(1024) void block_norm_sums_kernel(const gc_block_norm a, const float* part, float* sums, int slabs, int parts) {
+  const int k = blockIdx.y, C = a.cols;
+  if (!sum_used(k, parts, a)) return;
+  __shared__ float red[1][64][17];
+  const int c = blockIdx.x * 16 + (threadIdx.x & 15);
+  const int64_t sample = blockIdx.z;
+  float t[1];
+  column_sums<1>(part + (sample * slabs * kSums + k) * C, slabs, C, c, t, red);
+  if (threadIdx.x < 16 && c < C) sums[(sample * kSums + k) * C + c] = t[0];
+}
+
+// One sample (or one run of rows): the sums and the parameters' gradients in one launch.  Blocks of 16 channels x 64 rows; the last
+// block: a scalar residual scale.
+__global__ __launch_bounds__(1024) void block_norm_finish_kernel(const gc_block_norm a, const float* part, const float* rho_part, int slabs, int parts) {
+  __shared__ float red[kSums][64][17];
+  const int C = a.cols, c = blockIdx.x * 16 + (threadIdx.x & 15);
+  if (blockIdx.x == gridDim.x - 1) {
+    if (rho_part != nullptr) scalar_rho(a, rho_part, slabs, &red[0][0][0], 1024);
+    return;
+  }
+  float S[kSums];
+  column_sums<kSums>(part, slabs, C, c, S, red);
+  if (threadIdx.x >= 16 || c >= C) return;
+  if (parts != kIn) {
+    const float wo = a.out_weight ? a.out_weight[c] : 1.f, bo = a.out_bias ? a.out_bias[c] : 0.f, g = a.gate ? a.gate[c] : 1.f;
+    if (a.d_out_weight) a.d_out_weight[c] = g * S[0];
+    if (a.d_out_bias) a.d_out_bias[c] = g * S[1];
+    if (a.d_gate) a.d_gate[c] = wo * S[0] + bo * S[1];
+    if (a.residual_per_channel && a.d_residual_scale) a.d_residual_scale[c] = S[4];
+  }
+  if (parts != kOut) {
+    const float wi = a.in_weight ? a.in_weight[c] : 1.f, bi = a.in_bias ? a.in_bias[c] : 0.f, m = 1.f + (a.scale ? a.scale[c] : 0.f);
+    if (a.d_in_weight) a.d_in_weight[c] = m * S[2];
+    if (a.d_in_bias) a.d_in_bias[c] = m * S[3];
+    if (a.d_scale) a.d_scale[c] = wi * S[2] + bi * S[3];
+    if (a.d_shift) a.d_shift[c] = S[3];
   }
 }
 
 // Parameter gradients from the samples' sums.  Blocks 0 .. n - 1: 64 channels x 4 threads each; block n: the gradient of a
 // scalar residual scale.
-__global__ __launch_bounds__(kThreads) void block_norm_params_kernel(const gc_block_norm a, const float* sums, int parts) {
+__global__ __launch_bounds__(kThreads) void block_norm_params_kernel(const gc_block_norm a, const float* sums, const float* rho_part, int slabs, int parts) {
   __shared__ float red[5][4][64];
   const int C = a.cols;
   if (blockIdx.x == gridDim.x - 1) {
-    if (a.d_residual_scale == nullptr || a.residual_per_channel || parts == kIn) return;
-    float s = 0.f;
-    for (int64_t b = 0; b < a.batch; b++)
-      for (int c = threadIdx.x; c < C; c += kThreads) s += sums[(b * kSums + 4) * C + c];
-    float* r = &red[0][0][0];
-    r[threadIdx.x] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      float t = 0.f;
-      for (int i = 0; i < kThreads; i++) t += r[i];
-      a.d_residual_scale[0] = t;
-    }
+    if (rho_part != nullptr) scalar_rho(a, rho_part, a.batch * slabs, &red[0][0][0], kThreads);
     return;
   }
   const int lc = threadIdx.x & 63, q = threadIdx.x >> 6, c = blockIdx.x * 64 + lc;
   float acc[5] = {0.f, 0.f, 0.f, 0.f, 0.f};      // out_weight, out_bias, in_weight, in_bias, residual scale
-  float gsum = 0.f, ssum = 0.f, tsum = 0.f;       // gate, scale, shift where all samples share them (those have batch 1 or are summed)
+  float shared[3] = {0.f, 0.f, 0.f};              // gate, scale, shift that all samples share
   const float wo = c < C && a.out_weight ? a.out_weight[c] : 1.f, bo = c < C && a.out_bias ? a.out_bias[c] : 0.f;
   const float wi = c < C && a.in_weight ? a.in_weight[c] : 1.f, bi = c < C && a.in_bias ? a.in_bias[c] : 0.f;
   if (c < C)
+#pragma unroll 2
     for (int64_t b = q; b < a.batch; b += 4) {
       const float* S = sums + b * kSums * C + c;
       if (parts != kIn) {
         const float g = a.gate ? a.gate[(a.gate_per_sample ? b * C : 0) + c] : 1.f, s0 = S[0], s1 = S[C];
         acc[0] += g * s0;
         acc[1] += g * s1;
-        acc[4] += S[4 * C];
+        if (a.residual_per_channel) acc[4] += S[4 * C];
         const float dg = wo * s0 + bo * s1;
         if (a.gate_per_sample) { if (a.d_gate) a.d_gate[b * C + c] = dg; }
-        else gsum += dg;
+        else shared[0] += dg;
       }
       if (parts != kOut) {
         const float m = 1.f + (a.scale ? a.scale[(a.mod_per_sample ? b * C : 0) + c] : 0.f), s2 = S[2 * C], s3 = S[3 * C];
@@ -409,7 +546,7 @@ __global__ __launch_bounds__(kThreads) void block_norm_params_kernel(const gc_bl
         if (a.mod_per_sample) {
           if (a.d_scale) a.d_scale[b * C + c] = ds;
           if (a.d_shift) a.d_shift[b * C + c] = s3;
-        } else { ssum += ds; tsum += s3; }
+        } else { shared[1] += ds; shared[2] += s3; }
       }
     }
 #pragma unroll
@@ -422,9 +559,8 @@ __global__ __launch_bounds__(kThreads) void block_norm_params_kernel(const gc_bl
       if (dst[k]) dst[k][c] = ((red[k][0][lc] + red[k][1][lc]) + red[k][2][lc]) + red[k][3][lc];
   }
   __syncthreads();
-  red[0][q][lc] = gsum;
-  red[1][q][lc] = ssum;
-  red[2][q][lc] = tsum;
+#pragma unroll
+  for (int k = 0; k < 3; k++) red[k][q][lc] = shared[k];
   __syncthreads();
   if (q == 0 && c < C) {
     float* dst[3] = {a.gate_per_sample ? nullptr : a.d_gate, a.mod_per_sample ? nullptr : a.d_scale, a.mod_per_sample ? nullptr : a.d_shift};
@@ -460,42 +596,67 @@ int check_desc(const gc_block_norm* d, bool bwd, int& parts) {
   return GC_OK;
 }
 
-int slab_count(const gc_block_norm* d, int tpr, bool bwd) {
-  const int64_t rpw = tpr > 64 ? 1 : kThreads / tpr, passes = (d->rows + rpw - 1) / rpw;
-  // enough workgroups to fill the chip; the backward pass writes (and its second launch reads) one row of sums per workgroup
-  const int64_t fill = (int64_t)device_cu_count() * (bwd ? 4 : 8) * (tpr > kThreads ? 1 : 1);
-  int64_t s = (fill + d->batch - 1) / d->batch;
+// Workgroups per sample: at most `per_cu` per CU in all, so that every workgroup works on several rows (it reads the parameters once,
+// and its next rows are under way while it works).
+constexpr int kMostPerCu = 8;
+int slab_count(int64_t batch, int64_t rows, int tpr, int per_cu) {
+  const int64_t rpw = tpr > 64 ? 1 : kThreads / tpr, passes = (rows + rpw - 1) / rpw;
+  int64_t s = ((int64_t)device_cu_count() * per_cu + batch - 1) / batch;
   if (s > passes) s = passes;
   return (int)(s < 1 ? 1 : s);
 }
+int row_threads(int cols) {
+  int tpr = 1;
+  while (tpr * kE < cols) tpr *= 2;
+  return tpr;
+}
+// Workgroups of a kernel that a CU holds (asked once per kernel; 36 of them)
+int held_per_cu(const void* kernel, int threads) {
+  struct Entry { const void* kernel; int threads, n; };
+  static std::mutex mu;
+  static Entry known[64];
+  static int count = 0;
+  std::lock_guard<std::mutex> lock(mu);
+  for (int i = 0; i < count; i++)
+    if (known[i].kernel == kernel && known[i].threads == threads) return known[i].n;
+  int n = 0;
+  if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0) != hipSuccess || n < 1) n = 2;
+  if (n > kMostPerCu) n = kMostPerCu;
+  if (count < 64) known[count++] = Entry{kernel, threads, n};
+  return n;
+}
 
-NormParams make_params(const gc_block_norm* d, bool bwd) {
+NormParams make_params(const gc_block_norm* d) {
   NormParams P{};
   P.a = *d;
-  int tpr = 1;
-  while (tpr * kE < d->cols) tpr *= 2;
-  P.tpr = tpr;
-  const int unit = kE;
+  P.tpr = row_threads(d->cols);
+  const int unit = d->dtype == GC_F32 ? 4 : 8;             // 16 bytes
   P.vec = d->cols % unit == 0 && d->x_row_stride % unit == 0 && d->x_batch_stride % unit == 0 && d->f_row_stride % unit == 0 &&
           d->f_batch_stride % unit == 0 && aligned16(d->x) && aligned16(d->f) && aligned16(d->y) && aligned16(d->h) && aligned16(d->dy) &&
           aligned16(d->dh) && aligned16(d->dx) && aligned16(d->df);
-  P.slabs = slab_count(d, tpr, bwd);
   return P;
 }
 
-template <typename T, bool WIDE>
-void launch_fwd(const NormParams& P, int parts, hipStream_t s) {
-  const dim3 grid(P.slabs, (unsigned)P.a.batch), block(WIDE ? P.tpr : kThreads);
-  if (parts == kIn) hipLaunchKernelGGL((block_norm_fwd_kernel<T, WIDE, kIn>), grid, block, 0, s, P);
-  else if (parts == kOut) hipLaunchKernelGGL((block_norm_fwd_kernel<T, WIDE, kOut>), grid, block, 0, s, P);
-  else hipLaunchKernelGGL((block_norm_fwd_kernel<T, WIDE, kBoth>), grid, block, 0, s, P);
+typedef void (*NormKernel)(const NormParams);
+template <typename T, int MAXT, int W>
+NormKernel kernel_for(int parts, bool bwd) {
+  if (bwd) return parts == kIn ? block_norm_bwd_kernel<T, MAXT, kIn, W> : (parts == kOut ? block_norm_bwd_kernel<T, MAXT, kOut, W> : block_norm_bwd_kernel<T, MAXT, kBoth, W>);
+  return parts == kIn ? block_norm_fwd_kernel<T, MAXT, kIn, W> : (parts == kOut ? block_norm_fwd_kernel<T, MAXT, kOut, W> : block_norm_fwd_kernel<T, MAXT, kBoth, W>);
 }
-template <typename T, bool WIDE>
-void launch_bwd(const NormParams& P, int parts, hipStream_t s) {
-  const dim3 grid(P.slabs, (unsigned)P.a.batch), block(WIDE ? P.tpr : kThreads);
-  if (parts == kIn) hipLaunchKernelGGL((block_norm_bwd_kernel<T, WIDE, kIn>), grid, block, 0, s, P);
-  else if (parts == kOut) hipLaunchKernelGGL((block_norm_bwd_kernel<T, WIDE, kOut>), grid, block, 0, s, P);
-  else hipLaunchKernelGGL((block_norm_bwd_kernel<T, WIDE, kBoth>), grid, block, 0, s, P);
+template <typename T, int W>
+NormKernel kernel_width(int tpr, int parts, bool bwd) {
+  if (tpr <= 64) return kernel_for<T, kThreads, W>(parts, bwd);
+  return tpr <= 512 ? kernel_for<T, 512, W>(parts, bwd) : kernel_for<T, kMaxThreads, W>(parts, bwd);
+}
+// Launches the kernel for P (whose slabs it sets)
+int launch(NormParams& P, int parts, bool bwd, hipStream_t s) {
+  NormKernel k;
+  if (P.a.dtype == GC_F32) k = P.vec ? kernel_width<float, 4>(P.tpr, parts, bwd) : kernel_width<float, 1>(P.tpr, parts, bwd);
+  else k = P.vec ? kernel_width<uint16_t, 8>(P.tpr, parts, bwd) : kernel_width<uint16_t, 1>(P.tpr, parts, bwd);
+  const int threads = P.tpr > 64 ? P.tpr : kThreads;
+  P.slabs = slab_count(P.a.batch, P.a.rows, P.tpr, held_per_cu(reinterpret_cast<const void*>(k), threads));
+  hipLaunchKernelGGL(k, dim3(P.slabs, (unsigned)P.a.batch), dim3(threads), 0, s, P);
+  return check_hip(hipGetLastError(), bwd ? "block_norm bwd launch" : "block_norm fwd launch");
 }
 
 }  // namespace
@@ -507,22 +668,17 @@ extern "C" int gc_block_norm_fwd(const gc_block_norm* desc, void* stream) {
   int parts = 0;
   if (int e = check_desc(desc, false, parts)) return e;
   if (desc->batch == 0 || desc->rows == 0) return GC_OK;
-  const NormParams P = make_params(desc, false);
+  NormParams P = make_params(desc);
   hipStream_t s = (hipStream_t)stream;
   ProfScope ps("gc::block_norm_fwd_kernel", 0.0, s);
-  const bool wide = P.tpr > 64;
-  if (desc->dtype == GC_F32) { if (wide) launch_fwd<float, true>(P, parts, s); else launch_fwd<float, false>(P, parts, s); }
-  else { if (wide) launch_fwd<uint16_t, true>(P, parts, s); else launch_fwd<uint16_t, false>(P, parts, s); }
-  return check_hip(hipGetLastError(), "block_norm fwd launch");
+  return launch(P, parts, false, s);
 }
 
+// floats: the samples' sums, the scalar residual scale's shares, the workgroups' sums
 extern "C" size_t gc_block_norm_workspace_bytes(int64_t batch, int64_t rows, int32_t cols) {
   if (batch <= 0 || rows <= 0 || cols <= 0) return 0;
-  int tpr = 1;
-  while (tpr * kE < cols) tpr *= 2;
-  gc_block_norm d{};
-  d.batch = batch; d.rows = rows; d.cols = cols;
-  return ((size_t)batch * slab_count(&d, tpr, true) + batch) * kSums * (size_t)cols * sizeof(float);
+  const size_t wgs = (size_t)batch * slab_count(batch, rows, row_threads(cols), kMostPerCu);
+  return ((size_t)batch * kSums * cols + (wgs + 3) / 4 * 4 + wgs * kSums * cols) * sizeof(float);
 }
 
 extern "C" int gc_block_norm_bwd(const gc_block_norm* desc, void* workspace, size_t workspace_bytes, void* stream) {
@@ -537,24 +693,29 @@ extern "C" int gc_block_norm_bwd(const gc_block_norm* desc, void* workspace, siz
     set_error("block norm backward: a 16-byte aligned workspace of %zu bytes is needed", need);
     return GC_WORKSPACE_TOO_SMALL;
   }
-  NormParams P = make_params(desc, true);
+  NormParams P = make_params(desc);
+  const size_t wgs = (size_t)desc->batch * slab_count(desc->batch, desc->rows, P.tpr, kMostPerCu);
   float* sums = static_cast<float*>(workspace);
-  P.part = sums + (size_t)desc->batch * kSums * desc->cols;
+  const bool scalar = parts != kIn && desc->d_residual_scale != nullptr && !desc->residual_per_channel;
+  P.rho_part = scalar ? sums + (size_t)desc->batch * kSums * desc->cols : nullptr;
+  P.part = sums + (size_t)desc->batch * kSums * desc->cols + (wgs + 3) / 4 * 4;
   hipStream_t s = (hipStream_t)stream;
   {
     ProfScope ps("gc::block_norm_bwd_kernel", 0.0, s);
-    const bool wide = P.tpr > 64;
-    if (desc->dtype == GC_F32) { if (wide) launch_bwd<float, true>(P, parts, s); else launch_bwd<float, false>(P, parts, s); }
-    else { if (wide) launch_bwd<uint16_t, true>(P, parts, s); else launch_bwd<uint16_t, false>(P, parts, s); }
-    if (check_hip(hipGetLastError(), "block_norm bwd launch")) return GC_HIP_ERROR;
+    if (int e = launch(P, parts, true, s)) return e;
+  }
+  if (desc->batch == 1) {
+    hipLaunchKernelGGL(block_norm_finish_kernel, dim3((desc->cols + 15) / 16 + 1), dim3(1024), 0, s, *desc, (const float*)P.part, (const float*)P.rho_part,
+                       P.slabs, parts);
+    return check_hip(hipGetLastError(), "block_norm finish launch");
   }
   const float* totals = P.part;
   if (P.slabs > 1) {
-    hipLaunchKernelGGL(block_norm_sums_kernel, dim3((desc->cols + 15) / 16, kSums, (unsigned)desc->batch), dim3(1024), 0, s, (const float*)P.part,
-                       sums, P.slabs, desc->cols, parts);
+    hipLaunchKernelGGL(block_norm_sums_kernel, dim3((desc->cols + 15) / 16, kSums, (unsigned)desc->batch), dim3(1024), 0, s, *desc, (const float*)P.part,
+                       sums, P.slabs, parts);
     if (check_hip(hipGetLastError(), "block_norm sums launch")) return GC_HIP_ERROR;
     totals = sums;
   }
-  hipLaunchKernelGGL(block_norm_params_kernel, dim3((desc->cols + 63) / 64 + 1), dim3(kThreads), 0, s, *desc, totals, parts);
+  hipLaunchKernelGGL(block_norm_params_kernel, dim3((desc->cols + 63) / 64 + 1), dim3(kThreads), 0, s, *desc, totals, (const float*)P.rho_part, P.slabs, parts);
   return check_hip(hipGetLastError(), "block_norm params launch");
 }

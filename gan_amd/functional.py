@@ -214,7 +214,8 @@ def block_output_norm(x, f, weight=None, bias=None, *, gate=None, residual_scale
     """The norm behind a transformer block, its gate and the residual sum: residual_scale * x + gate * (norm(f) * weight + bias)
     for the residual stream x and the block's output f, both [B, ..., C].  gate: [C] or [B, C]; residual_scale: a number, or a
     tensor of one element or [C].  Otherwise as block_input_norm."""
-    token_ops._require(f is not None, "block_output_norm: f must be a tensor")
+    if f is None:
+        raise RuntimeError("ganconv: block_output_norm: f must be a tensor")
     return token_ops.block_norm("block_output_norm", x, f, weight, bias, gate, residual_scale, None, None, None, None, kind, eps, False)
 
 
@@ -223,7 +224,8 @@ def block_boundary_norm(x, f, out_weight=None, in_weight=None, out_bias=None, in
     """The boundary between two transformer blocks as one sweep: y = block_output_norm(x, f, out_weight, out_bias, ...), the
     residual stream behind the first, and h = block_input_norm(y, in_weight, in_bias, ...), what the second reads.  Returns
     (y, h).  h is computed from y before y is rounded to its storage type."""
-    token_ops._require(f is not None, "block_boundary_norm: f must be a tensor")
+    if f is None:
+        raise RuntimeError("ganconv: block_boundary_norm: f must be a tensor")
     return token_ops.block_norm("block_boundary_norm", x, f, out_weight, out_bias, gate, residual_scale, in_weight, in_bias, scale, shift, kind,
                                 eps, True)
 

@@ -218,15 +218,21 @@ def test_block_norm_gradients_against_differences(F):
 
 @pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
 def test_block_norm_of_strided_and_shifted_tensors(F, dt):
-    """Slices of wider tensors, a channels-last image, an odd offset, a transposed view: the values of the contiguous copy."""
+    """Slices of wider tensors, a channels-last image, an odd offset, a transposed view: the definition on the view's values (an odd
+    offset or stride takes narrower accesses and another order of the sums, which the counted bound covers)."""
     g = torch.Generator().manual_seed(1)
     wide = torch.randn(3, 10, 200, generator=g).to(dt).cuda()
     w = torch.randn(64, generator=g).cuda()
     for view in (wide[:, 2:9, 64:128], wide[..., 3:67], wide[:, ::2, :64], wide[1:2].expand(3, 10, 200)[..., :64], wide.transpose(0, 1)[..., 64:128]):
-        a = F.block_input_norm(view, w, kind="layer")
-        assert a.is_contiguous() and torch.equal(a, F.block_input_norm(view.contiguous().clone(), w, kind="layer"))
-        y = F.block_output_norm(view, view.flip(0), w, gate=w)
-        assert torch.equal(y, F.block_output_norm(view.contiguous(), view.flip(0).contiguous(), w, gate=w))
+        a = F.block_input_norm(view, w, kind="layer", eps=1e-5)
+        outs, mags, _, _ = _norm_reference(view.cpu(), None, {"in_weight": w.cpu()}, "layer", 1e-5, None, view.cpu())
+        assert a.is_contiguous()
+        _check("h", a, outs["h"], DEPTH * mags["h"], dt)
+        y = F.block_output_norm(view, view.flip(0), w, gate=w, eps=1e-5)
+        outs, mags, _, _ = _norm_reference(view.cpu(), view.flip(0).cpu(), {"out_weight": w.cpu(), "gate": w.cpu()}, "rms", 1e-5, view.cpu(), None)
+        _check("y", y, outs["y"], DEPTH * mags["y"], dt)
+    same = wide[:, 2:9, 64:128]                                                  # the same accesses: the same bits
+    assert torch.equal(F.block_input_norm(same, w), F.block_input_norm(same.contiguous(), w))
     img = torch.randn(2, 64, 6, 5, generator=g).to(dt).cuda().contiguous(memory_format=torch.channels_last)
     t = F.block_input_norm(img.permute(0, 2, 3, 1), w)
     assert t.permute(0, 3, 1, 2).is_contiguous(memory_format=torch.channels_last)

@@ -174,5 +174,24 @@ def test_layout_helpers():
     assert v.is_contiguous()
     assert token_ops._strides(torch.zeros(4, 1, 8).expand(4, 1, 8).as_strided((4, 1, 8), (8, 3, 1))) == [8, 8, 1]
     q = torch.zeros(2, 1, 3, 2, 32, dtype=torch.bfloat16)
-    assert token_ops._aligned(q, 32) is q
-    assert token_ops._aligned(q.expand(2, 5, 3, 2, 32), 32).is_contiguous()
+    assert token_ops._aligned(q, 32)[0] is q and token_ops._aligned(q, 32)[1] == [192, 192, 64, 32]
+    assert token_ops._aligned(q.expand(2, 5, 3, 2, 32), 32)[0].is_contiguous()
+    wide = torch.zeros(2, 4, 3, 2, 40, dtype=torch.bfloat16)[..., :32]
+    v, st = token_ops._aligned(wide, 32)
+    assert v.data_ptr() == wide.data_ptr() and st == [960, 240, 80, 40]
+    assert token_ops._aligned(wide[..., 1:], 31)[0].is_contiguous()
+
+
+def test_packed_descriptors_match_the_structures():
+    """The one-line packings against the field-by-field structures of the C ABI."""
+    for packer, cls in ((token_ops._NORM, _lib.BlockNorm), (token_ops._ROTARY, _lib.Rotary), (token_ops._ATTENTION, _lib.DiffAttention)):
+        assert packer.size == ctypes.sizeof(cls)
+        flat = []
+        for name, kind in cls._fields_:
+            n = getattr(kind, "_length_", 1)
+            flat += [(name, i if n > 1 else None) for i in range(n)]
+        values = [float(i + 1) if getattr(cls, name).size == 4 and dict(cls._fields_)[name] is ctypes.c_float else i + 1 for i, (name, _) in enumerate(flat)]
+        d = cls.from_buffer_copy(packer.pack(*values))
+        for (name, i), value in zip(flat, values):
+            got = getattr(d, name) if i is None else getattr(d, name)[i]
+            assert got == value, (cls.__name__, name, i)
