@@ -431,31 +431,34 @@ __global__ __launch_bounds__(MAXT) void block_norm_bwd_kernel(const NormParams P
 __device__ __forceinline__ bool sum_used(int k, int parts, const gc_block_norm& a) {
   return (k < 2 && parts != kIn) || ((k == 2 || k == 3) && parts != kOut) || (k == 4 && parts != kIn && a.residual_per_channel);
 }
-// N sums' column c of a sample's partials over its rows: 64 threads per column, every load independent (also of the sums that the parts
+// N sums' column c of a sample's partials over its rows: 128 threads per column (8 columns a workgroup: one CU takes 16 cycles for every
+// wave's load, so the work has to be spread), every load independent (also of the sums that the parts
 // do not have, whose memory is there but was not written: nothing uses those totals)
 template <int N>
-__device__ __forceinline__ void column_sums(const float* part, int slabs, int C, int c, float (&total)[N], float (*red)[64][17]) {
-  const int r0 = threadIdx.x >> 4, lc = threadIdx.x & 15;
+__device__ __forceinline__ void column_sums(const float* part, int slabs, int C, int c, float (&total)[N], float (*red)[16][8]) {
+  const int r0 = threadIdx.x >> 3, lc = threadIdx.x & 7;
   float s[N];
 #pragma unroll
   for (int k = 0; k < N; k++) s[k] = 0.f;
   if (c < C) {
-#pragma unroll 4
-    for (int r = r0; r < slabs; r += 64)
+#pragma unroll 8
+    for (int r = r0; r < slabs; r += 128)
 #pragma unroll
       for (int k = 0; k < N; k++) s[k] += part[((size_t)r * kSums + k) * C + c];
   }
 #pragma unroll
-  for (int k = 0; k < N; k++) red[k][r0][lc] = s[k];
-  __syncthreads();
-  for (int o = 32; o > 0; o >>= 1) {
-    if (r0 < o)
-#pragma unroll
-      for (int k = 0; k < N; k++) red[k][r0][lc] += red[k][r0 + o][lc];
-    __syncthreads();
+  for (int k = 0; k < N; k++) {
+    s[k] = dpp_add<0x128>(s[k]);                           // the other 8 lanes of 16, the other 16 of 32, the other half
+    s[k] = swap_add<true>(swap_add<false>(s[k]));
+    if ((threadIdx.x & 63) < 8) red[k][threadIdx.x >> 6][lc] = s[k];
   }
+  __syncthreads();
 #pragma unroll
-  for (int k = 0; k < N; k++) total[k] = red[k][0][lc];
+  for (int k = 0; k < N; k++) {
+    total[k] = 0.f;
+#pragma unroll
+    for (int w = 0; w < 16; w++) total[k] += red[k][w][lc];
+  }
 }
 // the gradient of a scalar residual scale: the workgroups' shares in order
 __device__ __forceinline__ void scalar_rho(const gc_block_norm& a, const float* rho_part, int64_t n, float* red, int threads) {
@@ -471,30 +474,30 @@ __device__ __forceinline__ void scalar_rho(const gc_block_norm& a, const float* 
   }
 }
 
-// part [batch][slabs][kSums][C] -> sums [batch][kSums][C].  grid (C / 16, kSums, batch), 1024 threads: 16 channels x 64 rows
+// part [batch][slabs][kSums][C] -> sums [batch][kSums][C].  grid (C / 8, kSums, batch), 1024 threads: 8 channels x 128 rows
 __global__ __launch_bounds__(1024) void block_norm_sums_kernel(const gc_block_norm a, const float* part, float* sums, int slabs, int parts) {
   const int k = blockIdx.y, C = a.cols;
   if (!sum_used(k, parts, a)) return;
-  __shared__ float red[1][64][17];
-  const int c = blockIdx.x * 16 + (threadIdx.x & 15);
+  __shared__ float red[1][16][8];
+  const int c = blockIdx.x * 8 + (threadIdx.x & 7);
   const int64_t sample = blockIdx.z;
   float t[1];
   column_sums<1>(part + (sample * slabs * kSums + k) * C, slabs, C, c, t, red);
-  if (threadIdx.x < 16 && c < C) sums[(sample * kSums + k) * C + c] = t[0];
+  if (threadIdx.x < 8 && c < C) sums[(sample * kSums + k) * C + c] = t[0];
 }
 
-// One sample (or one run of rows): the sums and the parameters' gradients in one launch.  Blocks of 16 channels x 64 rows; the last
+// One sample (or one run of rows): the sums and the parameters' gradients in one launch.  Blocks of 8 channels x 128 rows; the last
 // block: a scalar residual scale.
 __global__ __launch_bounds__(1024) void block_norm_finish_kernel(const gc_block_norm a, const float* part, const float* rho_part, int slabs, int parts) {
-  __shared__ float red[kSums][64][17];
-  const int C = a.cols, c = blockIdx.x * 16 + (threadIdx.x & 15);
+  __shared__ float red[kSums][16][8];
+  const int C = a.cols, c = blockIdx.x * 8 + (threadIdx.x & 7);
   if (blockIdx.x == gridDim.x - 1) {
     if (rho_part != nullptr) scalar_rho(a, rho_part, slabs, &red[0][0][0], 1024);
     return;
   }
   float S[kSums];
   column_sums<kSums>(part, slabs, C, c, S, red);
-  if (threadIdx.x >= 16 || c >= C) return;
+  if (threadIdx.x >= 8 || c >= C) return;
   if (parts != kIn) {
     const float wo = a.out_weight ? a.out_weight[c] : 1.f, bo = a.out_bias ? a.out_bias[c] : 0.f, g = a.gate ? a.gate[c] : 1.f;
     if (a.d_out_weight) a.d_out_weight[c] = g * S[0];
@@ -705,13 +708,13 @@ extern "C" int gc_block_norm_bwd(const gc_block_norm* desc, void* workspace, siz
     if (int e = launch(P, parts, true, s)) return e;
   }
   if (desc->batch == 1) {
-    hipLaunchKernelGGL(block_norm_finish_kernel, dim3((desc->cols + 15) / 16 + 1), dim3(1024), 0, s, *desc, (const float*)P.part, (const float*)P.rho_part,
+    hipLaunchKernelGGL(block_norm_finish_kernel, dim3((desc->cols + 7) / 8 + 1), dim3(1024), 0, s, *desc, (const float*)P.part, (const float*)P.rho_part,
                        P.slabs, parts);
     return check_hip(hipGetLastError(), "block_norm finish launch");
   }
   const float* totals = P.part;
   if (P.slabs > 1) {
-    hipLaunchKernelGGL(block_norm_sums_kernel, dim3((desc->cols + 15) / 16, kSums, (unsigned)desc->batch), dim3(1024), 0, s, *desc, (const float*)P.part,
+    hipLaunchKernelGGL(block_norm_sums_kernel, dim3((desc->cols + 7) / 8, kSums, (unsigned)desc->batch), dim3(1024), 0, s, *desc, (const float*)P.part,
                        sums, P.slabs, parts);
     if (check_hip(hipGetLastError(), "block_norm sums launch")) return GC_HIP_ERROR;
     totals = sums;

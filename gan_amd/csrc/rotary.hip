@@ -17,7 +17,7 @@ namespace gc {
 namespace {
 
 constexpr int kMaxPairs = 256;
-constexpr int kTableBytes = 32768;         // cos / sin of tokens x pairs
+constexpr int kTableBytes = 32768;         // cos / sin of tokens x pairs, at most
 
 struct RotaryParams {
   gc_rotary a;
@@ -35,28 +35,25 @@ template <typename T> __device__ __forceinline__ void put1(void* p, int64_t i, f
   if constexpr (sizeof(T) == 4) static_cast<float*>(p)[i] = v;
   else static_cast<uint16_t*>(p)[i] = float_to_bf16_bits(v);
 }
-template <typename T> __device__ __forceinline__ void get8(const void* p, int64_t i, float (&v)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    const f32x4 a = load4<T>(p, i), b = load4<T>(p, i + 4);
+// 16 bytes: W = 4 (fp32) or 8 (bf16) elements
+template <typename T> struct Vec { static constexpr int W = 16 / sizeof(T); u32x4 q; };
+template <typename T> __device__ __forceinline__ Vec<T> get(const void* p, int64_t i) {
+  return Vec<T>{*reinterpret_cast<const u32x4*>(static_cast<const T*>(p) + i)};
+}
+template <typename T> __device__ __forceinline__ void widen(const Vec<T>& v, float (&f)[Vec<T>::W]) {
 #pragma unroll
-    for (int e = 0; e < 4; e++) { v[e] = a[e]; v[4 + e] = b[e]; }
-  } else {
-    const u32x4 q = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p) + i);
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      v[2 * e] = __builtin_bit_cast(float, q[e] << 16);
-      v[2 * e + 1] = __builtin_bit_cast(float, q[e] & 0xffff0000u);
-    }
+  for (int e = 0; e < Vec<T>::W; e++) {
+    if constexpr (sizeof(T) == 4) { const uint32_t u = v.q[e]; f[e] = __builtin_bit_cast(float, u); }
+    else f[e] = __builtin_bit_cast(float, (e & 1) ? (v.q[e / 2] & 0xffff0000u) : (v.q[e / 2] << 16));
   }
 }
-template <typename T> __device__ __forceinline__ void put8(void* p, int64_t i, const float (&v)[8]) {
-  const f32x4 a = {v[0], v[1], v[2], v[3]}, b = {v[4], v[5], v[6], v[7]};
+template <typename T> __device__ __forceinline__ void put(void* p, int64_t i, const float (&v)[Vec<T>::W]) {
+  T* d = static_cast<T*>(p) + i;
   if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<f32x4*>(static_cast<float*>(p) + i) = a;
-    *reinterpret_cast<f32x4*>(static_cast<float*>(p) + i + 4) = b;
+    *reinterpret_cast<f32x4*>(d) = f32x4{v[0], v[1], v[2], v[3]};
   } else {
-    const u32x2 lo = cvt_bf16x4(a), hi = cvt_bf16x4(b);
-    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p) + i) = u32x4{lo[0], lo[1], hi[0], hi[1]};
+    const u32x2 lo = cvt_bf16x4(f32x4{v[0], v[1], v[2], v[3]}), hi = cvt_bf16x4(f32x4{v[4], v[5], v[6], v[7]});
+    *reinterpret_cast<u32x4*>(d) = u32x4{lo[0], lo[1], hi[0], hi[1]};
   }
 }
 
@@ -69,11 +66,12 @@ __device__ __forceinline__ double position_at(const gc_rotary& a, int64_t i) {
   }
 }
 
-// A work item of a head: VEC: 8 neighbouring elements (NEIGHBOURS) or 8 elements of the first half and their partners, then
-// chunks of 8 elements that pass through; otherwise one pair, then single elements that pass through.
+// A work item of a head: VEC: 16 bytes of neighbouring elements (NEIGHBOURS), or 16 bytes of the first half and their partners, then
+// 16-byte runs that pass through; otherwise one pair, then single elements that pass through.
 template <typename T, bool VEC, bool NEIGHBOURS>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryParams P) {
-  __shared__ float2 table[kTableBytes / sizeof(float2)];        // [token][pair]: cos, sin
+  extern __shared__ float2 table[];                        // [token][pair]: cos, sin
+  constexpr int W = Vec<T>::W;
   const gc_rotary& a = P.a;
   const int np = a.pairs;
   const int64_t n0 = (int64_t)blockIdx.x * P.tokens;
@@ -92,64 +90,72 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryParams P) 
   __syncthreads();
 
   const int units = (int)P.units_row.d, per_head = (int)P.units_head.d;
-  const int turn_units = VEC ? (NEIGHBOURS ? np / 4 : np / 8) : np;
-  for (int b = 0; b < nb; b++)
-    for (int i = threadIdx.x; i < nt * units; i += kThreads) {
-      const int t = (int)fd_div((uint32_t)i, P.units_row);
-      int u = i - t * units;
-      const bool is_q = u < P.q_units;
-      if (!is_q) u -= P.q_units;
-      const int head = (int)fd_div((uint32_t)u, P.units_head), c = u - head * per_head;
-      const int64_t sb = b0 + b, n = n0 + t;
-      const void* src = is_q ? a.q : a.k;
-      void* dst = is_q ? a.q_out : a.k_out;
-      const int64_t* st = is_q ? a.q_stride : a.k_stride;
-      const int heads = is_q ? a.q_heads : a.k_heads;
-      const int64_t in = sb * st[0] + n * st[1] + head * st[2];
-      const int64_t out = ((sb * a.tokens + n) * heads + head) * a.dim;
-      const float2* cs = table + t * np;
-      if (VEC) {
-        if (c < turn_units) {
-          if (NEIGHBOURS) {
-            float v[8], w[8];
-            get8<T>(src, in + c * 8, v);
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-              const float2 z = cs[c * 4 + e];
-              w[2 * e] = v[2 * e] * z.x - v[2 * e + 1] * z.y;
-              w[2 * e + 1] = v[2 * e] * z.y + v[2 * e + 1] * z.x;
-            }
-            put8<T>(dst, out + c * 8, w);
-          } else {
-            float x[8], y[8], wx[8], wy[8];
-            get8<T>(src, in + c * 8, x);
-            get8<T>(src, in + np + c * 8, y);
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-              const float2 z = cs[c * 8 + e];
-              wx[e] = x[e] * z.x - y[e] * z.y;
-              wy[e] = x[e] * z.y + y[e] * z.x;
-            }
-            put8<T>(dst, out + c * 8, wx);
-            put8<T>(dst, out + np + c * 8, wy);
-          }
-        } else {
-          const int64_t o = 2 * np + (int64_t)(c - turn_units) * 8;
-          float v[8];
-          get8<T>(src, in + o, v);
-          put8<T>(dst, out + o, v);
+  const int turn_units = VEC ? np * (NEIGHBOURS ? 2 : 1) / W : np;
+  const int items = nt * units;
+  for (int i = threadIdx.x; i < items; i += kThreads) {
+    const int t = (int)fd_div((uint32_t)i, P.units_row);
+    int u = i - t * units;
+    const bool is_q = u < P.q_units;
+    if (!is_q) u -= P.q_units;
+    const int head = (int)fd_div((uint32_t)u, P.units_head), c = u - head * per_head;
+    const int64_t n = n0 + t;
+    const void* src = is_q ? a.q : a.k;
+    void* dst = is_q ? a.q_out : a.k_out;
+    const int64_t* st = is_q ? a.q_stride : a.k_stride;
+    const int heads = is_q ? a.q_heads : a.k_heads;
+    const int64_t out_step = a.tokens * heads * a.dim, in_step = st[0];
+    int64_t in = b0 * in_step + n * st[1] + head * st[2], out = b0 * out_step + (n * heads + head) * a.dim;
+    const float2* cs = table + t * np;
+    if (VEC) {
+      const bool turned = c < turn_units;
+      const int x0 = turned ? c * W : 2 * np + (c - turn_units) * W, y0 = NEIGHBOURS || !turned ? x0 : np + x0;
+      // all samples of this item: the next sample's elements are asked for before this one's are turned
+      Vec<T> vx = get<T>(src, in + x0), vy = vx;
+      if (!NEIGHBOURS) vy = get<T>(src, in + y0);
+      for (int b = 0; b < nb; b++, in += in_step, out += out_step) {
+        float x[W], y[W];
+        widen<T>(vx, x);
+        widen<T>(vy, y);
+        if (b + 1 < nb) {
+          vx = get<T>(src, in + in_step + x0);
+          if (!NEIGHBOURS) vy = get<T>(src, in + in_step + y0);
         }
-      } else if (c < turn_units) {
-        const int i0 = NEIGHBOURS ? 2 * c : c, i1 = NEIGHBOURS ? 2 * c + 1 : np + c;
-        const float x = get1<T>(src, in + i0), y = get1<T>(src, in + i1);
-        const float2 z = cs[c];
-        put1<T>(dst, out + i0, x * z.x - y * z.y);
-        put1<T>(dst, out + i1, x * z.y + y * z.x);
-      } else {
-        const int64_t o = 2 * np + (c - turn_units);
-        put1<T>(dst, out + o, get1<T>(src, in + o));
+        if (turned) {
+          if (NEIGHBOURS) {
+#pragma unroll
+            for (int e = 0; e < W / 2; e++) {
+              const float2 z = cs[c * (W / 2) + e];
+              y[2 * e] = x[2 * e] * z.x - x[2 * e + 1] * z.y;
+              y[2 * e + 1] = x[2 * e] * z.y + x[2 * e + 1] * z.x;
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < W; e++) {
+              const float2 z = cs[c * W + e];
+              const float r = x[e] * z.x - y[e] * z.y;
+              y[e] = x[e] * z.y + y[e] * z.x;
+              x[e] = r;
+            }
+            put<T>(dst, out + x0, x);
+          }
+        }
+        put<T>(dst, out + y0, y);
+      }
+    } else {
+      for (int b = 0; b < nb; b++, in += in_step, out += out_step) {
+        if (c < turn_units) {
+          const int i0 = NEIGHBOURS ? 2 * c : c, i1 = NEIGHBOURS ? 2 * c + 1 : np + c;
+          const float x = get1<T>(src, in + i0), y = get1<T>(src, in + i1);
+          const float2 z = cs[c];
+          put1<T>(dst, out + i0, x * z.x - y * z.y);
+          put1<T>(dst, out + i1, x * z.y + y * z.x);
+        } else {
+          const int64_t o = 2 * np + (c - turn_units);
+          put1<T>(dst, out + o, get1<T>(src, in + o));
+        }
       }
     }
+  }
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -174,12 +180,13 @@ extern "C" int gc_axial_rotary(const gc_rotary* d, void* stream) {
     return GC_UNSUPPORTED_GEOMETRY;
   }
   if (d->batch == 0 || d->tokens == 0) return GC_OK;
-  bool vec = d->dim % 8 == 0 && d->pairs % (d->halves ? 8 : 4) == 0 && aligned16(d->q) && aligned16(d->k) && aligned16(d->q_out) && aligned16(d->k_out);
-  for (int i = 0; i < 3; i++) vec = vec && d->q_stride[i] % 8 == 0 && (d->k_heads == 0 || d->k_stride[i] % 8 == 0);
+  const int W = d->dtype == GC_F32 ? 4 : 8;
+  bool vec = d->dim % W == 0 && d->pairs % (d->halves ? W : W / 2) == 0 && aligned16(d->q) && aligned16(d->k) && aligned16(d->q_out) && aligned16(d->k_out);
+  for (int i = 0; i < 3; i++) vec = vec && d->q_stride[i] % W == 0 && (d->k_heads == 0 || d->k_stride[i] % W == 0);
   RotaryParams P{};
   P.a = *d;
   const int rest = d->dim - 2 * d->pairs;
-  const int per_head = vec ? (d->halves ? d->pairs / 8 : d->pairs / 4) + rest / 8 : d->pairs + rest;
+  const int per_head = vec ? (d->halves ? d->pairs : 2 * d->pairs) / W + rest / W : d->pairs + rest;
   const int heads = d->q_heads + d->k_heads;
   P.units_head = make_fastdiv((uint32_t)per_head);
   P.units_row = make_fastdiv((uint32_t)(per_head * heads));
@@ -202,16 +209,17 @@ extern "C" int gc_axial_rotary(const gc_rotary* d, void* stream) {
   const int64_t gx = (d->tokens + tok - 1) / tok;
   if (gx >= (1ll << 31)) { set_error("axial rotary: too many tokens (%lld)", (long long)d->tokens); return GC_UNSUPPORTED_GEOMETRY; }
   const dim3 grid((unsigned)gx, (unsigned)((d->batch + P.samples - 1) / P.samples));
+  const size_t lds = (size_t)P.tokens * d->pairs * sizeof(float2);
   hipStream_t s = (hipStream_t)stream;
   ProfScope ps("gc::rotary_kernel", 0.0, s);
 #define GC_ROTARY(T)                                                                                                          \
   do {                                                                                                                        \
     if (vec) {                                                                                                                \
-      if (d->halves) hipLaunchKernelGGL((rotary_kernel<T, true, false>), grid, dim3(kThreads), 0, s, P);                      \
-      else hipLaunchKernelGGL((rotary_kernel<T, true, true>), grid, dim3(kThreads), 0, s, P);                                 \
+      if (d->halves) hipLaunchKernelGGL((rotary_kernel<T, true, false>), grid, dim3(kThreads), lds, s, P);                    \
+      else hipLaunchKernelGGL((rotary_kernel<T, true, true>), grid, dim3(kThreads), lds, s, P);                               \
     } else {                                                                                                                  \
-      if (d->halves) hipLaunchKernelGGL((rotary_kernel<T, false, false>), grid, dim3(kThreads), 0, s, P);                     \
-      else hipLaunchKernelGGL((rotary_kernel<T, false, true>), grid, dim3(kThreads), 0, s, P);                                \
+      if (d->halves) hipLaunchKernelGGL((rotary_kernel<T, false, false>), grid, dim3(kThreads), lds, s, P);                   \
+      else hipLaunchKernelGGL((rotary_kernel<T, false, true>), grid, dim3(kThreads), lds, s, P);                              \
     }                                                                                                                         \
   } while (0)
   if (d->dtype == GC_F32) GC_ROTARY(float);

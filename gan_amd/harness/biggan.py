@@ -19,7 +19,8 @@ quarter of the pixels).
 
 Options (off by default): set_activation_dtype(torch.bfloat16) stores activations in bf16 between layers;
 set_fused_attention(True) computes softmax(K Q) V with ops.attention, which never materialises the [B, 4096, 4096]
-weights.  Phases: hinge loss of BasicGANs/loss_functions.py:79-99, step order and orthogonal regularisation of
+weights.  Generator / Discriminator(attention="differential") put a differential-attention block where the reference has its
+self-attention block (other parameters; default "self").  Phases: hinge loss of BasicGANs/loss_functions.py:79-99, step order and orthogonal regularisation of
 BigGAN/train.py:115-127, 187-226.
 """
 import contextlib
@@ -229,6 +230,24 @@ class SelfAttentionBlock(torch.nn.Module):
         return torch.addcmul(x, mixed, self.gamma.to(mixed.dtype))
 
 
+class _SpectralHeads(gnn._DifferentialHeads):
+    def _project(self, conv, x, dtype):
+        return conv(x, out_dtype=dtype)
+
+
+class DifferentialAttentionBlock(gnn.DifferentialAttention2d):
+    """EXTENSION: differential attention with rotary positions and norms around it in the place of SelfAttentionBlock, on
+    spectrally normalised projections (Generator / Discriminator with attention="differential")."""
+
+    block_type = _SpectralHeads
+
+    def __init__(self, channels):
+        super().__init__(channels, conv=Conv2d)
+
+
+ATTENTION_BLOCKS = {"self": SelfAttentionBlock, "differential": DifferentialAttentionBlock}
+
+
 class GeneratorBlock(torch.nn.Module):
     """norm-relu-upsample-conv3x3-norm-relu-conv3x3 plus a 1x1 shortcut on the up-scaled input (BigGAN/model.py:100-133)."""
 
@@ -285,12 +304,12 @@ class DiscriminatorBlock(torch.nn.Module):
 
 
 class Generator(torch.nn.Module):
-    def __init__(self, n_classes=1000, ch=96):
+    def __init__(self, n_classes=1000, ch=96, attention="self"):
         super().__init__()
         self.linear_y = torch.nn.Embedding(n_classes, 128)
         self.linear_z = Linear(20, 4 * 4 * 16 * ch)
         self.main_sequence = torch.nn.ModuleList(
-            SelfAttentionBlock(2 * ch) if spec == "attention" else GeneratorBlock(spec[0] * ch, spec[1] * ch) for spec in GENERATOR_PLAN)
+            ATTENTION_BLOCKS[attention](2 * ch) if spec == "attention" else GeneratorBlock(spec[0] * ch, spec[1] * ch) for spec in GENERATOR_PLAN)
         self.bn = torch.nn.BatchNorm2d(ch)
         self.to_RGB_layer = Conv2d(ch, 3, 1)
 
@@ -313,12 +332,12 @@ class Generator(torch.nn.Module):
 
 
 class Discriminator(torch.nn.Module):
-    def __init__(self, n_classes=1000, ch=64, image_dim=3):
+    def __init__(self, n_classes=1000, ch=64, image_dim=3, attention="self"):
         super().__init__()
         blocks = []
         for spec in CRITIC_PLAN:
             if spec == "attention":
-                blocks.append(SelfAttentionBlock(ch))
+                blocks.append(ATTENTION_BLOCKS[attention](ch))
             else:
                 blocks.append(DiscriminatorBlock(image_dim if spec[0] is None else spec[0] * ch, spec[1] * ch, spec[2]))
         self.main_sequence = torch.nn.ModuleList(blocks)

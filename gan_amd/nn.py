@@ -11,6 +11,7 @@ Reference call sites: BasicGANs/models.py:35,77; Pix2Pix/models.py:17,83,123-124
 """
 import contextlib
 import weakref
+from copy import deepcopy as _deepcopy
 
 import torch
 
@@ -267,6 +268,124 @@ class BatchNormAct2d(torch.nn.Module):
     def extra_repr(self):
         return (f"{self.num_features}, eps={self.eps}, momentum={self.momentum}, affine={self.affine}, "
                 f"track_running_stats={self.track_running_stats}, activation={self.activation}")
+
+
+class AxialRotary(torch.nn.Module):
+    """EXTENSION (the reference's attention has no positions): rotary positions with several axes for the heads of q and k, see
+    functional.axial_rotary.  dims: rotated elements per axis; forward(q, k, positions).  Holds no parameters or buffers."""
+
+    def __init__(self, dims, base=10000.0, interleaved=True):
+        super().__init__()
+        self.dims, self.base, self.interleaved = tuple(dims), base, interleaved
+        self._tables = {}
+
+    def forward(self, q, k, positions):
+        table = self._tables.get(q.device)
+        if table is None:
+            table = self._tables[q.device] = F.rotary_table(self.dims, self.base, self.interleaved, q.device)
+        return F.axial_rotary(q, k, positions, table)
+
+    def __deepcopy__(self, memo):
+        return AxialRotary(self.dims, self.base, self.interleaved)
+
+    def extra_repr(self):
+        return f"dims={self.dims}, base={self.base}, interleaved={self.interleaved}"
+
+
+class _DifferentialHeads(torch.nn.Module):
+    """One block's computation between its two norms: projections, rotary positions, differential attention, a norm per head, and
+    the projection back."""
+
+    def __init__(self, channels, heads, conv, rotary, lambda_init):
+        super().__init__()
+        self.heads, self.head_dim, self.lambda_init = heads, channels // heads // 2, lambda_init
+        self.qkv = conv(channels, 3 * channels, 1, bias=False)
+        self.out = conv(channels, channels, 1, bias=False)
+        for name in ("lambda_q1", "lambda_k1", "lambda_q2", "lambda_k2"):
+            self.register_parameter(name, torch.nn.Parameter(torch.randn(heads, self.head_dim) * 0.1))
+        self.head_norm = torch.nn.Parameter(torch.full((2 * self.head_dim,), 1.0 - lambda_init))
+        self.rotary = rotary
+
+    def lam(self):
+        """The weight of the second map, [heads]."""
+        return (self.lambda_q1 * self.lambda_k1).sum(1).exp() - (self.lambda_q2 * self.lambda_k2).sum(1).exp() + self.lambda_init
+
+    def _project(self, conv, x, dtype):
+        conv.out_dtype = dtype
+        return conv(x)
+
+    def forward(self, h, positions, dtype):
+        """h: [B, C, H, W] in channels-last memory; returns the same shape in `dtype`."""
+        B, C, H, W = h.shape
+        N, heads, d = H * W, self.heads, self.head_dim
+        qkv = self._project(self.qkv, h, torch.bfloat16).permute(0, 2, 3, 1).reshape(B, N, 3 * C)
+        q, k = (qkv[..., i * C:(i + 1) * C].unflatten(-1, (2 * heads, d)) for i in (0, 1))
+        if self.rotary is not None:
+            q, k = self.rotary(q, k, positions)
+        v = qkv[..., 2 * C:].unflatten(-1, (heads, 2 * d))
+        o = F.differential_attention(q.unflatten(2, (heads, 2)), k.unflatten(2, (heads, 2)), v, self.lam())
+        o = F.block_input_norm(o, self.head_norm)
+        return self._project(self.out, o.reshape(B, H, W, C).permute(0, 3, 1, 2), dtype)
+
+
+class DifferentialAttention2d(torch.nn.Module):
+    """EXTENSION (the reference's counterpart is the self-attention block, BigGAN/model.py:80-105): `depth` differential-attention
+    blocks over the positions of an image [B, C, H, W], each
+        x = x + gate * norm(out(head_norm(differential_attention(rotary(q), rotary(k), v))))      q, k, v = qkv(norm(x))
+    with 1x1 convolutions, rotary positions along height and width, and the norm behind a block, its gate, the residual sum and
+    the norm in front of the next block in one sweep.  heads: C / 64 by default; a head's values are C / heads wide (a multiple of
+    16 up to 256), each of its two maps half of that.  gate starts at zero: the module starts as the identity, like the reference's
+    gamma.  The attention runs in bf16 (precision "bf16" only); x and the result are fp32 or bf16.  First-order gradients."""
+
+    block_type = _DifferentialHeads
+
+    def __init__(self, channels, heads=None, depth=1, *, conv=Conv2d, base=10000.0, rotary=True, lambda_init=0.2, eps=1e-6):
+        super().__init__()
+        heads = max(1, channels // 64) if heads is None else heads
+        if channels % heads or channels // heads % 16 or channels // heads > 256:
+            raise ValueError(f"{channels} channels do not divide into {heads} heads of a multiple of 16 channels, at most 256")
+        d = channels // heads // 2
+        self.channels, self.eps = channels, eps
+        axial = AxialRotary((d // 4 * 2, d - d // 4 * 2), base) if rotary else None
+        self.blocks = torch.nn.ModuleList(self.block_type(channels, heads, conv, axial, lambda_init) for _ in range(depth))
+        self.in_norm = torch.nn.ParameterList(torch.nn.Parameter(torch.ones(channels)) for _ in range(depth))
+        self.out_norm = torch.nn.ParameterList(torch.nn.Parameter(torch.ones(channels)) for _ in range(depth))
+        self.gate = torch.nn.ParameterList(torch.nn.Parameter(torch.zeros(channels)) for _ in range(depth))
+        self._positions = {}
+
+    def positions(self, height, width, device):
+        """Row and column of every position, [H * W, 2] (made once per size and device)."""
+        key = (height, width, device)
+        if key not in self._positions:
+            n = torch.arange(height * width, device=device, dtype=torch.int32)
+            self._positions[key] = torch.stack((n // width, n % width), dim=1)
+        return self._positions[key]
+
+    def __deepcopy__(self, memo):
+        copy = self.__class__.__new__(self.__class__)
+        memo[id(self)] = copy
+        for name, value in self.__dict__.items():
+            copy.__dict__[name] = {} if name == "_positions" else _deepcopy(value, memo)
+        return copy
+
+    def forward(self, x):
+        if x.dim() != 4 or x.shape[1] != self.channels:
+            raise RuntimeError(f"expected [B, {self.channels}, H, W], got {tuple(x.shape)}")
+        if ops.get_precision() != ops._lib.GC_PREC_BF16:
+            raise RuntimeError("ganconv: DifferentialAttention2d computes in bf16; set_precision('bf16')")
+        ops._check_cuda(x)
+        pos = self.positions(x.shape[2], x.shape[3], x.device)
+        tokens = lambda t: t.permute(0, 2, 3, 1)            # noqa: E731  [B, H, W, C], without a copy in channels-last memory
+        image = lambda t: t.permute(0, 3, 1, 2)             # noqa: E731
+        y = tokens(x)
+        h = F.block_input_norm(y, self.in_norm[0], eps=self.eps)
+        for i, block in enumerate(self.blocks):
+            f = tokens(block(image(h), pos, x.dtype))
+            if i + 1 < len(self.blocks):
+                y, h = F.block_boundary_norm(y, f, self.out_norm[i], self.in_norm[i + 1], gate=self.gate[i], eps=self.eps)
+            else:
+                y = F.block_output_norm(y, f, self.out_norm[i], gate=self.gate[i], eps=self.eps)
+        return image(y)
 
 
 def convert_sync_batchnorm(module, process_group=None):

@@ -195,3 +195,38 @@ def test_packed_descriptors_match_the_structures():
         for (name, i), value in zip(flat, values):
             got = getattr(d, name) if i is None else getattr(d, name)[i]
             assert got == value, (cls.__name__, name, i)
+
+
+def test_modules_and_the_biggan_option():
+    import copy
+
+    from gan_amd.harness import biggan as H
+    m = gan_amd.nn.DifferentialAttention2d(128, depth=2)
+    assert m.blocks[0].heads == 2 and m.blocks[0].head_dim == 32 and m.blocks[0].rotary.dims == (16, 16)
+    names = set(dict(m.named_parameters()))
+    assert {"blocks.0.qkv.weight", "blocks.1.out.weight", "blocks.0.lambda_q1", "blocks.0.head_norm", "in_norm.1", "out_norm.0", "gate.1"} <= names
+    assert not list(m.buffers()) and torch.equal(m.blocks[0].lam().detach().shape and m.blocks[0].lam() * 0, torch.zeros(2))
+    c = copy.deepcopy(m)
+    c.load_state_dict(m.state_dict())
+    with pytest.raises(RuntimeError, match="GPU"):
+        m(torch.zeros(1, 128, 4, 4))
+    with pytest.raises(RuntimeError, match="expected"):
+        m(torch.zeros(1, 64, 4, 4))
+    with pytest.raises(ValueError, match="heads"):
+        gan_amd.nn.DifferentialAttention2d(40)
+    gan_amd.set_precision("fp32x3")
+    try:
+        with pytest.raises(RuntimeError, match="bf16"):
+            m(torch.zeros(1, 128, 4, 4))
+    finally:
+        gan_amd.set_precision("bf16")
+    torch.manual_seed(0)
+    plain = H.Generator(10, 16).state_dict()
+    torch.manual_seed(0)
+    again = H.Generator(10, 16, attention="self").state_dict()
+    assert list(plain) == list(again) and all(torch.equal(plain[n], again[n]) for n in plain)
+    g, d = H.Generator(10, 16, attention="differential"), H.Discriminator(10, 16, attention="differential")
+    assert isinstance(g.main_sequence[4], H.DifferentialAttentionBlock) and isinstance(d.main_sequence[1], H.DifferentialAttentionBlock)
+    assert "main_sequence.4.blocks.0.qkv.U_vector" in g.state_dict()
+    with pytest.raises(KeyError):
+        H.Generator(10, 16, attention="none")
