@@ -36,6 +36,7 @@ constexpr int kRows = 128;                       // rows of a workgroup: 32 per 
 constexpr int kBlk = 64;                         // rows staged per step
 constexpr uint32_t kOutOfRange = 0x80000000u;
 constexpr float kLazy = 8.f;                     // log2 units by which a score may exceed the running maximum
+constexpr float kLazyExp = 256.f;                // 2^kLazy
 constexpr float kLargeScore = 1048576.f;         // log2 units
 
 struct DiffParams {
@@ -231,18 +232,19 @@ struct Cfg {
   static constexpr int WAVES = DV > 128 ? 1 : 2;      // per SIMD: the accumulators of the widest form take the registers of two
 };
 
-// One step of the running softmax of both maps over 32 keys: masks (room: this lane's first hidden key, relative to its first), moves
-// the running maxima, and leaves s[m] and base[m] so that the exponential of a score is exp2(s c2 - base).
-template <int VC>
-__device__ __forceinline__ void softmax_step(f32x16 (&s)[2], f32x16 (&acc)[2][VC], float (&mrun)[2], float (&lsum)[2], float (&base)[2], bool masked,
-                                             int room, float c2, float lazy) {
-  if (masked) {
+// Scores of hidden keys (from `room` on, counted from this lane's first) of both maps
+__device__ __forceinline__ void hide(f32x16 (&s)[2], int room) {
 #pragma unroll
-    for (int e = 0; e < 16; e++) {
-      s[0][e] = 8 * (e >> 2) + (e & 3) >= room ? -INFINITY : s[0][e];
-      s[1][e] = 8 * (e >> 2) + (e & 3) >= room ? -INFINITY : s[1][e];
-    }
+  for (int e = 0; e < 16; e++) {
+    s[0][e] = 8 * (e >> 2) + (e & 3) >= room ? -INFINITY : s[0][e];
+    s[1][e] = 8 * (e >> 2) + (e & 3) >= room ? -INFINITY : s[1][e];
   }
+}
+// The careful way of the running softmax of both maps over 32 keys: moves the running maxima where a score exceeds them by kLazy, and
+// leaves s[m] and base[m] so that the exponential of a score is exp2(s c2 - base).
+template <int VC>
+__device__ __forceinline__ void softmax_step(f32x16 (&s)[2], f32x16 (&acc)[2][VC], float (&mrun)[2], float (&lsum)[2], float (&base)[2], float c2,
+                                             float lazy) {
   float mx[2], top[2];
 #pragma unroll
   for (int m = 0; m < 2; m++) {
@@ -330,7 +332,8 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_fwd_kerne
     for (int ks = 0; ks < F::KS; ks++) qf[m][ks] = global_frag(qrow + m * a.q_stride[3], valid, ks * 16 + 8 * h, a.d);
 
   f32x16 acc[2][F::VC];
-  float mrun[2] = {-INFINITY, -INFINITY}, lsum[2] = {0.f, 0.f};
+  float mrun[2] = {-INFINITY, -INFINITY}, lsum[2] = {0.f, 0.f}, base[2] = {0.f, 0.f};
+  bool careful = true;                                     // (of the whole wave) no maximum yet, or scores too large for the short way
 #pragma unroll
   for (int m = 0; m < 2; m++)
 #pragma unroll
@@ -364,33 +367,65 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_fwd_kerne
     for (int jb = 0; jb < 2; jb++) {
       const int j0 = blk * kBlk + jb * 32;
       const uint32_t ka = kaddr + stage + jb * 32 * F::KROW, va = vaddr + stage + jb * 32 * F::VROW;
-      // LDS reads are issued well in front of the matrix instructions that use them, all K fragments first, the first half of the V
-      // fragments in front of the exponentials; the fences keep the compiler from moving them back down
-      bf16x8 kf[2][F::KS], vf[F::VC];
+      // LDS reads are issued well in front of the matrix instructions that use them, all K fragments first, the V fragments in two
+      // halves; the fences keep the compiler from moving them back down
       f32x16 s[2];
+      {
+        bf16x8 kf[2][F::KS];
 #pragma unroll
-      for (int ks = 0; ks < F::KS; ks++)
+        for (int ks = 0; ks < F::KS; ks++)
 #pragma unroll
-        for (int m = 0; m < 2; m++) kf[m][ks] = read_row((ka ^ (ks << 5)) + m * F::KB);
-      __builtin_amdgcn_sched_barrier(0);
+          for (int m = 0; m < 2; m++) kf[m][ks] = read_row((ka ^ (ks << 5)) + m * F::KB);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int ks = 0; ks < F::KS; ks++)
+        for (int ks = 0; ks < F::KS; ks++)
 #pragma unroll
-        for (int m = 0; m < 2; m++) s[m] = mfma(kf[m][ks], qf[m][ks], ks == 0 ? zero16() : s[m]);
-      float base[2];
-      softmax_step<F::VC>(s, acc, mrun, lsum, base, j0 + 32 > wmin, lim - j0 - 4 * h, P.c2, P.lazy);
-      __builtin_amdgcn_sched_barrier(0);
+          for (int m = 0; m < 2; m++) s[m] = mfma(kf[m][ks], qf[m][ks], ks == 0 ? zero16() : s[m]);
+      }
+      if (j0 + 32 > wmin) hide(s, lim - j0 - 4 * h);
+      // Exponentials against the maxima so far, without looking for new ones: the sum of a lane's 16 exponentials, wanted anyway,
+      // tells whether one of them passed 2^8 (it is then above 2^8 ... 2^12, or infinite).  Then, and while a row has no maximum
+      // yet, the scores are formed again and take the careful way.
+      float sum[2];
+      auto exponentials = [&]() {
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+          sum[m] = 0.f;
+#pragma unroll
+          for (int e = 0; e < 16; e++) {
+            s[m][e] = __builtin_amdgcn_exp2f(s[m][e] * P.c2 - base[m]);
+            sum[m] += s[m][e];
+          }
+        }
+      };
+      bool again = careful;
+      if (!again) {
+        exponentials();
+        again = __builtin_amdgcn_ballot_w64(fmaxf(sum[0], sum[1]) > 16.f * kLazyExp) != 0;
+      }
+      if (again) {
+        if (!careful) {
+#pragma unroll
+          for (int m = 0; m < 2; m++)
+#pragma unroll
+            for (int ks = 0; ks < F::KS; ks++) {
+              s[m] = mfma(read_row((ka ^ (ks << 5)) + m * F::KB), qf[m][ks], ks == 0 ? zero16() : s[m]);
+              __builtin_amdgcn_sched_barrier(0);           // (one operand at a time: rare, and the registers are taken)
+            }
+          if (j0 + 32 > wmin) hide(s, lim - j0 - 4 * h);
+        }
+        softmax_step<F::VC>(s, acc, mrun, lsum, base, P.c2, P.lazy);
+        exponentials();
+        careful = __builtin_amdgcn_ballot_w64(mrun[0] == -INFINITY || mrun[1] == -INFINITY ||
+                                              fmaxf(fabsf(mrun[0]), fabsf(mrun[1])) * P.c2 > kLargeScore) != 0;
+      }
+      bf16x8 vf[F::VC], pb[2][2];
 #pragma unroll
       for (int cb = 0; cb < F::VC; cb++) vf[cb] = read_col(va ^ (cb << 6), (va ^ (cb << 6)) + 8 * F::VROW);
       __builtin_amdgcn_sched_barrier(0);
-      bf16x8 pb[2][2];
 #pragma unroll
       for (int m = 0; m < 2; m++) {
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-          s[m][e] = __builtin_amdgcn_exp2f(s[m][e] * P.c2 - base[m]);
-          lsum[m] += s[m][e];
-        }
+        lsum[m] += sum[m];
         pb[m][0] = pack8(s[m], 0);
         pb[m][1] = pack8(s[m], 8);
       }
@@ -521,7 +556,8 @@ __global__ __launch_bounds__((FewCfg<DK, DV>::NW * 64), 1) void diff_few_rows_ke
 #pragma unroll
       for (int m = 0; m < 2; m++) s[m] = mfma(read_row((ka ^ (ks << 5)) + m * X::KB), qf[m][ks], ks == 0 ? zero16() : s[m]);
     float base[2];
-    softmax_step<F::VC>(s, acc, mrun, lsum, base, j0 + 32 > wmin, lim - j0 - 4 * h, P.c2, P.lazy);
+    if (j0 + 32 > wmin) hide(s, lim - j0 - 4 * h);
+    softmax_step<F::VC>(s, acc, mrun, lsum, base, P.c2, P.lazy);
     bf16x8 hi[2][2], lo[2][2];
 #pragma unroll
     for (int m = 0; m < 2; m++) {
