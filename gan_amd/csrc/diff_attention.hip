@@ -44,7 +44,7 @@ struct DiffParams {
   int G, tiles, nsplit, blocks_per_split, few;     // few: at most 32 rows per key head (diff_few_rows_kernel; shares in tiles of 32 keys)
   FastDiv div_nq;
   float c2, lazy;                                // scale * log2(e); kLazy in units of a score
-  float *part, *ml, *delta, *lampart;
+  float *part, *ml, *delta, *rows4, *lampart;
 };
 
 __device__ __forceinline__ bf16x8 zero8() { return __builtin_bit_cast(bf16x8, u32x4{0u, 0u, 0u, 0u}); }
@@ -59,12 +59,12 @@ __device__ __forceinline__ bf16x8 pack8(const f32x16& v, int r0) {
   const u32x2 lo = cvt_bf16x4(f32x4{v[r0], v[r0 + 1], v[r0 + 2], v[r0 + 3]}), hi = cvt_bf16x4(f32x4{v[r0 + 4], v[r0 + 5], v[r0 + 6], v[r0 + 7]});
   return __builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], hi[0], hi[1]});
 }
-__device__ __forceinline__ bf16x8 pack8_sum(const f32x16& u, const f32x16& v, int r0) {
+__device__ __forceinline__ bf16x8 pack8_sum(const f32x16& u, const f32x16& v, float f, int r0) {
   f32x4 a, b;
 #pragma unroll
   for (int x = 0; x < 4; x++) {
-    a[x] = u[r0 + x] + v[r0 + x];
-    b[x] = u[r0 + 4 + x] + v[r0 + 4 + x];
+    a[x] = u[r0 + x] + f * v[r0 + x];
+    b[x] = u[r0 + 4 + x] + f * v[r0 + 4 + x];
   }
   const u32x2 lo = cvt_bf16x4(a), hi = cvt_bf16x4(b);
   return __builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], hi[0], hi[1]});
@@ -664,7 +664,9 @@ __global__ __launch_bounds__(kJoinThreads) void diff_join_kernel(const DiffParam
     a.lse[((size_t)b * a.H + head) * 2 * a.NQ + (size_t)tid * a.NQ + i] = (tid == 0 ? L[0] : L[1]) != 0.f ? (tid == 0 ? top[0] : top[1]) * P.c2 + __log2f(tid == 0 ? L[0] : L[1]) : INFINITY;
 }
 
-// delta [B][H][2][NQ]: dO . O1 = dO . out + lam dO . O2, and dO . O2; 16 lanes per row
+// delta [B][H][2][NQ]: dO . O1 = dO . out + lam dO . O2, and dO . O2; 16 lanes per row.  rows4 [B][H][4][NQ]: what the key gradients' kernel
+// stages of a query: L1, L2 - log2|lam|, -delta1, sgn (delta1 - delta2) with sgn = -sign(lam): with p2' = |lam| p2 the mixed
+// probability is p1 + sgn p2', dP - delta1 comes out of the matrix instructions, and dS2 = p2' (sgn (dP - delta1) + sgn (delta1 - delta2))
 __global__ __launch_bounds__(kThreads) void diff_delta_kernel(const DiffParams P) {
   const gc_diff_attention& a = P.a;
   const size_t rows = (size_t)a.B * a.NQ * a.H, row = ((size_t)blockIdx.x * kThreads + threadIdx.x) >> 4;
@@ -691,8 +693,15 @@ __global__ __launch_bounds__(kThreads) void diff_delta_kernel(const DiffParams P
     const int head = (int)(row % a.H);
     const size_t bi = row / a.H, b = bi / a.NQ, i = bi - b * a.NQ;
     float* d = P.delta + (b * a.H + head) * 2 * a.NQ + i;
-    d[0] = s[0] + a.lam[head] * s[1];
-    d[a.NQ] = s[1];
+    const float lam = a.lam[head], d0 = s[0] + lam * s[1], d1 = s[1];
+    d[0] = d0;
+    d[a.NQ] = d1;
+    const float* l = a.lse + (b * a.H + head) * 2 * a.NQ + i;
+    float* q = P.rows4 + (b * a.H + head) * 4 * a.NQ + i;
+    q[0] = l[0];
+    q[a.NQ] = l[a.NQ] - __log2f(fabsf(lam));
+    q[2 * a.NQ] = -d0;
+    q[3 * a.NQ] = lam > 0.f ? d1 - d0 : d0 - d1;
   }
 }
 
@@ -738,6 +747,10 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dq_ke
 #pragma unroll
     for (int cb = 0; cb < F::KC; cb++) acc[m][cb] = zero16();
   float left = 0.f;                                        // sum_j p2 (dP - delta2)
+  const float gap = D[0] - D[1];
+  f32x16 start;
+#pragma unroll
+  for (int e = 0; e < 16; e++) start[e] = -D[0];
 
   const uint16_t* kbase = static_cast<const uint16_t*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[2];
   const uint16_t* vbase = static_cast<const uint16_t*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[2];
@@ -765,38 +778,54 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dq_ke
     for (int jb = 0; jb < 2; jb++) {
       const int j0 = blk * kBlk + jb * 32;
       const uint32_t ka = kra + stage + jb * 32 * F::KROW, va = vra + stage + jb * 32 * F::VROW, kc = kca + stage + jb * 32 * F::KROW;
-      f32x16 s[2], dp = zero16();
+      // (LDS reads ahead of their matrix instructions, as in the forward kernel)
+      f32x16 s[2], dp;
+      {
+        bf16x8 kf[2][F::KS];
 #pragma unroll
-      for (int m = 0; m < 2; m++) {
-        s[m] = zero16();
+        for (int ks = 0; ks < F::KS; ks++)
 #pragma unroll
-        for (int ks = 0; ks < F::KS; ks++) s[m] = mfma(read_row((ka ^ (ks << 5)) + m * F::KB), qf[m][ks], s[m]);
+          for (int m = 0; m < 2; m++) kf[m][ks] = read_row((ka ^ (ks << 5)) + m * F::KB);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int ks = 0; ks < F::KS; ks++)
+#pragma unroll
+          for (int m = 0; m < 2; m++) s[m] = mfma(kf[m][ks], qf[m][ks], ks == 0 ? zero16() : s[m]);
       }
+      {
+        constexpr int HALF = F::VS / 2;
+        bf16x8 vf[HALF];
 #pragma unroll
-      for (int ks = 0; ks < F::VS; ks++) dp = mfma(read_row(va ^ (ks << 5)), gf[ks], dp);
-      if (j0 + 32 > wmin) {
+        for (int x = 0; x < 2; x++) {
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-          const bool hidden = 8 * (e >> 2) + (e & 3) >= lim - j0 - 4 * h;
-          s[0][e] = hidden ? -INFINITY : s[0][e];
-          s[1][e] = hidden ? -INFINITY : s[1][e];
+          for (int ks = 0; ks < HALF; ks++) vf[ks] = read_row(va ^ ((x * HALF + ks) << 5));
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int ks = 0; ks < HALF; ks++) dp = mfma(vf[ks], gf[x * HALF + ks], x + ks == 0 ? start : dp);      // dP - delta1
         }
       }
+      if (j0 + 32 > wmin) hide(s, lim - j0 - 4 * h);
 #pragma unroll
       for (int e = 0; e < 16; e++) {
-        const float p0 = __builtin_amdgcn_exp2f(s[0][e] * P.c2 - L[0]), p1 = __builtin_amdgcn_exp2f(s[1][e] * P.c2 - L[1]);
-        s[0][e] = p0 * (dp[e] - D[0]);
-        s[1][e] = p1 * (dp[e] - D[1]);
+        s[0][e] = __builtin_amdgcn_exp2f(s[0][e] * P.c2 - L[0]) * dp[e];
+        s[1][e] = __builtin_amdgcn_exp2f(s[1][e] * P.c2 - L[1]) * (dp[e] + gap);
         left += s[1][e];
       }
 #pragma unroll
-      for (int m = 0; m < 2; m++)
+      for (int t = 0; t < 2; t++) {
+        bf16x8 kt[2][F::KC], d[2];
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-          const bf16x8 d = pack8(s[m], 8 * t);
+        for (int m = 0; m < 2; m++)
 #pragma unroll
-          for (int cb = 0; cb < F::KC; cb++) acc[m][cb] = mfma(read_col_both<F::KROW>((kc ^ (cb << 6)) + m * F::KB + t * 16 * F::KROW), d, acc[m][cb]);
-        }
+          for (int cb = 0; cb < F::KC; cb++) kt[m][cb] = read_col_both<F::KROW>((kc ^ (cb << 6)) + m * F::KB + t * 16 * F::KROW);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int m = 0; m < 2; m++) d[m] = pack8(s[m], 8 * t);
+#pragma unroll
+        for (int cb = 0; cb < F::KC; cb++)
+#pragma unroll
+          for (int m = 0; m < 2; m++) acc[m][cb] = mfma(kt[m][cb], d[m], acc[m][cb]);
+      }
     }
   }
   const float lam = a.lam[head];
@@ -929,8 +958,8 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dkv_k
     lq.load(q, (int64_t)blk * ROWS, a.NQ, qst, a.d, st);
     lq.load(q + a.q_stride[3], (int64_t)blk * ROWS, a.NQ, qst, a.d, st + X::KB);
     lg.load(go, (int64_t)blk * ROWS, a.NQ, gst, a.dv, st + 2 * X::KB);
-    // wave 0, 1: L of the two maps; 2, 3: delta.  ROWS floats, then zeros (also past the last query), 64 in all
-    const float* v = (wave < 2 ? a.lse : P.delta) + ((size_t)(b * a.H + head) * 2 + (wave & 1)) * a.NQ + (int64_t)blk * ROWS;
+    // a wave each: the four floats of a query.  ROWS floats, then zeros (also past the last query), 64 in all
+    const float* v = P.rows4 + ((size_t)(b * a.H + head) * 4 + wave) * a.NQ + (int64_t)blk * ROWS;
     load_to_lds4(buffer_at(v, min(ROWS, a.NQ - blk * ROWS) * 4), lane * 4, st + 2 * X::KB + X::VB + wave * kBlk * 4);
   };
   const uint32_t qra = base0 + row_addr<F::KROW, kBothWays>(lane), qca = base0 + col_addr<F::KROW, kBothWays>(lane, 0);
@@ -942,7 +971,7 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dkv_k
   int g = per_head > 0 ? step0 / per_head : 0, blk = first + step0 - g * per_head, odd = 0;
   if (step0 < step1) fetch(g, blk, base0);
   for (int step = step0; step < step1; step++) {
-    const float nlam = -a.lam[hk * P.G + g];               // (asked for in front of the next step's loads, which it would wait for)
+    const float sgn = a.lam[hk * P.G + g] > 0.f ? -1.f : 1.f;      // (asked for in front of the next step's loads, which it would wait for)
     tile_ready();
     const int i_blk = blk * ROWS;
     if (++blk == nblk) { blk = first; g++; }
@@ -959,10 +988,17 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dkv_k
       // the order keeps few values alive at once: scores and probabilities, their mix and dV, then dP, the score gradients and dK
       f32x16 s[2];
 #pragma unroll
-      for (int m = 0; m < 2; m++) {
-        s[m] = zero16();
+      for (int x = 0; x < F::KS; x += 2) {                 // (four LDS reads ahead of the matrix instructions: what the registers hold)
+        bf16x8 q[2][2];
 #pragma unroll
-        for (int ks = 0; ks < F::KS; ks++) s[m] = mfma(read_row((qr ^ (ks << 5)) + m * X::KB), kf[m][ks], s[m]);
+        for (int y = 0; y < 2; y++)
+#pragma unroll
+          for (int m = 0; m < 2; m++) q[m][y] = read_row((qr ^ ((x + y) << 5)) + m * X::KB);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int y = 0; y < 2; y++)
+#pragma unroll
+          for (int m = 0; m < 2; m++) s[m] = mfma(q[m][y], kf[m][x + y], x + y == 0 ? zero16() : s[m]);
       }
       if (i0 < w0 + 31 + shift) {
         const int hidden = w0 + (lane & 31) + shift - i0 - 4 * h;      // this lane's key is seen from there on
@@ -978,38 +1014,65 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dkv_k
 #pragma unroll
         for (int x = 0; x < 4; x++) {
           s[0][4 * e4 + x] = __builtin_amdgcn_exp2f(s[0][4 * e4 + x] * P.c2 - L0[x]);
-          s[1][4 * e4 + x] = __builtin_amdgcn_exp2f(s[1][4 * e4 + x] * P.c2 - L1[x]) * nlam;
+          s[1][4 * e4 + x] = __builtin_amdgcn_exp2f(s[1][4 * e4 + x] * P.c2 - L1[x]);
         }
       }
       if (OUT & 2) {
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-          const bf16x8 d = pack8_sum(s[0], s[1], 8 * t);
+          bf16x8 gt[F::VC];
 #pragma unroll
-          for (int cb = 0; cb < F::VC; cb++) adv[cb] = mfma(read_col_both<F::VROW>((gc ^ (cb << 6)) + t * 16 * F::VROW), d, adv[cb]);
+          for (int cb = 0; cb < F::VC; cb++) gt[cb] = read_col_both<F::VROW>((gc ^ (cb << 6)) + t * 16 * F::VROW);
+          __builtin_amdgcn_sched_barrier(0);
+          const bf16x8 d = pack8_sum(s[0], s[1], sgn, 8 * t);
+#pragma unroll
+          for (int cb = 0; cb < F::VC; cb++) adv[cb] = mfma(gt[cb], d, adv[cb]);
         }
       }
       if (OUT & 1) {
-        f32x16 dp = zero16();
-#pragma unroll
-        for (int ks = 0; ks < F::VS; ks++) dp = mfma(read_row(gr ^ (ks << 5)), X::VLDS ? read_row(vra ^ (ks << 5)) : vf[X::VLDS ? 0 : ks], dp);
+        f32x16 dp;                                         // dP - delta1
 #pragma unroll
         for (int e4 = 0; e4 < 4; e4++) {
-          const f32x4 D0 = *reinterpret_cast<const f32x4*>(vec + 2 * kBlk + 8 * e4), D1 = *reinterpret_cast<const f32x4*>(vec + 3 * kBlk + 8 * e4);
+          const f32x4 D = *reinterpret_cast<const f32x4*>(vec + 2 * kBlk + 8 * e4);
+#pragma unroll
+          for (int x = 0; x < 4; x++) dp[4 * e4 + x] = D[x];
+        }
+#pragma unroll
+        for (int x = 0; x < F::VS; x += 2) {
+          bf16x8 gg[2], vv[2];
+#pragma unroll
+          for (int y = 0; y < 2; y++) {
+            gg[y] = read_row(gr ^ ((x + y) << 5));
+            vv[y] = X::VLDS ? read_row(vra ^ ((x + y) << 5)) : vf[X::VLDS ? 0 : x + y];
+          }
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int y = 0; y < 2; y++) dp = mfma(gg[y], vv[y], dp);
+        }
+#pragma unroll
+        for (int e4 = 0; e4 < 4; e4++) {
+          const f32x4 E = *reinterpret_cast<const f32x4*>(vec + 3 * kBlk + 8 * e4);
 #pragma unroll
           for (int x = 0; x < 4; x++) {
-            s[0][4 * e4 + x] *= dp[4 * e4 + x] - D0[x];
-            s[1][4 * e4 + x] *= dp[4 * e4 + x] - D1[x];
+            s[0][4 * e4 + x] *= dp[4 * e4 + x];
+            s[1][4 * e4 + x] *= dp[4 * e4 + x] * sgn + E[x];
           }
         }
 #pragma unroll
-        for (int m = 0; m < 2; m++)
+        for (int t = 0; t < 2; t++) {
+          bf16x8 qt[2][F::KC];
 #pragma unroll
-          for (int t = 0; t < 2; t++) {
+          for (int m = 0; m < 2; m++)
+#pragma unroll
+            for (int cb = 0; cb < F::KC; cb++) qt[m][cb] = read_col_both<F::KROW>((qc ^ (cb << 6)) + m * X::KB + t * 16 * F::KROW);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int m = 0; m < 2; m++) {
             const bf16x8 d = pack8(s[m], 8 * t);
 #pragma unroll
-            for (int cb = 0; cb < F::KC; cb++) adk[m][cb] = mfma(read_col_both<F::KROW>((qc ^ (cb << 6)) + m * X::KB + t * 16 * F::KROW), d, adk[m][cb]);
+            for (int cb = 0; cb < F::KC; cb++) adk[m][cb] = mfma(qt[m][cb], d, adk[m][cb]);
           }
+        }
       }
     }
   }
@@ -1129,7 +1192,7 @@ size_t forward_bytes(const DiffParams& P, int DV) {
 // length, so dkv wants twice as many workgroups as run at a time.
 struct BackwardPlan {
   int dq_tiles, dq_shares, dq_blocks, dkv_tiles, dkv_shares;
-  size_t delta, lampart, part;                             // floats
+  size_t delta, rows4, lampart, part;                      // floats
 };
 BackwardPlan plan_backward(const gc_diff_attention* a) {
   BackwardPlan p{};
@@ -1147,12 +1210,13 @@ BackwardPlan plan_backward(const gc_diff_attention* a) {
   p.dkv_shares = n < 2 ? 1 : (int)n;
   const size_t rows = (size_t)a->B * a->H * a->NQ, keys = (size_t)a->B * a->HK * a->NK;
   p.delta = (rows * 2 + 3) / 4 * 4;
+  p.rows4 = rows * 4;
   p.lampart = ((size_t)a->B * a->H * p.dq_tiles * p.dq_shares + 3) / 4 * 4;
   const size_t dq = p.dq_shares > 1 ? (size_t)p.dq_shares * rows * 2 * a->d : 0, dkv = p.dkv_shares > 1 ? (size_t)p.dkv_shares * keys * (2 * a->d + a->dv) : 0;
   p.part = dq > dkv ? dq : dkv;                            // (used one after the other)
   return p;
 }
-size_t backward_bytes(const BackwardPlan& p) { return (p.delta + p.lampart + p.part) * sizeof(float); }
+size_t backward_bytes(const BackwardPlan& p) { return (p.delta + p.rows4 + p.lampart + p.part) * sizeof(float); }
 
 template <int DK, int DV>
 int launch_fwd(const DiffParams& P, hipStream_t s) {
@@ -1251,7 +1315,8 @@ extern "C" int gc_diff_attention_bwd(const gc_diff_attention* desc, void* worksp
   plan_forward(desc, P);
   const size_t rows = (size_t)desc->B * desc->H * desc->NQ, keys = (size_t)desc->B * desc->HK * desc->NK;
   P.delta = static_cast<float*>(workspace);
-  P.lampart = P.delta + plan.delta;
+  P.rows4 = P.delta + plan.delta;
+  P.lampart = P.rows4 + plan.rows4;
   P.part = P.lampart + plan.lampart;
   hipStream_t s = (hipStream_t)stream;
   const int form = form_of(desc);

@@ -414,7 +414,9 @@ def _attention_inputs(case, seed=11):
     g = torch.Generator().manual_seed(seed)
     r = lambda *s, k=1.0: (torch.randn(*s, generator=g) * k).to(torch.bfloat16)
     a = math.sqrt(spread)
-    return r(B, NQ, H, 2, d, k=a), r(B, NK, HK, 2, d, k=a), r(B, NK, HK, dv), torch.rand(H, generator=g) * 1.2 - 0.2, r(B, NQ, H, dv)
+    q, k, v, lam, dout = r(B, NQ, H, 2, d, k=a), r(B, NK, HK, 2, d, k=a), r(B, NK, HK, dv), torch.rand(H, generator=g) * 1.2 - 0.2, r(B, NQ, H, dv)
+    lam[1:2], lam[2:3] = -0.7, 0.0                       # a negative weight, none at all
+    return q, k, v, lam, dout
 
 
 @pytest.mark.parametrize("case", ATTENTION_CASES, ids=lambda c: "x".join(map(str, c[:7])) + ("-causal" if c[7] else "") + ("-lengths" if c[8] else ""))
