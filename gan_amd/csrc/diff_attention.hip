@@ -143,12 +143,10 @@ struct Loader {
     }
     step = NW * RPI * stride;                              // bytes between a wave's consecutive instructions
   }
-  // rows [row0, row0 + ROWS) of the tensor at `base`, of which those below `rows` exist, to LDS at `lds`.  The instructions' row offsets
-  // go into the (scalar) buffer base, so that one offset register serves all of them.
-  __device__ __forceinline__ void load(const uint16_t* base, int64_t row0, int64_t rows, uint32_t stride, int width, uint32_t lds) const {
-    const int64_t left = rows - row0;
-    const int n_rows = left < 0 ? 0 : (left > ROWS ? ROWS : (int)left);
-    const char* p = reinterpret_cast<const char*>(base) + row0 * (int64_t)stride;
+  // ROWS rows at p, of which the first `left` (possibly none or fewer) exist, to LDS at `lds`.  The instructions' row offsets go into the
+  // (scalar) buffer base, so that one offset register serves all of them.
+  __device__ __forceinline__ void load(const char* p, int left, uint32_t stride, int width, uint32_t lds) const {
+    const int n_rows = left < ROWS ? left : ROWS;
     const uint32_t bytes = n_rows > 0 ? (uint32_t)(n_rows - 1) * stride + width * 2 : 0u;
 #pragma unroll
     for (int n = 0; n < NI; n += BASES) {
@@ -157,6 +155,37 @@ struct Loader {
 #pragma unroll
       for (int b = 0; b < BASES; b++) load_to_lds16(rs, voff[b], lds + (wave + NW * (n + b)) * 1024);
     }
+  }
+};
+// Keys and values of one key head, staged tile after tile: running (scalar) addresses instead of products per tile.
+template <int KROW, int VROW, Use KU, Use VU, int ROWS, int NW>
+struct KeyTiles {
+  Loader<KROW, KU, ROWS, NW> lk;
+  Loader<VROW, VU, ROWS, NW> lv;
+  const char *k0, *k1, *v;
+  uint32_t kst, vst;
+  int left, d, dv;
+  __device__ __forceinline__ void init(const gc_diff_attention& a, int b, int hk, int row, int len, int wave, int lane) {
+    kst = (uint32_t)(a.k_stride[1] * 2);
+    vst = (uint32_t)(a.v_stride[1] * 2);
+    d = a.d;
+    dv = a.dv;
+    lk.init(wave, lane, kst, d);
+    lv.init(wave, lane, vst, dv);
+    k0 = reinterpret_cast<const char*>(static_cast<const uint16_t*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[2]) + row * (int64_t)kst;
+    k1 = k0 + a.k_stride[3] * 2;
+    v = reinterpret_cast<const char*>(static_cast<const uint16_t*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[2]) + row * (int64_t)vst;
+    left = len - row;
+  }
+  // the next tile's two maps of keys and its values, one behind the other
+  __device__ __forceinline__ void next(uint32_t lds) {
+    lk.load(k0, left, kst, d, lds);
+    lk.load(k1, left, kst, d, lds + ROWS * KROW);
+    lv.load(v, left, vst, dv, lds + 2 * ROWS * KROW);
+    k0 += ROWS * kst;
+    k1 += ROWS * kst;
+    v += ROWS * vst;
+    left -= ROWS;
   }
 };
 
@@ -339,27 +368,16 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_fwd_kerne
 #pragma unroll
     for (int cb = 0; cb < F::VC; cb++) acc[m][cb] = zero16();
 
-  const uint16_t* kbase = static_cast<const uint16_t*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[2];
-  const uint16_t* vbase = static_cast<const uint16_t*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[2];
-  const uint32_t kst = (uint32_t)(a.k_stride[1] * 2), vst = (uint32_t)(a.v_stride[1] * 2);
-  Loader<F::KROW, kRowWise> lk;
-  Loader<F::VROW, kTransposed> lv;
-  lk.init(wave, lane, kst, a.d);
-  lv.init(wave, lane, vst, a.dv);
-  auto fetch = [&](int blk, uint32_t st) {
-    lk.load(kbase, (int64_t)blk * kBlk, len, kst, a.d, st);
-    lk.load(kbase + a.k_stride[3], (int64_t)blk * kBlk, len, kst, a.d, st + F::KB);
-    lv.load(vbase, (int64_t)blk * kBlk, len, vst, a.dv, st + 2 * F::KB);
-  };
-
   const uint32_t base0 = lds_offset(smem);
   const uint32_t kaddr = base0 + row_addr<F::KROW, kRowWise>(lane), vaddr = base0 + 2 * F::KB + col_addr<F::VROW, kTransposed>(lane, 0);
   const int nblk = (kend + kBlk - 1) / kBlk;
   const int blk0 = split * P.blocks_per_split, blk1 = min(nblk, blk0 + P.blocks_per_split);
-  if (blk0 < blk1) fetch(blk0, base0);
+  KeyTiles<F::KROW, F::VROW, kRowWise, kTransposed, kBlk, kThreads / 64> tiles;
+  tiles.init(a, b, hk, blk0 * kBlk, len, wave, lane);
+  if (blk0 < blk1) tiles.next(base0);
   for (int blk = blk0; blk < blk1; blk++) {
     tile_ready();
-    if (blk + 1 < blk1) fetch(blk + 1, base0 + ((blk + 1 - blk0) & 1) * STAGE);
+    if (blk + 1 < blk1) tiles.next(base0 + ((blk + 1 - blk0) & 1) * STAGE);
     const uint32_t stage = ((blk - blk0) & 1) * STAGE;
     // (the whole wave; the barrier above is met by every wave in every step)
     if (blk * kBlk >= wmax) continue;
@@ -528,25 +546,16 @@ __global__ __launch_bounds__((FewCfg<DK, DV>::NW * 64), 1) void diff_few_rows_ke
 #pragma unroll
     for (int cb = 0; cb < F::VC; cb++) acc[m][cb] = zero16();
 
-  const uint16_t* kbase = static_cast<const uint16_t*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[2];
-  const uint16_t* vbase = static_cast<const uint16_t*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[2];
-  const uint32_t kst = (uint32_t)(a.k_stride[1] * 2), vst = (uint32_t)(a.v_stride[1] * 2);
-  Loader<F::KROW, kRowWise, 32, 1> lk;
-  Loader<F::VROW, kTransposed, 32, 1> lv;
-  lk.init(0, lane, kst, a.d);
-  lv.init(0, lane, vst, a.dv);
-  auto fetch = [&](int t, int rows, uint32_t st) {
-    lk.load(kbase, (int64_t)t * 32, rows, kst, a.d, st);
-    lk.load(kbase + a.k_stride[3], (int64_t)t * 32, rows, kst, a.d, st + X::KB);
-    lv.load(vbase, (int64_t)t * 32, rows, vst, a.dv, st + 2 * X::KB);
-  };
   const uint32_t base0 = lds_offset(smem) + wave * 2 * X::STAGE;
   const uint32_t kaddr = base0 + row_addr<F::KROW, kRowWise>(lane), vaddr = base0 + 2 * X::KB + col_addr<F::VROW, kTransposed>(lane, 0);
   const int t0 = share * P.blocks_per_split, t1 = min((wmax + 31) / 32, t0 + P.blocks_per_split);
-  if (t0 < t1) fetch(t0, len, base0);
+  KeyTiles<F::KROW, F::VROW, kRowWise, kTransposed, 32, 1> tiles;
+  tiles.init(a, b, hk, t0 * 32, len, 0, lane);
+  if (t0 < t1) tiles.next(base0);
   for (int t = t0; t < t1; t++) {
     // (behind the last tile: loads of no rows, which read nothing; the count of loads in flight stays the same)
-    fetch(t + 1, t + 1 < t1 ? len : 0, base0 + ((t + 1 - t0) & 1) * X::STAGE);
+    if (t + 1 == t1) tiles.left = 0;
+    tiles.next(base0 + ((t + 1 - t0) & 1) * X::STAGE);
     wait_loads<X::LOADS>();
     const int j0 = t * 32;
     const uint32_t ka = kaddr + ((t - t0) & 1) * X::STAGE, va = vaddr + ((t - t0) & 1) * X::STAGE;
@@ -752,26 +761,16 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dq_ke
 #pragma unroll
   for (int e = 0; e < 16; e++) start[e] = -D[0];
 
-  const uint16_t* kbase = static_cast<const uint16_t*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[2];
-  const uint16_t* vbase = static_cast<const uint16_t*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[2];
-  const uint32_t kst = (uint32_t)(a.k_stride[1] * 2), vst = (uint32_t)(a.v_stride[1] * 2);
-  Loader<F::KROW, kBothWays> lk;
-  Loader<F::VROW, kRowWise> lv;
-  lk.init(wave, lane, kst, a.d);
-  lv.init(wave, lane, vst, a.dv);
-  auto fetch = [&](int blk, uint32_t st) {
-    lk.load(kbase, (int64_t)blk * kBlk, len, kst, a.d, st);
-    lk.load(kbase + a.k_stride[3], (int64_t)blk * kBlk, len, kst, a.d, st + F::KB);
-    lv.load(vbase, (int64_t)blk * kBlk, len, vst, a.dv, st + 2 * F::KB);
-  };
   const uint32_t base0 = lds_offset(smem);
   const uint32_t kra = base0 + row_addr<F::KROW, kBothWays>(lane), kca = base0 + col_addr<F::KROW, kBothWays>(lane, 0);
   const uint32_t vra = base0 + 2 * F::KB + row_addr<F::VROW, kRowWise>(lane);
   const int blk0 = share * P.blocks_per_split, blk1 = min((kend + kBlk - 1) / kBlk, blk0 + P.blocks_per_split);
-  if (blk0 < blk1) fetch(blk0, base0);
+  KeyTiles<F::KROW, F::VROW, kBothWays, kRowWise, kBlk, kThreads / 64> tiles;
+  tiles.init(a, b, hk, blk0 * kBlk, len, wave, lane);
+  if (blk0 < blk1) tiles.next(base0);
   for (int blk = blk0; blk < blk1; blk++) {
     tile_ready();
-    if (blk + 1 < blk1) fetch(blk + 1, base0 + ((blk + 1 - blk0) & 1) * STAGE);
+    if (blk + 1 < blk1) tiles.next(base0 + ((blk + 1 - blk0) & 1) * STAGE);
     const uint32_t stage = ((blk - blk0) & 1) * STAGE;
     if (blk * kBlk >= wmax) continue;
 #pragma unroll 1
@@ -930,7 +929,8 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dkv_k
     const uint32_t vst = (uint32_t)(a.v_stride[1] * 2);
     lv.init(wave, lane, vst, a.dv);
 #pragma unroll
-    for (int x = 0; x < kRows / kBlk; x++) lv.load(vbase, (int64_t)j0 + x * kBlk, len, vst, a.dv, base0 + 2 * STAGE + x * kBlk * F::VROW);
+    for (int x = 0; x < kRows / kBlk; x++)
+      lv.load(reinterpret_cast<const char*>(vbase) + (j0 + x * kBlk) * (int64_t)vst, len - j0 - x * kBlk, vst, a.dv, base0 + 2 * STAGE + x * kBlk * F::VROW);
   } else if (OUT & 1) {
 #pragma unroll
     for (int ks = 0; ks < F::VS; ks++) vf[ks] = global_frag(vbase + jc * a.v_stride[1], valid, ks * 16 + 8 * h, a.dv);
@@ -950,17 +950,30 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dkv_k
   // first query that sees key j: i >= j + NQ - len
   const int shift = a.causal ? a.NQ - len : -a.NK - 1;
   const int first = max(0, (j0 + shift) / ROWS), nblk = j0 < len ? (a.NQ + ROWS - 1) / ROWS : 0;
-  // staged step: query block `blk` of the group's head `g`
-  auto fetch = [&](int g, int blk, uint32_t st) {
+  // the staged queries: running (scalar) addresses, set anew for every head of the group
+  const char *q0 = nullptr, *q1 = nullptr, *go = nullptr;
+  const float* four = nullptr;
+  int left = 0;
+  auto seek = [&](int g, int blk) {
     const int head = hk * P.G + g;
-    const uint16_t* q = static_cast<const uint16_t*>(a.q) + b * a.q_stride[0] + head * a.q_stride[2];
-    const uint16_t* go = static_cast<const uint16_t*>(a.dout) + ((size_t)b * a.NQ * a.H + head) * a.dv;
-    lq.load(q, (int64_t)blk * ROWS, a.NQ, qst, a.d, st);
-    lq.load(q + a.q_stride[3], (int64_t)blk * ROWS, a.NQ, qst, a.d, st + X::KB);
-    lg.load(go, (int64_t)blk * ROWS, a.NQ, gst, a.dv, st + 2 * X::KB);
+    const int64_t row = (int64_t)blk * ROWS;
+    q0 = reinterpret_cast<const char*>(static_cast<const uint16_t*>(a.q) + b * a.q_stride[0] + head * a.q_stride[2]) + row * qst;
+    q1 = q0 + a.q_stride[3] * 2;
+    go = reinterpret_cast<const char*>(static_cast<const uint16_t*>(a.dout) + ((size_t)b * a.NQ * a.H + head) * a.dv) + row * gst;
+    four = P.rows4 + ((size_t)(b * a.H + head) * 4 + wave) * a.NQ + row;
+    left = a.NQ - (int)row;
+  };
+  auto fetch = [&](uint32_t st) {
+    lq.load(q0, left, qst, a.d, st);
+    lq.load(q1, left, qst, a.d, st + X::KB);
+    lg.load(go, left, gst, a.dv, st + 2 * X::KB);
     // a wave each: the four floats of a query.  ROWS floats, then zeros (also past the last query), 64 in all
-    const float* v = P.rows4 + ((size_t)(b * a.H + head) * 4 + wave) * a.NQ + (int64_t)blk * ROWS;
-    load_to_lds4(buffer_at(v, min(ROWS, a.NQ - blk * ROWS) * 4), lane * 4, st + 2 * X::KB + X::VB + wave * kBlk * 4);
+    load_to_lds4(buffer_at(four, min(ROWS, left) * 4), lane * 4, st + 2 * X::KB + X::VB + wave * kBlk * 4);
+    q0 += ROWS * qst;
+    q1 += ROWS * qst;
+    go += ROWS * gst;
+    four += ROWS;
+    left -= ROWS;
   };
   const uint32_t qra = base0 + row_addr<F::KROW, kBothWays>(lane), qca = base0 + col_addr<F::KROW, kBothWays>(lane, 0);
   const uint32_t gra = base0 + 2 * X::KB + row_addr<F::VROW, kBothWays>(lane), gca = base0 + 2 * X::KB + col_addr<F::VROW, kBothWays>(lane, 0);
@@ -969,13 +982,21 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dkv_k
   const int per_head = nblk > first ? nblk - first : 0, steps = per_head * P.G;
   const int step0 = (int)((int64_t)steps * share / P.nsplit), step1 = (int)((int64_t)steps * (share + 1) / P.nsplit);
   int g = per_head > 0 ? step0 / per_head : 0, blk = first + step0 - g * per_head, odd = 0;
-  if (step0 < step1) fetch(g, blk, base0);
+  if (step0 < step1) {
+    seek(g, blk);
+    fetch(base0);
+  }
   for (int step = step0; step < step1; step++) {
     const float sgn = a.lam[hk * P.G + g] > 0.f ? -1.f : 1.f;      // (asked for in front of the next step's loads, which it would wait for)
     tile_ready();
     const int i_blk = blk * ROWS;
-    if (++blk == nblk) { blk = first; g++; }
-    if (step + 1 < step1) fetch(g, blk, base0 + (odd ^ 1) * STAGE);
+    const bool more = step + 1 < step1;
+    if (++blk == nblk) {
+      blk = first;
+      g++;
+      if (more) seek(g, blk);
+    }
+    if (more) fetch(base0 + (odd ^ 1) * STAGE);
     const uint32_t stage = odd * STAGE;
     odd ^= 1;
     if (i_blk + ROWS - 1 < w0 + shift) continue;           // no query of the block sees a key of this wave
