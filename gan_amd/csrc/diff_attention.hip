@@ -151,7 +151,7 @@ struct Loader {
 #pragma unroll
     for (int n = 0; n < NI; n += BASES) {
       const uint32_t skip = (uint32_t)n * step;
-      const u32x4s rs = buffer_at(p + skip, bytes > skip ? bytes - skip : 0u);
+      const u32x4s rs = buffer_at(p + skip, (uint32_t)max((int)bytes - (int)skip, 0));
 #pragma unroll
       for (int b = 0; b < BASES; b++) load_to_lds16(rs, voff[b], lds + (wave + NW * (n + b)) * 1024);
     }
