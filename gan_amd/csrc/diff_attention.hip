@@ -600,6 +600,58 @@ __global__ __launch_bounds__((FewCfg<DK, DV>::NW * 64), 1) void diff_few_rows_ke
   if (valid) store_share<F::VC>(P, ((size_t)share * a.B * a.HK + bh) * R + r, h, acc, mrun, lsum);
 }
 
+// Joins up to 32 shares: DV / 4 lanes per row, four columns of both maps each; a lane forms the weights of all shares for itself.  (A
+// workgroup per row, as for more shares, took eight times the attention's own time with many rows: N 1024, 16 heads of 64/128 in 4
+// shares 315 us in all, against 41.)
+constexpr int kFewShares = 32;
+template <int DV>
+__global__ __launch_bounds__(kThreads) void diff_join_rows_kernel(const DiffParams P) {
+  constexpr int LANES = DV / 4;
+  const gc_diff_attention& a = P.a;
+  const int64_t R = (int64_t)P.G * a.NQ, rows = R * a.B * a.HK, idx = (int64_t)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
+  if (idx >= rows) return;
+  const int c = threadIdx.x % LANES * 4, bh = (int)(idx / R), r = (int)(idx - bh * R), b = bh / a.HK, hk = bh - b * a.HK;
+  const int g = (int)fd_div((uint32_t)r, P.div_nq), i = r - g * a.NQ, head = hk * P.G + g;
+  const float* ml = P.ml + idx * 4;
+  float top[2] = {-INFINITY, -INFINITY}, L[2] = {0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < P.nsplit; s++) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(ml + s * rows * 4);
+#pragma unroll
+    for (int m = 0; m < 2; m++) top[m] = v[2 * m + 1] != 0.f ? fmaxf(top[m], v[2 * m]) : top[m];
+  }
+  f32x4 o1 = {0.f, 0.f, 0.f, 0.f}, o2 = {0.f, 0.f, 0.f, 0.f};
+  const float* part = P.part + idx * 2 * DV + c;
+#pragma unroll 4
+  for (int s = 0; s < P.nsplit; s++) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(ml + s * rows * 4);
+    const f32x4 p1 = *reinterpret_cast<const f32x4*>(part + s * rows * 2 * DV), p2 = *reinterpret_cast<const f32x4*>(part + s * rows * 2 * DV + DV);
+    float w[2];
+#pragma unroll
+    for (int m = 0; m < 2; m++) {
+      // an empty share has no weight; a sum that is not a number has to reach the result
+      const float l = v[2 * m + 1];
+      w[m] = l == 0.f ? 0.f : (l != l ? l : __builtin_amdgcn_exp2f((v[2 * m] - top[m]) * P.c2));
+      L[m] += w[m] * l;
+    }
+    o1 += w[0] * p1;
+    o2 += w[1] * p2;
+  }
+  const float inv0 = L[0] != 0.f ? 1.f / L[0] : 0.f, inv1 = L[1] != 0.f ? 1.f / L[1] : 0.f, lam = a.lam[head];
+  o2 *= inv1;
+  o1 = o1 * inv0 - lam * o2;
+  if (c < a.dv) {
+    const int64_t at = (((int64_t)b * a.NQ + i) * a.H + head) * a.dv + c;
+    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + at) = cvt_bf16x4(o1);
+    if (a.out2 != nullptr) *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out2) + at) = cvt_bf16x4(o2);
+  }
+  if (a.lse != nullptr && c == 0) {
+    float* l = a.lse + ((int64_t)b * a.H + head) * 2 * a.NQ + i;
+    l[0] = L[0] != 0.f ? top[0] * P.c2 + __log2f(L[0]) : INFINITY;
+    l[a.NQ] = L[1] != 0.f ? top[1] * P.c2 + __log2f(L[1]) : INFINITY;
+  }
+}
+
 // Joins the shares of a row that was split over the keys: one workgroup per row.  The shares' weights are worked out first (a thread
 // per share), then every thread adds one value column of one map over every 4th or 8th share, all its loads independent: latency is
 // what this kernel is made of.
@@ -1198,11 +1250,15 @@ void plan_forward(const gc_diff_attention* a, DiffParams& P) {
     P.blocks_per_split = (int)((tiles32 + P.nsplit - 1) / P.nsplit);
     return;
   }
-  // a grid that leaves three quarters of the workgroup slots (two per CU) empty: split, each share at least four blocks
+  // Fewer workgroups than CUs: the keys are split, each share at least four blocks of 64, into as many shares as give every CU one
+  // workgroup.  A second one on a CU makes the walk only 1.2 times as fast, which pays for its join in long walks alone (8192 queries
+  // and keys, 4 heads: 250 us unsplit, 216 in two shares; 2048, 16 heads: 69 and 76), and finds no registers in the widest form.
+  // The join costs about three blocks' time and one more for every 28 workgroups whose rows it reads (N 1024, 4 heads, 16 blocks: 36 us
+  // unsplit, 27 in 4 shares; 16 heads: 38 and 41; N 512, 8 blocks, 1 and 16 heads: 21 and 22 unsplit, 18 and 27 in two shares).
   const int64_t nblk = ((int64_t)a->NK + kBlk - 1) / kBlk, groups = heads * P.tiles;
-  n = groups > 0 ? 2 * cus / groups : 1;
-  if (n < 4) n = 1;
+  n = groups > 0 ? (nblk >= 64 && form_of(a) < 2 ? 2 : 1) * cus / groups : 1;
   if (n > nblk / 4) n = nblk / 4;
+  if (n > 1 && nblk - nblk / n < 3 + groups * n / 28) n = 1;
   if (n > 256) n = 256;
   if (n < 1) n = 1;
   P.blocks_per_split = (int)((nblk + n - 1) / n);
@@ -1321,7 +1377,10 @@ extern "C" int gc_diff_attention_fwd(const gc_diff_attention* desc, void* worksp
   }
   if (P.nsplit > 1) {
     const size_t out_rows = (size_t)desc->B * desc->H * desc->NQ;
-    hipLaunchKernelGGL(diff_join_kernel, dim3((unsigned)out_rows), dim3(kJoinThreads), 0, s, P, DV);
+    if (P.nsplit > kFewShares) hipLaunchKernelGGL(diff_join_kernel, dim3((unsigned)out_rows), dim3(kJoinThreads), 0, s, P, DV);
+    else if (form == 0) hipLaunchKernelGGL(diff_join_rows_kernel<64>, dim3((unsigned)((out_rows + 15) / 16)), dim3(kThreads), 0, s, P);
+    else if (form == 1) hipLaunchKernelGGL(diff_join_rows_kernel<128>, dim3((unsigned)((out_rows + 7) / 8)), dim3(kThreads), 0, s, P);
+    else hipLaunchKernelGGL(diff_join_rows_kernel<256>, dim3((unsigned)((out_rows + 3) / 4)), dim3(kThreads), 0, s, P);
     return check_hip(hipGetLastError(), "diff_join launch");
   }
   return GC_OK;

@@ -406,6 +406,11 @@ ATTENTION_CASES = [
     (1, 700, 700, 3, 1, 32, 64, True, None, 1.0),
     (1, 520, 300, 2, 1, 64, 128, False, None, 1.0),
     (1, 300, 520, 2, 2, 128, 256, False, (500,), 1.0),
+    # a few shares of the keys for many rows (some of the shares without a visible key), and many shares for more rows than a short run
+    (1, 600, 1100, 2, 1, 32, 64, True, (1000,), 1.0),
+    (3, 260, 1030, 1, 1, 72, 136, False, (0, 1030, 70), 1.0),
+    (1, 130, 2200, 2, 2, 64, 128, True, (40,), 1.0),
+    (1, 40, 9000, 1, 1, 64, 128, True, None, 1.0),
 ]
 
 
