@@ -794,6 +794,13 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dq_ke
     for (int ks = 0; ks < F::KS; ks++) qf[m][ks] = global_frag(qrow + m * a.q_stride[3], valid, ks * 16 + 8 * h, a.d);
 #pragma unroll
   for (int ks = 0; ks < F::VS; ks++) gf[ks] = global_frag(grow, valid, ks * 16 + 8 * h, a.dv);
+  // The matrix unit rounds its sums down by a small part of their last bit, whatever their sign.  The sum of 1e5 rows that makes dlam
+  // showed it (1e-7 of the terms' sizes, 3e-5 of what is left of them); with dP of every other row formed with its sign turned the
+  // bias cancels (4096 queries, batch 32: off by 3.5e-3 for every input, and by 1e-4 either way).
+  const float turn = (r & 1) ? -1.f : 1.f;
+  if (r & 1)
+#pragma unroll
+    for (int ks = 0; ks < F::VS; ks++) gf[ks] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, gf[ks]) ^ 0x80008000u);
   float L[2], D[2];
 #pragma unroll
   for (int m = 0; m < 2; m++) {
@@ -807,11 +814,11 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dq_ke
   for (int m = 0; m < 2; m++)
 #pragma unroll
     for (int cb = 0; cb < F::KC; cb++) acc[m][cb] = zero16();
-  float left = 0.f;                                        // sum_j p2 (dP - delta2)
-  const float gap = D[0] - D[1];
+  float left = 0.f;                                        // sum_j p2 (dP - delta2), its sign turned in odd rows
+  const float gap = turn * (D[0] - D[1]);
   f32x16 start;
 #pragma unroll
-  for (int e = 0; e < 16; e++) start[e] = -D[0];
+  for (int e = 0; e < 16; e++) start[e] = -turn * D[0];
 
   const uint32_t base0 = lds_offset(smem);
   const uint32_t kra = base0 + row_addr<F::KROW, kBothWays>(lane), kca = base0 + col_addr<F::KROW, kBothWays>(lane, 0);
@@ -885,7 +892,7 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dq_ke
   }
   const float lam = a.lam[head];
   if (valid) {
-    const float f[2] = {a.scale, -lam * a.scale};
+    const float f[2] = {turn * a.scale, -turn * lam * a.scale};
     const size_t row = (((size_t)b * a.NQ + i) * a.H + head) * 2 * a.d;
     uint16_t* dst = static_cast<uint16_t*>(a.dq) + row;
     float* part = P.part + (size_t)share * a.B * a.NQ * a.H * 2 * a.d + row;
@@ -902,7 +909,7 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dq_ke
           else *reinterpret_cast<u32x2*>(dst + m * a.d + c) = cvt_bf16x4(v);
         }
   }
-  float t = valid ? left + (h == 0 && share == 0 ? D[1] : 0.f) : 0.f;
+  float t = valid ? turn * left + (h == 0 && share == 0 ? D[1] : 0.f) : 0.f;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
   if (lane == 0) red[wave] = t;

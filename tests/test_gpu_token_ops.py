@@ -538,6 +538,27 @@ def test_differential_attention_gradients_against_differences(F):
     assert abs(diff - along) < 2.0 ** -7 * float(gq.double().norm()) * 4 + 1e-6 * abs(diff), (diff, along)
 
 
+def test_differential_attention_weight_gradient_of_many_rows(F):
+    """dlam is one sum over 131072 rows of either sign: a rounding that always goes one way would add up.  A row's term, dO . O2, is a
+    difference of sums of fp32 values no larger than S = |delta1| + |delta2| + sum_j p2 |dP|, each step of them off by half of 2^-23 of S
+    at most; three steps (the products' sum, the start value, the sum over the keys) and independent signs leave
+    sqrt(sum S^2) x 3 x 2^-24, four times which nothing should pass."""
+    B, N, d, dv = 32, 4096, 64, 128
+    g = torch.Generator(device="cuda").manual_seed(6)
+    q, k = (torch.randn(B, N, 1, 2, d, generator=g, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    v, dout = (torch.randn(B, N, 1, dv, generator=g, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    lam = torch.tensor([0.4], device="cuda", requires_grad=True)
+    got, = torch.autograd.grad(F.differential_attention(q, k, v, lam), lam, dout)
+    want, spread = 0.0, 0.0
+    for b in range(B):
+        dP = dout[b, :, 0].double() @ v[b, :, 0].double().t().contiguous()
+        P = [torch.softmax(q[b, :, 0, m].double() @ k[b, :, 0, m].double().t().contiguous() * d ** -0.5, -1) for m in range(2)]
+        d1, d2 = ((p * dP).sum(-1) for p in P)
+        want -= float(d2.sum())
+        spread += float(((d1.abs() + d2.abs() + (P[1] * dP.abs()).sum(-1)) ** 2).sum())
+    assert abs(float(got) - want) <= 4 * 3 * 2.0 ** -24 * math.sqrt(spread), (float(got) - want, math.sqrt(spread))
+
+
 def test_differential_attention_empty_tensors(F):
     for B, NQ, NK in ((0, 4, 4), (2, 0, 5), (2, 3, 0)):
         q = torch.randn(B, NQ, 2, 2, 32, device="cuda").bfloat16().requires_grad_(True)
