@@ -110,12 +110,12 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryParams P) 
       const bool turned = c < turn_units;
       const int x0 = turned ? c * W : 2 * np + (c - turn_units) * W, y0 = NEIGHBOURS || !turned ? x0 : np + x0;
       // all samples of this item: the next sample's elements are asked for before this one's are turned
-      Vec<T> vx = get<T>(src, in + x0), vy = vx;
+      Vec<T> vx = get<T>(src, in + x0), vy;
       if (!NEIGHBOURS) vy = get<T>(src, in + y0);
       for (int b = 0; b < nb; b++, in += in_step, out += out_step) {
         float x[W], y[W];
         widen<T>(vx, x);
-        widen<T>(vy, y);
+        widen<T>(NEIGHBOURS ? vx : vy, y);
         if (b + 1 < nb) {
           vx = get<T>(src, in + in_step + x0);
           if (!NEIGHBOURS) vy = get<T>(src, in + in_step + y0);

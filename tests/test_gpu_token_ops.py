@@ -330,6 +330,22 @@ def test_axial_rotary_strides_single_gradient_and_empty(F):
     assert e.shape == (2, 0, 4, 16) and f_.shape == (2, 0, 4, 16)
 
 
+@pytest.mark.parametrize("extra", [0, 8, 3])
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_axial_rotary_of_many_samples_equals_each_alone(F, dt, interleaved, extra):
+    """Large batches with shared positions give a workgroup several samples: every sample has to come out as in a call of its own, its
+    elements behind the turned pairs unchanged.  The last workgroup's run of samples is a short one."""
+    B, N, D = 155, 1024, 16 + extra
+    q = torch.randn(B, N, 1, D, generator=torch.Generator().manual_seed(1)).to(dt).cuda()
+    table = F.rotary_table((8, 8), interleaved=interleaved, device="cuda")
+    pos = torch.arange(2 * N, device="cuda").view(N, 2)
+    out = F.axial_rotary(q, None, pos, table)
+    assert torch.equal(out[..., 16:], q[..., 16:])
+    for b in (0, 1, 2, 3, 77, 151, 152, 153, 154):
+        assert torch.equal(out[b:b + 1], F.axial_rotary(q[b:b + 1], None, pos, table)), b
+
+
 # ---- differential attention ------------------------------------------------------------------------------------------------
 def _attention_reference(q, k, v, lam, scale, causal, lengths, dout):
     """Output, gradients and their error bounds in float64.  u = 2^-8 * 1.06: a bf16 rounding of an intermediate, with room for the
