@@ -252,6 +252,49 @@ def test_block_norm_empty_rows_and_zero_rows(F):
     assert float(h.abs().max()) == 0.0 and torch.isfinite(gx).all()
 
 
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,C", [(150000, 16), (150000, 40), (20000, 256), (20002, 387), (9000, 1040), (5000, 4096)])
+@pytest.mark.parametrize("part", ["in", "out", "both"])
+def test_block_norm_of_many_rows_equals_a_few_alone(F, part, rows, C, dt, kind):
+    """A workgroup walks many rows, asking for the next while it works on one: a row's outputs and gradients have to be those of a
+    call on a few rows (the same kernel and the same order of sums), and the parameters' gradients the sum over three parts of the rows.
+    Those are sums of n terms of size one: runs of m <= 1000 rows whose partial sums stay below 4 sqrt(m), each step off by half a unit
+    of that with either sign, n / m of them: 4 x 2^-24 x sqrt(m n) < 128 x 2^-24 sqrt(n), and four times that for products of two or
+    three normal factors."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    x, f = r(1, rows, C).to(dt).requires_grad_(True), r(1, rows, C).to(dt).requires_grad_(True)
+    ow, gate, iw = (r(C).requires_grad_(True) for _ in range(3))
+    dy, dh = r(1, rows, C).to(dt), r(1, rows, C).to(dt)
+
+    def call(lo, hi):
+        a, b = x[:, lo:hi], f[:, lo:hi]
+        if part == "in":
+            outs, seeds, leaves = (F.block_input_norm(a, iw, kind=kind),), (dh[:, lo:hi],), (x, iw)
+        elif part == "out":
+            outs, seeds, leaves = (F.block_output_norm(a, b, ow, gate=gate, kind=kind),), (dy[:, lo:hi],), (x, f, ow, gate)
+        else:
+            outs, seeds, leaves = F.block_boundary_norm(a, b, ow, iw, gate=gate, kind=kind), (dy[:, lo:hi], dh[:, lo:hi]), (x, f, ow, gate, iw)
+        grads = torch.autograd.grad(outs, leaves, seeds)
+        rowwise = [t.detach() for t in outs] + [t[:, lo:hi] for t in grads if t.dim() == 3]
+        return rowwise, [t for t in grads if t.dim() == 1]
+
+    whole, params = call(0, rows)
+    step = 8 * ((rows // 3) // 8)
+    sums = None
+    for lo in range(0, rows, step):
+        hi = min(rows, lo + step)
+        some, ps = call(lo, hi)
+        sums = [p.double() for p in ps] if sums is None else [a + p.double() for a, p in zip(sums, ps)]
+    for p, q in zip(params, sums):
+        assert float((p.double() - q).abs().max()) <= 4 * 128 * 2.0 ** -24 * rows ** 0.5
+    for lo in (0, 8 * (rows // 16), 8 * ((rows - 17) // 8)):
+        few, _ = call(lo, min(rows, lo + 16))
+        for n, (a, b) in enumerate(zip(whole, few)):
+            assert torch.equal(a[:, lo:lo + 16], b), (n, lo)
+
+
 # ---- rotary --------------------------------------------------------------------------------------------------------------
 def _rotary_reference(t, positions, dims, bases, interleaved, sign):
     w = torch.cat([torch.tensor(b, dtype=torch.float64) ** (-torch.arange(0, n, 2, dtype=torch.float64) / n) for n, b in zip(dims, bases)])
