@@ -1209,7 +1209,7 @@ int check_desc(const gc_diff_attention* a, bool backward) {
     set_error("differential attention: too many rows (B=%d NQ=%d NK=%d H=%d)", a->B, a->NQ, a->NK, a->H);
     return GC_UNSUPPORTED_GEOMETRY;
   }
-  if (!(a->scale > 0.f) || a->scale > 1e30f) { set_error("differential attention: scale must be positive and finite"); return GC_BAD_ARGUMENT; }
+  if (!(a->scale >= 1e-30f) || a->scale > 1e30f) { set_error("differential attention: scale must be positive and finite (1e-30 to 1e30)"); return GC_BAD_ARGUMENT; }
   for (int i = 0; i < 4; i++)
     if (a->q_stride[i] % 8 != 0 || a->k_stride[i] % 8 != 0 || (i < 3 && a->v_stride[i] % 8 != 0)) {
       set_error("differential attention: strides must be multiples of 8 elements");

@@ -356,10 +356,15 @@ class DifferentialAttention2d(torch.nn.Module):
     def positions(self, height, width, device):
         """Row and column of every position, [H * W, 2] (made once per size and device)."""
         key = (height, width, device)
-        if key not in self._positions:
-            n = torch.arange(height * width, device=device, dtype=torch.int32)
-            self._positions[key] = torch.stack((n // width, n % width), dim=1)
-        return self._positions[key]
+        found = self._positions.get(key)
+        if found is None:
+            with torch.inference_mode(False):              # (a training step may be the next to save it)
+                n = torch.arange(height * width, device=device, dtype=torch.int32)
+                found = torch.stack((n // width, n % width), dim=1)
+            # one made while a graph is recorded holds nothing until that graph runs: it stays the recording's own
+            if not (found.is_cuda and torch.cuda.is_current_stream_capturing()):
+                self._positions[key] = found
+        return found
 
     def __deepcopy__(self, memo):
         copy = self.__class__.__new__(self.__class__)

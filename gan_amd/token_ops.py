@@ -119,8 +119,22 @@ def _param(who, name, t, C, B=None):
 _KINDS = {"rms": 0, "layer": 1}
 
 
-def _norm_forward(cfg, x, f, out_weight, out_bias, gate, rho, in_weight, in_bias, scale, shift, stats_wanted):
-    """(y or None, h or None, what the backward pass needs)"""
+def _copies(given, used):
+    """What a backward pass keeps of the tensors that a descriptor points to: the copies that were made of them.  Those that are the
+    given tensors themselves are saved by autograd and may lie elsewhere when it hands them back (offloaded, gathered anew)."""
+    return [u if (u is not None and u.data_ptr() != t.data_ptr()) else (t if t is None else t.stride()) for t, u in zip(given, used)]
+
+
+def _moved(given, copies, pointers):
+    """Whether a tensor that the descriptor points to directly lies elsewhere or otherwise by now"""
+    for t, c, p in zip(given, copies, pointers):
+        if type(c) is tuple and (t.data_ptr() != p or t.stride() != c):
+            return True
+    return False
+
+
+def _norm_layout(cfg, x, f, out_weight, out_bias, gate, rho, in_weight, in_bias, scale, shift):
+    """(the descriptor's fields up to the outputs, the tensors that they point to)"""
     who, layer, eps, with_in, constant = cfg
     B, C = x.size(0), x.size(-1)
     ow, _ = _param(who, "out_weight", out_weight, C)
@@ -145,38 +159,49 @@ def _norm_forward(cfg, x, f, out_weight, out_bias, gate, rho, in_weight, in_bias
     batch, per = B, rows
     if shared and (x.dim() == 2 or (xb == rows * xs and (fr is None or fb == rows * fs))):
         batch, per = 1, B * rows
+    head = (batch, per, C, _code(who, x), layer, with_in, eps, constant, gate_per, mod_per, per_channel, 0, xb, xs, fb, fs, xr.data_ptr(), _p(fr),
+            _p(ow), _p(ob), _p(gt), _p(rt), _p(iw), _p(ib), _p(sc), _p(sh))
+    return head, (xr, fr, ow, ob, gt, rt, iw, ib, sc, sh)
+
+
+def _norm_forward(cfg, tensors, stats_wanted):
+    """(y or None, h or None, statistics or None, descriptor fields, the tensors they point to)"""
+    x = tensors[0]
     with _on(x):
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if f is not None else None
-        h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if with_in else None
-        stats = torch.empty(4 * B * rows, dtype=torch.float32, device=x.device) if stats_wanted else None
-        head = (batch, per, C, _code(who, x), layer, with_in, eps, constant, gate_per, mod_per, per_channel, 0, xb, xs, fb, fs, xr.data_ptr(), _p(fr),
-                _p(ow), _p(ob), _p(gt), _p(rt), _p(iw), _p(ib), _p(sc), _p(sh))
+        head, used = _norm_layout(cfg, *tensors)
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if tensors[1] is not None else None
+        h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if cfg[3] else None
+        stats = torch.empty(4 * (x.numel() // x.size(-1)), dtype=torch.float32, device=x.device) if stats_wanted else None
         if x.numel():
             rc = _lib.lib().gc_block_norm_fwd(_NORM.pack(*head, _p(y), _p(h), _p(stats), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0), _stream(x))
             if rc:
                 _lib.check(rc, "gc_block_norm_fwd")
-    return y, h, (head, stats, (xr, fr, ow, ob, gt, rt, iw, ib, sc, sh))
+    return y, h, stats, head, used
 
 
 class _BlockNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, cfg, x, f, *params):
-        y, h, ctx.kept = _norm_forward(cfg, x, f, *params, True)
+    def forward(ctx, cfg, *tensors):
+        y, h, ctx.stats, ctx.head, used = _norm_forward(cfg, tensors, True)
+        ctx.copies = _copies(tensors, used)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x, f, *params)
-        ctx.who = cfg[0]
+        ctx.save_for_backward(*tensors)
+        ctx.cfg = cfg
         return (y, h) if (y is not None and h is not None) else (y if y is not None else h)
 
     @staticmethod
     def backward(ctx, *gs):
-        _no_second_order(ctx.who, *gs)
-        x, f, *given = ctx.saved_tensors               # (raises if one of them was written since)
-        head, stats, _ = ctx.kept
+        _no_second_order(ctx.cfg[0], *gs)
+        tensors = ctx.saved_tensors                    # (raises if one of them was written since)
+        x, f, *given = tensors
+        head, stats, used = ctx.head, ctx.stats, None
         dy, dh = (gs if len(gs) == 2 else ((gs[0], None) if f is not None else (None, gs[0])))
         if dy is None and dh is None:
             return (None,) * 11
         dev, empty = x.device, x.numel() == 0
         with _on(x):
+            if _moved(tensors, ctx.copies, head[16:]):
+                head, used = _norm_layout(ctx.cfg, *tensors)
             dy, dh = (None if g is None else (g if g.dtype == x.dtype else g.to(x.dtype)).contiguous() for g in (dy, dh))
             make = torch.zeros if empty else torch.empty
             dx = make(x.shape, dtype=x.dtype, device=dev)
@@ -213,7 +238,7 @@ def block_norm(who, x, f, out_weight, out_bias, gate, residual_scale, in_weight,
     cfg = (who, _KINDS[kind], eps, int(with_input_norm), constant)
     if _graph_follows(*tensors):
         return _BlockNorm.apply(cfg, *tensors)
-    y, h, _ = _norm_forward(cfg, *tensors, False)
+    y, h, *_ = _norm_forward(cfg, tensors, False)
     return (y, h) if (y is not None and h is not None) else (y if y is not None else h)
 
 
@@ -343,15 +368,23 @@ def _aligned(t, width):
     return t, st
 
 
-def _attention_forward(q, k, v, lam, lengths, causal, scale, grads):
+def _attention_layout(q, k, v, lam, lengths, causal, scale):
+    """(the descriptor's fields up to the outputs, the tensors that they point to)"""
     B, NQ, H, _, d = q.shape
     _, NK, HK, dv = v.shape
     (qa, qs), (ka, ks), (va, vs), la = _aligned(q, d), _aligned(k, d), _aligned(v, dv), _fp32(lam)
+    head = (*qs, *ks, *vs, B, NQ, NK, H, HK, d, dv, causal, scale, 0, qa.data_ptr(), ka.data_ptr(), va.data_ptr(), la.data_ptr(), _p(lengths))
+    return head, (qa, ka, va, la, lengths)
+
+
+def _attention_forward(q, k, v, lam, lengths, causal, scale, grads):
+    B, NQ, H = q.shape[:3]
+    NK, dv = v.size(1), v.size(3)
     with _on(q):
+        head, used = _attention_layout(q, k, v, lam, lengths, causal, scale)
         out = (torch.empty if NK else torch.zeros)(B, NQ, H, dv, dtype=q.dtype, device=q.device)
         out2 = torch.empty(out.shape, dtype=q.dtype, device=q.device) if grads else None
         lse = torch.empty(B, H, 2, NQ, dtype=torch.float32, device=q.device) if grads else None
-        head = (*qs, *ks, *vs, B, NQ, NK, H, HK, d, dv, causal, scale, 0, qa.data_ptr(), ka.data_ptr(), va.data_ptr(), la.data_ptr(), _p(lengths))
         if NK and out.numel():
             L = _lib.lib()
             desc = _ATTENTION.pack(*head, out.data_ptr(), _p(out2), _p(lse), 0, 0, 0, 0, 0)
@@ -360,29 +393,32 @@ def _attention_forward(q, k, v, lam, lengths, causal, scale, grads):
             rc = L.gc_diff_attention_fwd(desc, _p(ws), n, _stream(q))
             if rc:
                 _lib.check(rc, "gc_diff_attention_fwd")
-    return out, (head, out2, lse, (qa, ka, va, la, lengths))
+    return out, out2, lse, head, used
 
 
 class _DiffAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lam, lengths, causal, scale):
-        out, ctx.kept = _attention_forward(q, k, v, lam, lengths, causal, scale, True)
+        out, ctx.out2, ctx.lse, ctx.head, used = _attention_forward(q, k, v, lam, lengths, causal, scale, True)
+        ctx.copies = _copies((q, k, v, lam, lengths), used)
         ctx.save_for_backward(q, k, v, lam, lengths, out)
+        ctx.cfg = (causal, scale)
         return out
 
     @staticmethod
     def backward(ctx, g):
         _no_second_order("differential_attention", g)
         q, k, v, lam, lengths, out = ctx.saved_tensors
-        head, out2, lse, _ = ctx.kept
+        head, out2, lse, used = ctx.head, ctx.out2, ctx.lse, None
         with _on(q):
             if not (out.numel() and k.size(1)):
                 return tuple(torch.zeros_like(t) for t in (q, k, v, lam)) + (None,) * 3
             dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
             dlam = torch.empty(lam.shape, dtype=torch.float32, device=q.device)
-            g = (g if g.dtype == q.dtype else g.to(q.dtype)).contiguous()
-            if g.data_ptr() % 16:
-                g = g.clone()
+            if _moved((q, k, v, lam, lengths), ctx.copies, head[21:]):
+                head, used = _attention_layout(q, k, v, lam, lengths, *ctx.cfg)
+            g, out = ((t if t.dtype == q.dtype else t.to(q.dtype)).contiguous() for t in (g, out))
+            g, out = (t.clone() if t.data_ptr() % 16 else t for t in (g, out))
             L = _lib.lib()
             desc = _ATTENTION.pack(*head, out.data_ptr(), out2.data_ptr(), lse.data_ptr(), g.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                    dlam.data_ptr())
@@ -410,8 +446,8 @@ def differential_attention(q, k, v, lam, scale=None, causal=False, key_lengths=N
         if t.dtype != torch.bfloat16:
             _refuse(f"{who}: operands are bf16, got {t.dtype}")
     scale = d ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < 1e30:
-        _refuse(f"{who}: scale must be positive and finite, got {scale}")
+    if not 1e-30 < scale < 1e30:
+        _refuse(f"{who}: scale must be positive and finite (1e-30 to 1e30), got {scale}")
     if key_lengths is not None and (key_lengths.dim() != 1 or key_lengths.numel() != B or key_lengths.dtype not in (torch.int32, torch.int64)):
         _refuse(f"{who}: key_lengths must be int32 or int64 [{B}]")
     _same_gpu(who, q, k, v, lam, key_lengths)

@@ -5,6 +5,7 @@ Bounds are elementwise and counted, not chosen: a stored bf16 value is off by at
 one by 2^-24; where a kernel rounds an intermediate to bf16 (the probabilities and score gradients of the attention), 2^-8 of every
 addend's magnitude is carried through the formula with absolute values.  Sums of n fp32 addends are off by at most their depth
 times 2^-24 of the sum of magnitudes; DEPTH bounds every summation depth in the kernels."""
+import contextlib
 import math
 
 import pytest
@@ -753,3 +754,41 @@ def test_second_order_and_changed_operands_are_refused(F):
     v.zero_()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         out.float().sum().backward()
+
+
+def test_saved_tensors_that_come_back_elsewhere(F):
+    """Tensors offloaded between the passes (saved-tensor hooks) come back at other addresses, sliced ones with other strides, and a
+    parameter's storage may be given up and gathered anew: the backward pass reads them where they are then."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    qkv = r(2, 70, 2, 2, 96).bfloat16().requires_grad_(True)
+    lam, x, w, gate = r(2).requires_grad_(True), r(2, 70, 128).requires_grad_(True), r(128).requires_grad_(True), r(2, 128).bfloat16().requires_grad_(True)
+    dout = r(2, 70, 128)
+    table, places = F.rotary_table((16, 16), device="cuda"), torch.arange(140, device="cuda").view(70, 2)
+
+    def grads(hooks, between=lambda: None):
+        with hooks:
+            q, k = F.axial_rotary(qkv[..., :32].reshape(2, 70, 4, 32), qkv[..., 32:64].reshape(2, 70, 4, 32), places, table)
+            a = F.differential_attention(q.view(2, 70, 2, 2, 32), qkv[..., 32:64], qkv[:, :, :, 0, 32:], lam)
+            y, h = F.block_boundary_norm(x, a.float().flatten(2), w, None, gate=gate, residual_scale=w)
+            loss = ((y + h) * dout).sum()
+        between()
+        return torch.autograd.grad(loss, (qkv, lam, x, w, gate))
+
+    class Elsewhere(torch.autograd.graph.saved_tensors_hooks):
+        def __init__(self):
+            super().__init__(lambda t: (t.cpu(), t.stride()), lambda p: torch.cat([p[0].flatten()[:1], p[0].flatten()]).cuda()[1:].view(p[0].shape))
+
+    plain = grads(contextlib.nullcontext())
+    assert all(torch.equal(a, b) for a, b in zip(plain, grads(torch.autograd.graph.save_on_cpu())))
+    # off by one element the norm's kernel takes narrower accesses and adds in another order; the bf16 gradient that reaches the attention
+    # then rounds to a neighbouring value here and there, 2^-7 of itself, and all others are linear in it
+    for a, b in zip(plain, grads(Elsewhere())):
+        assert float((a.float() - b.float()).norm()) <= 2.0 ** -7 * float(a.float().norm())
+
+    def gather_anew():
+        old = w.data
+        w.data = old.clone()
+        old.fill_(float("nan"))
+
+    assert all(torch.equal(a, b) for a, b in zip(plain, grads(contextlib.nullcontext(), gather_anew)))

@@ -79,6 +79,8 @@ def test_attention_refusals():
         call(torch.zeros(2, 5, 4, 2, 136, dtype=bf), torch.zeros(2, 7, 2, 2, 136, dtype=bf), v, lam)
     with pytest.raises(RuntimeError, match="scale"):
         call(q, k, v, lam, scale=0.0)
+    with pytest.raises(RuntimeError, match="scale"):
+        call(q, k, v, lam, scale=1e-38)
     with pytest.raises(RuntimeError, match="key_lengths"):
         call(q, k, v, lam, key_lengths=torch.zeros(3, dtype=torch.int32))
     with pytest.raises(RuntimeError, match="key_lengths"):
@@ -230,3 +232,13 @@ def test_modules_and_the_biggan_option():
     assert "main_sequence.4.blocks.0.qkv.U_vector" in g.state_dict()
     with pytest.raises(KeyError):
         H.Generator(10, 16, attention="none")
+
+
+def test_positions_made_in_inference_mode_serve_training():
+    from gan_amd import nn as gnn
+
+    block = gnn.DifferentialAttention2d(32, heads=1)
+    with torch.inference_mode():
+        first = block.positions(3, 5, torch.device("cpu"))
+    assert not first.is_inference() and block.positions(3, 5, torch.device("cpu")) is first
+    assert first.tolist() == [[i, j] for i in range(3) for j in range(5)]
