@@ -24,6 +24,8 @@
 // between d and its padded width, are answered with zeros by the buffer's range check, so nothing behind a sample's length is read.
 // Probabilities and score gradients are rounded to bf16 for the second products (the operands' own type; 2^-9 each, independent),
 // everything else is fp32.
+#include <algorithm>
+
 #include "common.h"
 
 namespace gc {
@@ -324,6 +326,35 @@ __device__ __forceinline__ void store_share(const DiffParams& P, size_t row, int
             f32x4{acc[m][cb][4 * e], acc[m][cb][4 * e + 1], acc[m][cb][4 * e + 2], acc[m][cb][4 * e + 3]};
 }
 
+// A finished row: out = O1 - lam O2, and for a backward pass O2 and the log2-sums
+template <int VC>
+__device__ __forceinline__ void store_row(const DiffParams& P, const f32x16 (&acc)[2][VC], const float (&mrun)[2], const float (&lsum)[2], int b, int i,
+                                          int head, int h) {
+  const gc_diff_attention& a = P.a;
+  const float inv0 = lsum[0] != 0.f ? 1.f / lsum[0] : 0.f, inv1 = lsum[1] != 0.f ? 1.f / lsum[1] : 0.f, lam = a.lam[head];
+  const size_t orow = (((size_t)b * a.NQ + i) * a.H + head) * a.dv;
+#pragma unroll
+  for (int cb = 0; cb < VC; cb++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const int c = cb * 32 + 8 * e + 4 * h;
+      if (c >= a.dv) continue;
+      f32x4 o2, o;
+#pragma unroll
+      for (int x = 0; x < 4; x++) {
+        o2[x] = acc[1][cb][4 * e + x] * inv1;
+        o[x] = acc[0][cb][4 * e + x] * inv0 - lam * o2[x];
+      }
+      *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + orow + c) = cvt_bf16x4(o);
+      if (a.out2 != nullptr) *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out2) + orow + c) = cvt_bf16x4(o2);
+    }
+  if (a.lse != nullptr && h == 0) {
+    float* l = a.lse + ((size_t)b * a.H + head) * 2 * a.NQ + i;
+    l[0] = lsum[0] != 0.f ? mrun[0] * P.c2 + __log2f(lsum[0]) : INFINITY;
+    l[a.NQ] = lsum[1] != 0.f ? mrun[1] * P.c2 + __log2f(lsum[1]) : INFINITY;
+  }
+}
+
 // ---------------------------------------------------------------------------------------------------------------------------
 // Rows of a workgroup: 128 of the G * NQ rows (head of the group, query) that share a key head.
 template <int DK, int DV>
@@ -472,33 +503,14 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_fwd_kerne
     store_share<F::VC>(P, ((size_t)split * a.B * a.HK + bh) * R + r, h, acc, mrun, lsum);
     return;
   }
-  const float inv0 = lsum[0] != 0.f ? 1.f / lsum[0] : 0.f, inv1 = lsum[1] != 0.f ? 1.f / lsum[1] : 0.f, lam = a.lam[head];
-  const size_t orow = (((size_t)b * a.NQ + i) * a.H + head) * a.dv;
-#pragma unroll
-  for (int cb = 0; cb < F::VC; cb++)
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const int c = cb * 32 + 8 * e + 4 * h;
-      if (c >= a.dv) continue;
-      f32x4 o2, o;
-#pragma unroll
-      for (int x = 0; x < 4; x++) {
-        o2[x] = acc[1][cb][4 * e + x] * inv1;
-        o[x] = acc[0][cb][4 * e + x] * inv0 - lam * o2[x];
-      }
-      *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + orow + c) = cvt_bf16x4(o);
-      if (a.out2 != nullptr) *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out2) + orow + c) = cvt_bf16x4(o2);
-    }
-  if (a.lse != nullptr && h == 0) {
-    float* l = a.lse + ((size_t)b * a.H + head) * 2 * a.NQ + i;
-    l[0] = lsum[0] != 0.f ? mrun[0] * P.c2 + __log2f(lsum[0]) : INFINITY;
-    l[a.NQ] = lsum[1] != 0.f ? mrun[1] * P.c2 + __log2f(lsum[1]) : INFINITY;
-  }
+  store_row<F::VC>(P, acc, mrun, lsum, b, i, head, h);
 }
 
 // At most 32 rows per key head (single queries and short runs of them against long keys): bound by reading the keys and values once.
 // Every wave walks a share of the keys of its own in tiles of 32, staged privately (no barriers; the loads of the next tile are in
-// flight while one is worked on), so that a CU keeps 64 KiB of loads under way; the shares are joined by diff_join_kernel.  The matrix
+// flight while one is worked on), so that a CU keeps 64 KiB of loads under way; the waves' shares become one in LDS (4 x 65536 keys, 16
+// heads on 4: 117 us either way; 16384 keys, one head: 32 us with every wave's share left to the joining kernel, 20 so), the
+// workgroups' are joined by a second launch, or the row is finished where there is one.  The matrix
 // instructions are idle most of the time here, which pays for probabilities held to 16 bits: their bf16 rounding and its remainder
 // are multiplied with the values separately.
 template <int DK, int DV>
@@ -527,7 +539,7 @@ __global__ __launch_bounds__((FewCfg<DK, DV>::NW * 64), 1) void diff_few_rows_ke
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const gc_diff_attention& a = P.a;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), h = lane >> 5;
-  const int bh = (int)(blockIdx.x / ((uint32_t)P.nsplit / X::NW)), share = (int)(blockIdx.x % ((uint32_t)P.nsplit / X::NW)) * X::NW + wave;
+  const int bh = (int)(blockIdx.x / (uint32_t)P.nsplit), share = (int)(blockIdx.x % (uint32_t)P.nsplit);
   const int b = bh / a.HK, hk = bh - b * a.HK, R = P.G * a.NQ, len = sample_length(a, b), r = lane & 31;
   const bool valid = r < R;
   const int rc = valid ? r : R - 1, g = (int)fd_div((uint32_t)rc, P.div_nq), i = rc - g * a.NQ, head = hk * P.G + g;
@@ -548,7 +560,7 @@ __global__ __launch_bounds__((FewCfg<DK, DV>::NW * 64), 1) void diff_few_rows_ke
 
   const uint32_t base0 = lds_offset(smem) + wave * 2 * X::STAGE;
   const uint32_t kaddr = base0 + row_addr<F::KROW, kRowWise>(lane), vaddr = base0 + 2 * X::KB + col_addr<F::VROW, kTransposed>(lane, 0);
-  const int t0 = share * P.blocks_per_split, t1 = min((wmax + 31) / 32, t0 + P.blocks_per_split);
+  const int t0 = (share * X::NW + wave) * P.blocks_per_split, t1 = min((wmax + 31) / 32, t0 + P.blocks_per_split);
   KeyTiles<F::KROW, F::VROW, kRowWise, kTransposed, 32, 1> tiles;
   tiles.init(a, b, hk, t0 * 32, len, 0, lane);
   if (t0 < t1) tiles.next(base0);
@@ -594,10 +606,52 @@ __global__ __launch_bounds__((FewCfg<DK, DV>::NW * 64), 1) void diff_few_rows_ke
         }
       }
   }
-  wait_loads<0>();                                         // (nothing of this wave is still writing LDS when the workgroup ends)
+  wait_loads<0>();                                         // (nothing of this wave is still writing LDS)
   lsum[0] = half_sum(lsum[0]);
   lsum[1] = half_sum(lsum[1]);
-  if (valid) store_share<F::VC>(P, ((size_t)share * a.B * a.HK + bh) * R + r, h, acc, mrun, lsum);
+  // The waves' shares become one, by halves, through the LDS that held the tiles
+  f32x4* const half = reinterpret_cast<f32x4*>(smem) + lane;
+  constexpr int ITEMS = 8 * F::VC + 1;
+#pragma unroll
+  for (int n = X::NW / 2; n > 0; n /= 2) {
+    __syncthreads();
+    if (wave >= n && wave < 2 * n && valid) {
+      f32x4* p = half + (wave - n) * ITEMS * 64;
+#pragma unroll
+      for (int m = 0; m < 2; m++)
+#pragma unroll
+        for (int cb = 0; cb < F::VC; cb++)
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            p[((m * F::VC + cb) * 4 + e) * 64] = f32x4{acc[m][cb][4 * e], acc[m][cb][4 * e + 1], acc[m][cb][4 * e + 2], acc[m][cb][4 * e + 3]};
+      p[8 * F::VC * 64] = f32x4{mrun[0], lsum[0], mrun[1], lsum[1]};
+    }
+    __syncthreads();
+    if (wave < n && valid) {
+      const f32x4* p = half + wave * ITEMS * 64;
+      const f32x4 ml = p[8 * F::VC * 64];
+#pragma unroll
+      for (int m = 0; m < 2; m++) {
+        const float mn = fmaxf(mrun[m], ml[2 * m]), top = mn == -INFINITY ? 0.f : mn;
+        const float own = __builtin_amdgcn_exp2f((mrun[m] - top) * P.c2), other = __builtin_amdgcn_exp2f((ml[2 * m] - top) * P.c2);
+        mrun[m] = mn;
+        lsum[m] = lsum[m] * own + ml[2 * m + 1] * other;
+#pragma unroll
+        for (int cb = 0; cb < F::VC; cb++) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const f32x4 v = p[((m * F::VC + cb) * 4 + e) * 64];
+#pragma unroll
+            for (int x = 0; x < 4; x++) acc[m][cb][4 * e + x] = acc[m][cb][4 * e + x] * own + v[x] * other;
+          }
+          if (F::VC > 4) __builtin_amdgcn_sched_barrier(0);      // (few values at once: the accumulators fill the registers)
+        }
+      }
+    }
+  }
+  if (wave > 0 || !valid) return;
+  if (P.nsplit > 1) store_share<F::VC>(P, ((size_t)share * a.B * a.HK + bh) * R + r, h, acc, mrun, lsum);
+  else store_row<F::VC>(P, acc, mrun, lsum, b, i, head, h);
 }
 
 // Joins up to 32 shares: DV / 4 lanes per row, four columns of both maps each; a lane forms the weights of all shares for itself.  (A
@@ -1235,6 +1289,19 @@ int check_desc(const gc_diff_attention* a, bool backward) {
 }
 
 // Whether and how far the keys of a row are split.
+// Shares of a walk of `steps` blocks by `groups` workgroups: as many as give every CU one workgroup, at least 4 blocks each (forward, N
+// 1024, one head: 35 us unsplit, 20 in 4 shares of 4, 26 in 2), or two workgroups per CU where these still have `least` blocks each and
+// the registers hold two.  Two at a time walk only 1.2 times as fast as one, and their results are twice the work to add: N 4096, one
+// head forward 40 us in 16 shares of 4, 35 in 8 of 8; 8192, 4 heads 250 us unsplit, 214 in two shares.  Backward (with the forward, N
+// 3000, 8 heads): 335 us in one share, 307 in two; N 4096, one head: 142 in 16 shares of 4, 124 in 8; 4 x 1024, 8 heads: 170 in two
+// shares of 8, 146 in one.
+int64_t shares_of(const gc_diff_attention* a, int64_t groups, int64_t steps, int64_t least) {
+  if (groups <= 0) return 1;
+  const int64_t cus = device_cu_count();
+  int64_t n = std::min(cus / groups, steps / 4);
+  if (form_of(a) < 2) n = std::max(n, std::min(2 * cus / groups, steps / least));
+  return std::max<int64_t>(n, 1);
+}
 void plan_forward(const gc_diff_attention* a, DiffParams& P) {
   P.a = *a;
   P.G = a->H / a->HK;
@@ -1243,28 +1310,30 @@ void plan_forward(const gc_diff_attention* a, DiffParams& P) {
   P.div_nq = make_fastdiv((uint32_t)a->NQ);
   P.c2 = a->scale * 1.44269504088896340736f;
   P.lazy = kLazy / P.c2;
-  P.few = R <= 32 && a->NK >= 256;
+  const int form = form_of(a);
+  // Up to 32 rows: the kernel for few rows, measured beside the general one with its shares (one query, us).  64 wide: it is ahead from 256
+  // keys on (1 head 8 and 10, 64 heads x 16384 keys 53 and 73, 512 x 4096 106 and 134).  128 wide: level or ahead as long as it runs at
+  // once, on one CU per head (1 x 256 keys 11.5 and 12.5, 256 x 1024 32 and 38, 16 heads of interleaved keys x 65536 117 and 143;
+  // 512 heads x 256 30 and 21).  256 wide: only ahead in short walks (64 x 512 19 and 35, 1 x 256 17 and 21; 1 x 4096 25 and 23,
+  // 1 x 16384 40 and 32).
+  P.few = R <= 32 && a->NK >= 256 && (form == 0 || heads <= cus) && (form < 2 || a->NK <= 512);
   int64_t n = 1;
   if (P.few) {
     // one workgroup per CU (two of the narrow form, whose stages are half as large), every wave a share of at least two tiles
-    const int form = form_of(a), nw = form == 2 ? 2 : 4;
+    const int nw = form == 2 ? 2 : 4;
     const int64_t tiles32 = ((int64_t)a->NK + 31) / 32;
     n = cus * (form == 0 ? 2 : 1) / (heads > 0 ? heads : 1);
-    if (n > kMaxShares / nw) n = kMaxShares / nw;
+    if (n > kMaxShares) n = kMaxShares;
     if (n > tiles32 / 2 / nw) n = tiles32 / 2 / nw;
     if (n < 1) n = 1;
-    P.nsplit = (int)n * nw;
-    P.blocks_per_split = (int)((tiles32 + P.nsplit - 1) / P.nsplit);
+    P.nsplit = (int)n;
+    P.blocks_per_split = (int)((tiles32 + n * nw - 1) / (n * nw));
     return;
   }
-  // Fewer workgroups than CUs: the keys are split, each share at least four blocks of 64, into as many shares as give every CU one
-  // workgroup.  A second one on a CU makes the walk only 1.2 times as fast, which pays for its join in long walks alone (8192 queries
-  // and keys, 4 heads: 250 us unsplit, 216 in two shares; 2048, 16 heads: 69 and 76), and finds no registers in the widest form.
   // The join costs about three blocks' time and one more for every 28 workgroups whose rows it reads (N 1024, 4 heads, 16 blocks: 36 us
   // unsplit, 27 in 4 shares; 16 heads: 38 and 41; N 512, 8 blocks, 1 and 16 heads: 21 and 22 unsplit, 18 and 27 in two shares).
   const int64_t nblk = ((int64_t)a->NK + kBlk - 1) / kBlk, groups = heads * P.tiles;
-  n = groups > 0 ? (nblk >= 64 && form_of(a) < 2 ? 2 : 1) * cus / groups : 1;
-  if (n > nblk / 4) n = nblk / 4;
+  n = shares_of(a, groups, nblk, 8);
   if (n > 1 && nblk - nblk / n < 3 + groups * n / 28) n = 1;
   if (n > 256) n = 256;
   if (n < 1) n = 1;
@@ -1280,7 +1349,8 @@ size_t forward_bytes(const DiffParams& P, int DV) {
 }
 // The backward kernels' shares: of the keys of a query tile (dq), of the queries of a key tile (dkv).  A grid that fills the chip takes
 // one share and stores its result; otherwise the shares' fp32 partial results are added by diff_sum_kernel.  Causal key tiles differ in
-// length, so dkv wants twice as many workgroups as run at a time.
+// length: in long walks dkv takes twice as many workgroups as run at a time (8192, 16 heads on 4, forward and backward: 1653 us with as
+// many, 1446 with twice as many; 2048, where that leaves 8 blocks a share: 215 and 250).
 struct BackwardPlan {
   int dq_tiles, dq_shares, dq_blocks, dkv_tiles, dkv_shares;
   size_t delta, rows4, lampart, part;                      // floats
@@ -1290,13 +1360,12 @@ BackwardPlan plan_backward(const gc_diff_attention* a) {
   const int64_t cus = device_cu_count(), nkb = ((int64_t)a->NK + kBlk - 1) / kBlk, nqb = ((int64_t)a->NQ + kBlk - 1) / kBlk, G = a->H / a->HK;
   p.dq_tiles = (a->NQ + kRows - 1) / kRows;
   p.dkv_tiles = (a->NK + kRows - 1) / kRows;
-  int64_t n = 2 * cus / ((int64_t)a->B * a->H * p.dq_tiles);
-  if (n > nkb / 4) n = nkb / 4;
-  if (n < 4) n = 1;
+  int64_t n = shares_of(a, (int64_t)a->B * a->H * p.dq_tiles, nkb, 10);
   p.dq_blocks = (int)((nkb + n - 1) / n);
   p.dq_shares = (int)((nkb + p.dq_blocks - 1) / p.dq_blocks);
-  n = (a->causal ? 4 : 2) * cus / ((int64_t)a->B * a->HK * p.dkv_tiles);
-  if (n > G * nqb / 4) n = G * nqb / 4;
+  const int64_t groups = (int64_t)a->B * a->HK * p.dkv_tiles, steps = G * nqb;
+  n = shares_of(a, groups, steps, 10);
+  if (a->causal && n < std::min(4 * cus / groups, steps / 16)) n = std::min(4 * cus / groups, steps / 16);
   if (n > 64) n = 64;
   p.dkv_shares = n < 2 ? 1 : (int)n;
   const size_t rows = (size_t)a->B * a->H * a->NQ, keys = (size_t)a->B * a->HK * a->NK;
@@ -1322,7 +1391,7 @@ int launch_few(const DiffParams& P, hipStream_t s) {
   typedef FewCfg<DK, DV> X;
   constexpr int lds = X::NW * 2 * X::STAGE;
   if (int e = ensure_dynamic_smem(reinterpret_cast<const void*>(diff_few_rows_kernel<DK, DV>), lds)) return e;
-  hipLaunchKernelGGL((diff_few_rows_kernel<DK, DV>), dim3((unsigned)P.a.B * P.a.HK * (P.nsplit / X::NW)), dim3(X::NW * 64), lds, s, P);
+  hipLaunchKernelGGL((diff_few_rows_kernel<DK, DV>), dim3((unsigned)P.a.B * P.a.HK * P.nsplit), dim3(X::NW * 64), lds, s, P);
   return check_hip(hipGetLastError(), "diff_few_rows launch");
 }
 template <int DK, int DV>
@@ -1340,7 +1409,6 @@ int launch_sum(const float* part, int shares, void* out0, size_t n0, void* out1,
 }
 template <int DK, int DV, int OUT>
 int launch_dkv(const DiffParams& P, hipStream_t s) {
-  typedef Cfg<DK, DV> F;
   constexpr int lds = DkvCfg<DK, DV, OUT>::LDS;
   if (int e = ensure_dynamic_smem(reinterpret_cast<const void*>(diff_bwd_dkv_kernel<DK, DV, OUT>), lds)) return e;
   hipLaunchKernelGGL((diff_bwd_dkv_kernel<DK, DV, OUT>), dim3((unsigned)P.a.B * P.a.HK * P.tiles * P.nsplit), dim3(kThreads), lds, s, P);

@@ -471,6 +471,11 @@ ATTENTION_CASES = [
     (3, 260, 1030, 1, 1, 72, 136, False, (0, 1030, 70), 1.0),
     (1, 130, 2200, 2, 2, 64, 128, True, (40,), 1.0),
     (1, 40, 9000, 1, 1, 64, 128, True, None, 1.0),
+    # few rows: the widest form, one workgroup per head (its waves' shares are all there is), a workgroup whose later waves see no key
+    (1, 3, 400, 2, 1, 128, 256, False, None, 1.0),
+    (70, 1, 300, 4, 4, 32, 64, False, None, 1.0),
+    (64, 2, 260, 8, 4, 64, 128, True, None, 1.0),
+    (2, 5, 700, 2, 1, 64, 128, True, (700, 33), 1.0),
 ]
 
 
