@@ -666,34 +666,40 @@ __global__ __launch_bounds__(kThreads) void diff_join_rows_kernel(const DiffPara
   if (idx >= rows) return;
   const int c = threadIdx.x % LANES * 4, bh = (int)(idx / R), r = (int)(idx - bh * R), b = bh / a.HK, hk = bh - b * a.HK;
   const int g = (int)fd_div((uint32_t)r, P.div_nq), i = r - g * a.NQ, head = hk * P.G + g;
-  const float* ml = P.ml + idx * 4;
+  const float *ml = P.ml + idx * 4, *part = P.part + idx * 2 * DV + c;
   float top[2] = {-INFINITY, -INFINITY}, L[2] = {0.f, 0.f};
-#pragma unroll 4
-  for (int s = 0; s < P.nsplit; s++) {
-    const f32x4 v = *reinterpret_cast<const f32x4*>(ml + s * rows * 4);
+  f32x4 o[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  // eight shares at a time, all their loads under way together: latency is what this kernel is made of
+  for (int s0 = 0; s0 < P.nsplit; s0 += 8) {
+    f32x4 v[8], p[8][2];
 #pragma unroll
-    for (int m = 0; m < 2; m++) top[m] = v[2 * m + 1] != 0.f ? fmaxf(top[m], v[2 * m]) : top[m];
-  }
-  f32x4 o1 = {0.f, 0.f, 0.f, 0.f}, o2 = {0.f, 0.f, 0.f, 0.f};
-  const float* part = P.part + idx * 2 * DV + c;
-#pragma unroll 4
-  for (int s = 0; s < P.nsplit; s++) {
-    const f32x4 v = *reinterpret_cast<const f32x4*>(ml + s * rows * 4);
-    const f32x4 p1 = *reinterpret_cast<const f32x4*>(part + s * rows * 2 * DV), p2 = *reinterpret_cast<const f32x4*>(part + s * rows * 2 * DV + DV);
-    float w[2];
+    for (int x = 0; x < 8; x++) {
+      const int64_t at = (s0 + x < P.nsplit ? s0 + x : P.nsplit - 1) * rows;
+      v[x] = *reinterpret_cast<const f32x4*>(ml + at * 4);
+#pragma unroll
+      for (int m = 0; m < 2; m++) p[x][m] = *reinterpret_cast<const f32x4*>(part + (at * 2 + m) * DV);
+    }
 #pragma unroll
     for (int m = 0; m < 2; m++) {
-      // an empty share has no weight; a sum that is not a number has to reach the result
-      const float l = v[2 * m + 1];
-      w[m] = l == 0.f ? 0.f : (l != l ? l : __builtin_amdgcn_exp2f((v[2 * m] - top[m]) * P.c2));
-      L[m] += w[m] * l;
+      float now = top[m];
+#pragma unroll
+      for (int x = 0; x < 8; x++) now = v[x][2 * m + 1] != 0.f ? fmaxf(now, v[x][2 * m]) : now;
+      const float ref = now == -INFINITY ? 0.f : now, before = __builtin_amdgcn_exp2f((top[m] - ref) * P.c2);
+      top[m] = now;
+      L[m] *= before;
+      o[m] *= before;
+#pragma unroll
+      for (int x = 0; x < 8; x++) {
+        // an empty share has no weight; a sum that is not a number has to reach the result
+        const float l = v[x][2 * m + 1];
+        const float w = s0 + x >= P.nsplit || l == 0.f ? 0.f : (l != l ? l : __builtin_amdgcn_exp2f((v[x][2 * m] - ref) * P.c2));
+        L[m] += w == 0.f ? 0.f : w * l;
+        o[m] += w * p[x][m];
+      }
     }
-    o1 += w[0] * p1;
-    o2 += w[1] * p2;
   }
   const float inv0 = L[0] != 0.f ? 1.f / L[0] : 0.f, inv1 = L[1] != 0.f ? 1.f / L[1] : 0.f, lam = a.lam[head];
-  o2 *= inv1;
-  o1 = o1 * inv0 - lam * o2;
+  const f32x4 o2 = o[1] * inv1, o1 = o[0] * inv0 - lam * o2;
   if (c < a.dv) {
     const int64_t at = (((int64_t)b * a.NQ + i) * a.H + head) * a.dv + c;
     *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + at) = cvt_bf16x4(o1);
