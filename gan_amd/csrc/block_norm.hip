@@ -26,109 +26,115 @@
 namespace gc {
 namespace {
 
-constexpr int kE = 8;              // channels per thread
 constexpr int kSums = 5;
-constexpr int kMaxThreads = 1024;
+constexpr int kMaxThreads = 512, kMaxCols = 16 * kMaxThreads;
 
 enum Part { kIn = 0, kOut = 1, kBoth = 2 };
 
 struct NormParams {
   gc_block_norm a;
   int tpr;                        // threads per row (a power of two; more than 64: the workgroup)
-  int vec;                        // 16-byte loads and stores are possible
+  int width;                      // neighbouring elements per access
   int slabs;                      // workgroups per sample
   float* part;                    // backward: [batch][slabs][kSums][cols]
   float* rho_part;                // [batch][slabs], or null (no scalar residual scale asked for)
 };
 
-// A thread's 8 channels lie in 8 / W runs of W neighbours, a run of all threads of the row behind the other, so that every load
-// instruction of a wave covers one contiguous stretch: W = 8 (bf16) or 4 (fp32) for 16-byte accesses, 1 where the row length, a stride
-// or an address does not allow them.
+// A thread's E channels (8, or 16 in rows of more than 4096) lie in E / W runs of W neighbours, a run of all threads of the row behind the other, so that every load
+// instruction of a wave covers one contiguous stretch: W = 8 (bf16) or 4 (fp32) for 16-byte accesses; where the row length, a stride or
+// an address does not allow them 4 bytes, W = 2 or 1, at any address that an element may have (the memory takes unaligned ones; a row's
+// last element goes alone if the row is odd).  262144 rows of 128 bf16, forward and backward: 164 us in 16-byte, 172 in 4-byte accesses,
+// 411 element by element.
+typedef uint32_t __attribute__((aligned(2))) u32_any;
 template <int W>
 struct Lane {
   int first, step, C;
   __device__ __forceinline__ Lane(int t, int tpr, int C_) : first(t * W), step(tpr * W), C(C_) {}
   __device__ __forceinline__ int ch(int e) const { return (e / W) * step + first + e % W; }
-  __device__ __forceinline__ bool has(int e) const { return ch(e) < C; }       // (a run is there as a whole)
+  __device__ __forceinline__ bool has(int e) const { return ch(e) < C; }
 };
 
-template <typename T> struct Raw { uint32_t w[kE * sizeof(T) / 4]; };           // 8 values as stored
+template <typename T, int E> struct Raw { uint32_t w[E * sizeof(T) / 4]; };    // E values as stored
 
-template <typename T, int W>
-__device__ __forceinline__ Raw<T> load_raw(const void* base, int64_t off, const Lane<W>& L, bool live) {
-  Raw<T> r;
+template <typename T, int W, int E>
+__device__ __forceinline__ Raw<T, E> load_raw(const void* base, int64_t off, const Lane<W>& L, bool live) {
+  Raw<T, E> r;
 #pragma unroll
-  for (int i = 0; i < (int)(kE * sizeof(T) / 4); i++) r.w[i] = 0u;
+  for (int i = 0; i < (int)(E * sizeof(T) / 4); i++) r.w[i] = 0u;
   if (!live) return r;
   const T* p = static_cast<const T*>(base) + off;
   if constexpr (W > 1) {
-    constexpr int words = W * sizeof(T) / 4;                                    // 4: one 16-byte access per run
+    constexpr int words = W * sizeof(T) / 4;                                    // one access of 4 or 16 bytes per run
 #pragma unroll
-    for (int k = 0; k < kE / W; k++)
+    for (int k = 0; k < E / W; k++)
       if (L.has(k * W)) {
-        const u32x4 q = *reinterpret_cast<const u32x4*>(p + L.ch(k * W));
-#pragma unroll
-        for (int i = 0; i < words; i++) r.w[k * words + i] = q[i];
-      }
-  } else {
-#pragma unroll
-    for (int e = 0; e < kE; e++)
-      if (L.has(e)) {
-        if constexpr (sizeof(T) == 4) r.w[e] = __builtin_bit_cast(uint32_t, p[L.ch(e)]);
-        else r.w[e / 2] |= (uint32_t)p[L.ch(e)] << (16 * (e & 1));
-      }
-  }
-  return r;
-}
-template <typename T>
-__device__ __forceinline__ void widen(const Raw<T>& r, float (&v)[kE]) {
-#pragma unroll
-  for (int e = 0; e < kE; e++) {
-    if constexpr (sizeof(T) == 4) { const uint32_t u = r.w[e]; v[e] = __builtin_bit_cast(float, u); }
-    else v[e] = __builtin_bit_cast(float, (e & 1) ? (r.w[e / 2] & 0xffff0000u) : (r.w[e / 2] << 16));
-  }
-}
-template <typename T, int W>
-__device__ __forceinline__ void store_row(void* base, int64_t off, const Lane<W>& L, const float (&v)[kE]) {
-  T* p = static_cast<T*>(base) + off;
-  if constexpr (W > 1) {
-#pragma unroll
-    for (int k = 0; k < kE / W; k++)
-      if (L.has(k * W)) {
-        if constexpr (sizeof(T) == 4) {
-          *reinterpret_cast<f32x4*>(p + L.ch(k * W)) = f32x4{v[k * W], v[k * W + 1], v[k * W + 2], v[k * W + 3]};
+        if constexpr (words == 1) {
+          if (L.has(k * W + 1)) r.w[k] = *reinterpret_cast<const u32_any*>(p + L.ch(k * W));
+          else r.w[k] = p[L.ch(k * W)];
         } else {
-          const u32x2 lo = cvt_bf16x4(f32x4{v[0], v[1], v[2], v[3]}), hi = cvt_bf16x4(f32x4{v[4], v[5], v[6], v[7]});
-          *reinterpret_cast<u32x4*>(p + L.ch(0)) = u32x4{lo[0], lo[1], hi[0], hi[1]};
+          const u32x4 q = *reinterpret_cast<const u32x4*>(p + L.ch(k * W));
+#pragma unroll
+          for (int i = 0; i < words; i++) r.w[k * words + i] = q[i];
         }
       }
   } else {
 #pragma unroll
-    for (int e = 0; e < kE; e++)
-      if (L.has(e)) {
-        if constexpr (sizeof(T) == 4) p[L.ch(e)] = v[e];
-        else p[L.ch(e)] = float_to_bf16_bits(v[e]);
+    for (int e = 0; e < E; e++)
+      if (L.has(e)) r.w[e] = __builtin_bit_cast(uint32_t, p[L.ch(e)]);
+  }
+  return r;
+}
+template <typename T, int E>
+__device__ __forceinline__ void widen(const Raw<T, E>& r, float (&v)[E]) {
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    if constexpr (sizeof(T) == 4) { const uint32_t u = r.w[e]; v[e] = __builtin_bit_cast(float, u); }
+    else v[e] = __builtin_bit_cast(float, (e & 1) ? (r.w[e / 2] & 0xffff0000u) : (r.w[e / 2] << 16));
+  }
+}
+template <typename T, int W, int E>
+__device__ __forceinline__ void store_row(void* base, int64_t off, const Lane<W>& L, const float (&v)[E]) {
+  T* p = static_cast<T*>(base) + off;
+  if constexpr (W > 1) {
+#pragma unroll
+    for (int k = 0; k < E / W; k++)
+      if (L.has(k * W)) {
+        if constexpr (sizeof(T) == 4) {
+          *reinterpret_cast<f32x4*>(p + L.ch(k * W)) = f32x4{v[k * W], v[k * W + 1], v[k * W + 2], v[k * W + 3]};
+        } else if constexpr (W == 2) {
+          const uint32_t u = cvt_bf16x4(f32x4{v[2 * k], v[2 * k + 1], 0.f, 0.f})[0];
+          if (L.has(k * W + 1)) *reinterpret_cast<u32_any*>(p + L.ch(k * W)) = u;
+          else p[L.ch(k * W)] = (uint16_t)u;
+        } else {
+          const float* u = v + k * W;
+          const u32x2 lo = cvt_bf16x4(f32x4{u[0], u[1], u[2], u[3]}), hi = cvt_bf16x4(f32x4{u[4], u[5], u[6], u[7]});
+          *reinterpret_cast<u32x4*>(p + L.ch(k * W)) = u32x4{lo[0], lo[1], hi[0], hi[1]};
+        }
       }
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; e++)
+      if (L.has(e)) p[L.ch(e)] = v[e];
   }
 }
 
 // fp32 parameter: null -> `neutral`; one value per channel, or per (sample, channel)
-template <int W>
-__device__ __forceinline__ void load_param(const float* p, int per_sample, int64_t sample, const Lane<W>& L, float neutral, float (&v)[kE]) {
+template <int W, int E>
+__device__ __forceinline__ void load_param(const float* p, int per_sample, int64_t sample, const Lane<W>& L, float neutral, float (&v)[E]) {
 #pragma unroll
-  for (int e = 0; e < kE; e++) v[e] = neutral;
+  for (int e = 0; e < E; e++) v[e] = neutral;
   if (p == nullptr) return;
   p += per_sample ? sample * L.C : 0;
 #pragma unroll
-  for (int e = 0; e < kE; e++)
+  for (int e = 0; e < E; e++)
     if (L.has(e)) v[e] = p[L.ch(e)];
 }
-template <int W>
-__device__ __forceinline__ void load_rho(const gc_block_norm& a, const Lane<W>& L, float (&v)[kE]) {
-  if (a.residual_per_channel) { load_param<W>(a.residual_scale, 0, 0, L, 1.f, v); return; }
+template <int W, int E>
+__device__ __forceinline__ void load_rho(const gc_block_norm& a, const Lane<W>& L, float (&v)[E]) {
+  if (a.residual_per_channel) { load_param<W, E>(a.residual_scale, 0, 0, L, 1.f, v); return; }
   const float r = a.residual_scale != nullptr ? a.residual_scale[0] : a.residual_constant;
 #pragma unroll
-  for (int e = 0; e < kE; e++) v[e] = r;
+  for (int e = 0; e < E; e++) v[e] = r;
 }
 
 // v + the value of the lane whose number differs in one bit, in the vector unit: within 16 lanes by data-parallel-primitive moves (the
@@ -180,21 +186,21 @@ __device__ __forceinline__ void row_sum(float (&v)[N], int tpr, float* red, int&
   }
 }
 
-// mean (0 for the root-mean-square norm) and 1 / standard deviation of a row held as 8 values per thread
-template <bool WIDE, int W>
-__device__ __forceinline__ void row_stats(const float (&v)[kE], const Lane<W>& L, bool layer, float eps, int tpr, float* red, int& turn, float& mu, float& r) {
+// mean (0 for the root-mean-square norm) and 1 / standard deviation of a row held as E values per thread
+template <bool WIDE, int W, int E>
+__device__ __forceinline__ void row_stats(const float (&v)[E], const Lane<W>& L, bool layer, float eps, int tpr, float* red, int& turn, float& mu, float& r) {
   const float inv = 1.f / (float)L.C;
   mu = 0.f;
   if (layer) {
     float s[1] = {0.f};
 #pragma unroll
-    for (int e = 0; e < kE; e++) s[0] += v[e];
+    for (int e = 0; e < E; e++) s[0] += v[e];
     row_sum<WIDE, 1>(s, tpr, red, turn);
     mu = s[0] * inv;
   }
   float q[1] = {0.f};
 #pragma unroll
-  for (int e = 0; e < kE; e++) {
+  for (int e = 0; e < E; e++) {
     const float t = L.has(e) ? v[e] - mu : 0.f;
     q[0] += t * t;
   }
@@ -204,8 +210,9 @@ __device__ __forceinline__ void row_stats(const float (&v)[kE], const Lane<W>& L
 
 // The rows of a workgroup: side by side (narrow rows) and one after the other.  The next rows are asked for before the current ones are
 // worked on: the two reductions of a row leave no other work to hide the loads behind.
-// MAXT: 256 (narrow rows), or the most threads a wide row takes: 512 leave the backward pass the registers it needs, 1024 do not.
-template <typename T, int MAXT, int PART, int W>
+// MAXT: 256 (narrow rows) or the most threads a wide row takes, 512: that leaves the backward pass the registers it needs, also for 16
+// channels per thread, and 1024 threads do not (16384 rows of 2048 bf16, forward and backward: 193 against 338 us; of 8192: 1260 against 624).
+template <typename T, int MAXT, int PART, int W, int E>
 __global__ __launch_bounds__(MAXT) void block_norm_fwd_kernel(const NormParams P) {
   constexpr bool WIDE = MAXT > kThreads;
   __shared__ float red[WIDE ? 4 * (kMaxThreads / 64) : 1];
@@ -218,57 +225,57 @@ __global__ __launch_bounds__(MAXT) void block_norm_fwd_kernel(const NormParams P
   int turn = 0;
   // a thread past the last row takes part in the sums with zeros
   int64_t row = (int64_t)blockIdx.x * rpw + sub;
-  Raw<T> rx = load_raw<T, W>(a.x, sample * a.x_batch_stride + row * a.x_row_stride, L, row < a.rows), rf;
-  if (PART != kIn) rf = load_raw<T, W>(a.f, sample * a.f_batch_stride + row * a.f_row_stride, L, row < a.rows);
-  float A[kE], B[kE], Cw[kE], D[kE], rho[kE];
+  Raw<T, E> rx = load_raw<T, W, E>(a.x, sample * a.x_batch_stride + row * a.x_row_stride, L, row < a.rows), rf;
+  if (PART != kIn) rf = load_raw<T, W, E>(a.f, sample * a.f_batch_stride + row * a.f_row_stride, L, row < a.rows);
+  float A[E], B[E], Cw[E], D[E], rho[E];
   if (PART != kIn) {
-    float g[kE];
-    load_param<W>(a.gate, a.gate_per_sample, sample, L, 1.f, g);
-    load_param<W>(a.out_weight, 0, 0, L, 1.f, A);
-    load_param<W>(a.out_bias, 0, 0, L, 0.f, B);
-    load_rho<W>(a, L, rho);
+    float g[E];
+    load_param<W, E>(a.gate, a.gate_per_sample, sample, L, 1.f, g);
+    load_param<W, E>(a.out_weight, 0, 0, L, 1.f, A);
+    load_param<W, E>(a.out_bias, 0, 0, L, 0.f, B);
+    load_rho<W, E>(a, L, rho);
 #pragma unroll
-    for (int e = 0; e < kE; e++) {
+    for (int e = 0; e < E; e++) {
       A[e] *= g[e];
       B[e] *= g[e];
     }
   }
   if (PART != kOut) {
-    float s[kE], sh[kE];
-    load_param<W>(a.in_weight, 0, 0, L, 1.f, Cw);
-    load_param<W>(a.in_bias, 0, 0, L, 0.f, D);
-    load_param<W>(a.scale, a.mod_per_sample, sample, L, 0.f, s);
-    load_param<W>(a.shift, a.mod_per_sample, sample, L, 0.f, sh);
+    float s[E], sh[E];
+    load_param<W, E>(a.in_weight, 0, 0, L, 1.f, Cw);
+    load_param<W, E>(a.in_bias, 0, 0, L, 0.f, D);
+    load_param<W, E>(a.scale, a.mod_per_sample, sample, L, 0.f, s);
+    load_param<W, E>(a.shift, a.mod_per_sample, sample, L, 0.f, sh);
 #pragma unroll
-    for (int e = 0; e < kE; e++) {
+    for (int e = 0; e < E; e++) {
       Cw[e] *= 1.f + s[e];
       D[e] = D[e] * (1.f + s[e]) + sh[e];
     }
   }
   for (int64_t row0 = (int64_t)blockIdx.x * rpw; row0 < a.rows; row0 += hop, row += hop) {
     const bool live = row < a.rows;
-    float y[kE], f[kE];
-    widen<T>(rx, y);
-    if (PART != kIn) widen<T>(rf, f);
+    float y[E], f[E];
+    widen<T, E>(rx, y);
+    if (PART != kIn) widen<T, E>(rf, f);
     if (row0 + hop < a.rows) {
       const int64_t next = row + hop;
-      rx = load_raw<T, W>(a.x, sample * a.x_batch_stride + next * a.x_row_stride, L, next < a.rows);
-      if (PART != kIn) rf = load_raw<T, W>(a.f, sample * a.f_batch_stride + next * a.f_row_stride, L, next < a.rows);
+      rx = load_raw<T, W, E>(a.x, sample * a.x_batch_stride + next * a.x_row_stride, L, next < a.rows);
+      if (PART != kIn) rf = load_raw<T, W, E>(a.f, sample * a.f_batch_stride + next * a.f_row_stride, L, next < a.rows);
     }
     const int64_t out = (sample * a.rows + row) * C;
     float mu_f = 0.f, r_f = 0.f, mu_y = 0.f, r_y = 0.f;
     if (PART != kIn) {
-      row_stats<WIDE, W>(f, L, layer, a.eps, tpr, red, turn, mu_f, r_f);
+      row_stats<WIDE, W, E>(f, L, layer, a.eps, tpr, red, turn, mu_f, r_f);
 #pragma unroll
-      for (int e = 0; e < kE; e++) y[e] = L.has(e) ? rho[e] * y[e] + (A[e] * ((f[e] - mu_f) * r_f) + B[e]) : 0.f;
-      if (live) store_row<T, W>(a.y, out, L, y);
+      for (int e = 0; e < E; e++) y[e] = L.has(e) ? rho[e] * y[e] + (A[e] * ((f[e] - mu_f) * r_f) + B[e]) : 0.f;
+      if (live) store_row<T, W, E>(a.y, out, L, y);
     }
     if (PART != kOut) {
-      row_stats<WIDE, W>(y, L, layer, a.eps, tpr, red, turn, mu_y, r_y);
-      float h[kE];
+      row_stats<WIDE, W, E>(y, L, layer, a.eps, tpr, red, turn, mu_y, r_y);
+      float h[E];
 #pragma unroll
-      for (int e = 0; e < kE; e++) h[e] = Cw[e] * ((y[e] - mu_y) * r_y) + D[e];
-      if (live) store_row<T, W>(a.h, out, L, h);
+      for (int e = 0; e < E; e++) h[e] = Cw[e] * ((y[e] - mu_y) * r_y) + D[e];
+      if (live) store_row<T, W, E>(a.h, out, L, h);
     }
     if (a.stats != nullptr && t == 0 && live) {            // [4][batch * rows]: r_f, r_y, mu_f, mu_y (those the parts have)
       const int64_t i = sample * a.rows + row;
@@ -278,11 +285,11 @@ __global__ __launch_bounds__(MAXT) void block_norm_fwd_kernel(const NormParams P
   }
 }
 
-template <typename T, int MAXT, int PART, int W>
+template <typename T, int MAXT, int PART, int W, int E>
 __global__ __launch_bounds__(MAXT) void block_norm_bwd_kernel(const NormParams P) {
   constexpr bool WIDE = MAXT > kThreads;
   __shared__ float red[WIDE ? 4 * (kMaxThreads / 64) : 1];
-  __shared__ float fold[WIDE ? 1 : kThreads * kE], scalar[MAXT / 64];
+  __shared__ float fold[WIDE ? 1 : kThreads * E], scalar[MAXT / 64];
   const gc_block_norm& a = P.a;
   const int C = a.cols, tpr = P.tpr, rpw = WIDE ? 1 : kThreads / tpr;
   const int t = WIDE ? (int)threadIdx.x : (int)threadIdx.x & (tpr - 1), sub = WIDE ? 0 : (int)threadIdx.x / tpr;
@@ -291,14 +298,14 @@ __global__ __launch_bounds__(MAXT) void block_norm_bwd_kernel(const NormParams P
   const int64_t sample = blockIdx.y, nstat = a.batch * a.rows, hop = (int64_t)gridDim.x * rpw;
   const float inv = 1.f / (float)C;
   int turn = 0;
-  struct Row { Raw<T> x, f, dy, dh; float st[4]; } next;
+  struct Row { Raw<T, E> x, f, dy, dh; float st[4]; } next;
   auto ask = [&](int64_t row) {
     const bool live = row < a.rows;
     const int64_t out = (sample * a.rows + row) * C, i = sample * a.rows + row;
-    next.x = load_raw<T, W>(a.x, sample * a.x_batch_stride + row * a.x_row_stride, L, live);
-    if (PART != kIn) next.f = load_raw<T, W>(a.f, sample * a.f_batch_stride + row * a.f_row_stride, L, live);
-    if (PART != kIn) next.dy = load_raw<T, W>(a.dy, out, L, live && a.dy != nullptr);
-    if (PART != kOut) next.dh = load_raw<T, W>(a.dh, out, L, live && a.dh != nullptr);
+    next.x = load_raw<T, W, E>(a.x, sample * a.x_batch_stride + row * a.x_row_stride, L, live);
+    if (PART != kIn) next.f = load_raw<T, W, E>(a.f, sample * a.f_batch_stride + row * a.f_row_stride, L, live);
+    if (PART != kIn) next.dy = load_raw<T, W, E>(a.dy, out, L, live && a.dy != nullptr);
+    if (PART != kOut) next.dh = load_raw<T, W, E>(a.dh, out, L, live && a.dh != nullptr);
 #pragma unroll
     for (int k = 0; k < 4; k++) next.st[k] = 0.f;
     if (live) {
@@ -306,53 +313,55 @@ __global__ __launch_bounds__(MAXT) void block_norm_bwd_kernel(const NormParams P
       if (PART != kOut) { next.st[1] = a.stats[nstat + i]; if (layer) next.st[3] = a.stats[3 * nstat + i]; }
     }
   };
+  constexpr bool AHEAD = E == 8 || PART != kBoth;          // (16 channels of everything leave no registers for the next row)
   int64_t row = (int64_t)blockIdx.x * rpw + sub;
-  ask(row);
-  float A[kE], B[kE], Cw[kE], rho[kE];
+  if (AHEAD) ask(row);
+  float A[E], B[E], Cw[E], rho[E];
   if (PART != kIn) {
-    float g[kE];
-    load_param<W>(a.gate, a.gate_per_sample, sample, L, 1.f, g);
-    load_param<W>(a.out_weight, 0, 0, L, 1.f, A);
-    load_param<W>(a.out_bias, 0, 0, L, 0.f, B);
-    load_rho<W>(a, L, rho);
+    float g[E];
+    load_param<W, E>(a.gate, a.gate_per_sample, sample, L, 1.f, g);
+    load_param<W, E>(a.out_weight, 0, 0, L, 1.f, A);
+    load_param<W, E>(a.out_bias, 0, 0, L, 0.f, B);
+    load_rho<W, E>(a, L, rho);
 #pragma unroll
-    for (int e = 0; e < kE; e++) {
+    for (int e = 0; e < E; e++) {
       A[e] *= g[e];
       B[e] *= g[e];
     }
   }
   if (PART != kOut) {
-    float s[kE];
-    load_param<W>(a.in_weight, 0, 0, L, 1.f, Cw);
-    load_param<W>(a.scale, a.mod_per_sample, sample, L, 0.f, s);
+    float s[E];
+    load_param<W, E>(a.in_weight, 0, 0, L, 1.f, Cw);
+    load_param<W, E>(a.scale, a.mod_per_sample, sample, L, 0.f, s);
 #pragma unroll
-    for (int e = 0; e < kE; e++) Cw[e] *= 1.f + s[e];
+    for (int e = 0; e < E; e++) Cw[e] *= 1.f + s[e];
   }
-  float S[kSums][kE];
+  float S[kSums][E];
 #pragma unroll
   for (int k = 0; k < kSums; k++)
 #pragma unroll
-    for (int e = 0; e < kE; e++) S[k][e] = 0.f;
+    for (int e = 0; e < E; e++) S[k][e] = 0.f;
 
   for (int64_t row0 = (int64_t)blockIdx.x * rpw; row0 < a.rows; row0 += hop, row += hop) {
     const bool live = row < a.rows;
-    float x[kE], f[kE], g[kE], dh[kE];
-    widen<T>(next.x, x);
-    if (PART != kIn) { widen<T>(next.f, f); widen<T>(next.dy, g); }
+    float x[E], f[E], g[E], dh[E];
+    if (!AHEAD) ask(row);
+    widen<T, E>(next.x, x);
+    if (PART != kIn) { widen<T, E>(next.f, f); widen<T, E>(next.dy, g); }
     else
 #pragma unroll
-      for (int e = 0; e < kE; e++) g[e] = 0.f;
-    if (PART != kOut) widen<T>(next.dh, dh);
+      for (int e = 0; e < E; e++) g[e] = 0.f;
+    if (PART != kOut) widen<T, E>(next.dh, dh);
     const float r_f = next.st[0], r_y = next.st[1], mu_f = next.st[2], mu_y = next.st[3];
-    if (row0 + hop < a.rows) ask(row + hop);
+    if (AHEAD && row0 + hop < a.rows) ask(row + hop);
     const int64_t out = (sample * a.rows + row) * C;
     if (PART != kIn)
 #pragma unroll
-      for (int e = 0; e < kE; e++) f[e] = L.has(e) ? (f[e] - mu_f) * r_f : 0.f;            // fh from here on
+      for (int e = 0; e < E; e++) f[e] = L.has(e) ? (f[e] - mu_f) * r_f : 0.f;            // fh from here on
     if (PART != kOut) {
-      float yh[kE], m[2] = {0.f, 0.f};
+      float yh[E], m[2] = {0.f, 0.f};
 #pragma unroll
-      for (int e = 0; e < kE; e++) {
+      for (int e = 0; e < E; e++) {
         const float y = PART == kIn ? x[e] : rho[e] * x[e] + (A[e] * f[e] + B[e]);
         yh[e] = L.has(e) ? (y - mu_y) * r_y : 0.f;
         S[2][e] += dh[e] * yh[e];
@@ -364,14 +373,14 @@ __global__ __launch_bounds__(MAXT) void block_norm_bwd_kernel(const NormParams P
       row_sum<WIDE, 2>(m, tpr, red, turn);
       const float mq = m[0] * inv, m1 = layer ? m[1] * inv : 0.f;
 #pragma unroll
-      for (int e = 0; e < kE; e++) g[e] += r_y * (Cw[e] * dh[e] - yh[e] * mq - m1);
+      for (int e = 0; e < E; e++) g[e] += r_y * (Cw[e] * dh[e] - yh[e] * mq - m1);
     }
     if (PART == kIn) {
-      if (live) store_row<T, W>(a.dx, out, L, g);
+      if (live) store_row<T, W, E>(a.dx, out, L, g);
     } else {
-      float p[kE], m[2] = {0.f, 0.f};
+      float p[E], m[2] = {0.f, 0.f};
 #pragma unroll
-      for (int e = 0; e < kE; e++) {
+      for (int e = 0; e < E; e++) {
         if (!L.has(e)) g[e] = 0.f;
         S[0][e] += g[e] * f[e];
         S[1][e] += g[e];
@@ -381,12 +390,12 @@ __global__ __launch_bounds__(MAXT) void block_norm_bwd_kernel(const NormParams P
         m[1] += p[e];
         x[e] = rho[e] * g[e];
       }
-      if (live) store_row<T, W>(a.dx, out, L, x);
+      if (live) store_row<T, W, E>(a.dx, out, L, x);
       row_sum<WIDE, 2>(m, tpr, red, turn);
       const float mp = m[0] * inv, m1 = layer ? m[1] * inv : 0.f;
 #pragma unroll
-      for (int e = 0; e < kE; e++) p[e] = r_f * (p[e] - f[e] * mp - m1);
-      if (live) store_row<T, W>(a.df, out, L, p);
+      for (int e = 0; e < E; e++) p[e] = r_f * (p[e] - f[e] * mp - m1);
+      if (live) store_row<T, W, E>(a.df, out, L, p);
     }
   }
 
@@ -395,7 +404,7 @@ __global__ __launch_bounds__(MAXT) void block_norm_bwd_kernel(const NormParams P
   if (PART != kIn && P.rho_part != nullptr) {              // a scalar residual scale: its sum runs over the channels too
     float s = 0.f;
 #pragma unroll
-    for (int e = 0; e < kE; e++) s += S[4][e];
+    for (int e = 0; e < E; e++) s += S[4][e];
     s = lanes_sum(s, 64);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) scalar[threadIdx.x >> 6] = s;
@@ -412,9 +421,9 @@ __global__ __launch_bounds__(MAXT) void block_norm_bwd_kernel(const NormParams P
     if (!WIDE) {
       __syncthreads();
 #pragma unroll
-      for (int e = 0; e < kE; e++) fold[e * kThreads + threadIdx.x] = S[k][e];
+      for (int e = 0; e < E; e++) fold[e * kThreads + threadIdx.x] = S[k][e];
       __syncthreads();
-      for (int i = threadIdx.x; i < tpr * kE; i += kThreads) {
+      for (int i = threadIdx.x; i < tpr * E; i += kThreads) {
         const int e = i / tpr, l = i - e * tpr, c = (e / W) * (tpr * W) + l * W + e % W;
         float s = 0.f;
         for (int r = 0; r < rpw; r++) s += fold[e * kThreads + r * tpr + l];
@@ -422,7 +431,7 @@ __global__ __launch_bounds__(MAXT) void block_norm_bwd_kernel(const NormParams P
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < kE; e++)
+      for (int e = 0; e < E; e++)
         if (L.has(e)) dst[(size_t)k * C + L.ch(e)] = S[k][e];
     }
   }
@@ -579,8 +588,8 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 int check_desc(const gc_block_norm* d, bool bwd, int& parts) {
   if (d == nullptr || d->x == nullptr) { set_error("block norm: descriptor and x must not be null"); return GC_BAD_ARGUMENT; }
   if (d->dtype != GC_F32 && d->dtype != GC_BF16) { set_error("block norm: dtype must be GC_F32 or GC_BF16"); return GC_BAD_ARGUMENT; }
-  if (d->batch < 0 || d->rows < 0 || d->cols <= 0 || d->cols > kMaxThreads * kE || d->batch > 65535) {
-    set_error("block norm: 1 <= cols <= %d, 0 <= batch <= 65535, rows >= 0 are supported (got batch=%lld rows=%lld cols=%d)", kMaxThreads * kE,
+  if (d->batch < 0 || d->rows < 0 || d->cols <= 0 || d->cols > kMaxCols || d->batch > 65535) {
+    set_error("block norm: 1 <= cols <= %d, 0 <= batch <= 65535, rows >= 0 are supported (got batch=%lld rows=%lld cols=%d)", kMaxCols,
               (long long)d->batch, (long long)d->rows, d->cols);
     return GC_UNSUPPORTED_GEOMETRY;
   }
@@ -610,14 +619,14 @@ int slab_count(int64_t batch, int64_t rows, int tpr, int per_cu) {
 }
 int row_threads(int cols) {
   int tpr = 1;
-  while (tpr * kE < cols) tpr *= 2;
+  while (tpr * 8 < cols && tpr < kMaxThreads) tpr *= 2;
   return tpr;
 }
-// Workgroups of a kernel that a CU holds (asked once per kernel; 36 of them)
+// Workgroups of a kernel that a CU holds (asked once per kernel; 72 of them)
 int held_per_cu(const void* kernel, int threads) {
   struct Entry { const void* kernel; int threads, n; };
   static std::mutex mu;
-  static Entry known[64];
+  static Entry known[128];
   static int count = 0;
   std::lock_guard<std::mutex> lock(mu);
   for (int i = 0; i < count; i++)
@@ -625,7 +634,7 @@ int held_per_cu(const void* kernel, int threads) {
   int n = 0;
   if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0) != hipSuccess || n < 1) n = 2;
   if (n > kMostPerCu) n = kMostPerCu;
-  if (count < 64) known[count++] = Entry{kernel, threads, n};
+  if (count < 128) known[count++] = Entry{kernel, threads, n};
   return n;
 }
 
@@ -633,29 +642,37 @@ NormParams make_params(const gc_block_norm* d) {
   NormParams P{};
   P.a = *d;
   P.tpr = row_threads(d->cols);
-  const int unit = d->dtype == GC_F32 ? 4 : 8;             // 16 bytes
-  P.vec = d->cols % unit == 0 && d->x_row_stride % unit == 0 && d->x_batch_stride % unit == 0 && d->f_row_stride % unit == 0 &&
-          d->f_batch_stride % unit == 0 && aligned16(d->x) && aligned16(d->f) && aligned16(d->y) && aligned16(d->h) && aligned16(d->dy) &&
-          aligned16(d->dh) && aligned16(d->dx) && aligned16(d->df);
+  auto fits = [&](int unit) {                              // accesses of `unit` elements
+    const uintptr_t mask = (d->dtype == GC_F32 ? 4 : 2) * unit - 1;
+    const void* all[] = {d->x, d->f, d->y, d->h, d->dy, d->dh, d->dx, d->df};
+    for (const void* p : all)
+      if (reinterpret_cast<uintptr_t>(p) & mask) return false;
+    return d->cols % unit == 0 && d->x_row_stride % unit == 0 && d->x_batch_stride % unit == 0 && d->f_row_stride % unit == 0 && d->f_batch_stride % unit == 0;
+  };
+  P.width = d->dtype == GC_F32 ? (fits(4) ? 4 : 1) : (fits(8) ? 8 : 2);
   return P;
 }
 
 typedef void (*NormKernel)(const NormParams);
-template <typename T, int MAXT, int W>
+template <typename T, int MAXT, int W, int E>
 NormKernel kernel_for(int parts, bool bwd) {
-  if (bwd) return parts == kIn ? block_norm_bwd_kernel<T, MAXT, kIn, W> : (parts == kOut ? block_norm_bwd_kernel<T, MAXT, kOut, W> : block_norm_bwd_kernel<T, MAXT, kBoth, W>);
-  return parts == kIn ? block_norm_fwd_kernel<T, MAXT, kIn, W> : (parts == kOut ? block_norm_fwd_kernel<T, MAXT, kOut, W> : block_norm_fwd_kernel<T, MAXT, kBoth, W>);
+  if (bwd)
+    return parts == kIn ? block_norm_bwd_kernel<T, MAXT, kIn, W, E>
+                        : (parts == kOut ? block_norm_bwd_kernel<T, MAXT, kOut, W, E> : block_norm_bwd_kernel<T, MAXT, kBoth, W, E>);
+  return parts == kIn ? block_norm_fwd_kernel<T, MAXT, kIn, W, E>
+                      : (parts == kOut ? block_norm_fwd_kernel<T, MAXT, kOut, W, E> : block_norm_fwd_kernel<T, MAXT, kBoth, W, E>);
 }
 template <typename T, int W>
-NormKernel kernel_width(int tpr, int parts, bool bwd) {
-  if (tpr <= 64) return kernel_for<T, kThreads, W>(parts, bwd);
-  return tpr <= 512 ? kernel_for<T, 512, W>(parts, bwd) : kernel_for<T, kMaxThreads, W>(parts, bwd);
+NormKernel kernel_width(int cols, int tpr, int parts, bool bwd) {
+  if (tpr <= 64) return kernel_for<T, kThreads, W, 8>(parts, bwd);
+  return cols <= 8 * kMaxThreads ? kernel_for<T, kMaxThreads, W, 8>(parts, bwd) : kernel_for<T, kMaxThreads, W, 16>(parts, bwd);
 }
 // Launches the kernel for P (whose slabs it sets)
 int launch(NormParams& P, int parts, bool bwd, hipStream_t s) {
   NormKernel k;
-  if (P.a.dtype == GC_F32) k = P.vec ? kernel_width<float, 4>(P.tpr, parts, bwd) : kernel_width<float, 1>(P.tpr, parts, bwd);
-  else k = P.vec ? kernel_width<uint16_t, 8>(P.tpr, parts, bwd) : kernel_width<uint16_t, 1>(P.tpr, parts, bwd);
+  const int C = P.a.cols;
+  if (P.a.dtype == GC_F32) k = P.width == 4 ? kernel_width<float, 4>(C, P.tpr, parts, bwd) : kernel_width<float, 1>(C, P.tpr, parts, bwd);
+  else k = P.width == 8 ? kernel_width<uint16_t, 8>(C, P.tpr, parts, bwd) : kernel_width<uint16_t, 2>(C, P.tpr, parts, bwd);
   const int threads = P.tpr > 64 ? P.tpr : kThreads;
   P.slabs = slab_count(P.a.batch, P.a.rows, P.tpr, held_per_cu(reinterpret_cast<const void*>(k), threads));
   hipLaunchKernelGGL(k, dim3(P.slabs, (unsigned)P.a.batch), dim3(threads), 0, s, P);
