@@ -1356,7 +1356,8 @@ size_t forward_bytes(const DiffParams& P, int DV) {
 // The backward kernels' shares: of the keys of a query tile (dq), of the queries of a key tile (dkv).  A grid that fills the chip takes
 // one share and stores its result; otherwise the shares' fp32 partial results are added by diff_sum_kernel.  Causal key tiles differ in
 // length: in long walks dkv takes twice as many workgroups as run at a time (8192, 16 heads on 4, forward and backward: 1653 us with as
-// many, 1446 with twice as many; 2048, where that leaves 8 blocks a share: 215 and 250).
+// many, 1446 with twice as many; 2048, where that leaves 8 blocks a share: 215 and 250), and 6 blocks are enough for a share where the grid
+// has room (6 x 777, 6 heads on 2 of 32/64: 32 us in 3 shares, 23 in 6).
 struct BackwardPlan {
   int dq_tiles, dq_shares, dq_blocks, dkv_tiles, dkv_shares;
   size_t delta, rows4, lampart, part;                      // floats
@@ -1370,7 +1371,7 @@ BackwardPlan plan_backward(const gc_diff_attention* a) {
   p.dq_blocks = (int)((nkb + n - 1) / n);
   p.dq_shares = (int)((nkb + p.dq_blocks - 1) / p.dq_blocks);
   const int64_t groups = (int64_t)a->B * a->HK * p.dkv_tiles, steps = G * nqb;
-  n = shares_of(a, groups, steps, 10);
+  n = shares_of(a, groups, steps, a->causal && 4 * groups <= 3 * cus ? 6 : 10);
   if (a->causal && n < std::min(4 * cus / groups, steps / 16)) n = std::min(4 * cus / groups, steps / 16);
   if (n > 64) n = 64;
   p.dkv_shares = n < 2 ? 1 : (int)n;
