@@ -3,7 +3,7 @@ several axes, differential attention.  Extensions beside the reference's one att
 in rows, an image [B, C, H, W] in channels-last memory being [B, H * W, C].
 
 Unlike the convolutions these are plain autograd functions, not torch.library operators, and their descriptors are packed in one go:
-a call on a single token is host time and little else (norm 35 -> 20 us, one query of attention 34 -> 25 us).  First-order
+a call on a single token is host time and little else (a norm 35 -> 18 us, one query of attention 34 -> 19 us).  First-order
 gradients only.  There is no fallback: on a CPU tensor or an unsupported geometry they raise RuntimeError.
 """
 import contextlib
