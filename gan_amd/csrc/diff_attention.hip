@@ -127,6 +127,11 @@ __device__ __forceinline__ u32x4s buffer_at(const void* p, uint32_t bytes) {
                 (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
 }
 
+template <int N>
+__device__ __forceinline__ void wait_loads() {             // all but the N youngest loads of this wave have landed
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+}
+
 // One tile of ROWS rows of `width` elements (padded to ROWB / 2 columns), from a tensor with row stride `stride` bytes.
 template <int ROWB, Use U, int ROWS = kBlk, int NW = kThreads / 64>
 struct Loader {
@@ -157,6 +162,42 @@ struct Loader {
 #pragma unroll
       for (int b = 0; b < BASES; b++) load_to_lds16(rs, voff[b], lds + (wave + NW * (n + b)) * 1024);
     }
+  }
+};
+// The same for tiles of kBlk rows that follow each other, fetched piece by piece in few scalar instructions: one descriptor, moved on by
+// a tile, and an offset register for every piece.
+template <int ROWB, Use U, int NW>
+struct TileStream {
+  static constexpr int CPR = ROWB / 16, RPI = 64 / CPR, NI = kBlk * ROWB / (1024 * NW);
+  static_assert(NI >= 1, "every wave loads a part of a tile");
+  uint32_t voff[NI], stride, full, last, bytes;            // bytes of a whole tile, of a row, of what is there of this tile
+  const char* p;
+  int left;
+  __device__ __forceinline__ void init(int wave, int lane, const char* first, int rows, uint32_t stride_, int width) {
+    stride = stride_;
+    last = width * 2;
+    full = (kBlk - 1) * stride + last;
+    p = first;
+    left = rows;
+    measure();
+#pragma unroll
+    for (int n = 0; n < NI; n++) {
+      const int row = (wave + NW * n) * RPI + lane / CPR, chunk = (lane % CPR) ^ swz<ROWB, U>(row);
+      voff[n] = chunk * 8 < width ? (uint32_t)row * stride + chunk * 16 : kOutOfRange;
+    }
+  }
+  // piece n of the tile to LDS at `lds`; rows that do not exist (possibly all) are answered with zeros
+  __device__ __forceinline__ void piece(int n, int wave, uint32_t lds) const {
+    load_to_lds16(buffer_at(p, bytes), voff[n], lds + (wave + NW * n) * 1024);
+  }
+  __device__ __forceinline__ void next() {
+    p += kBlk * stride;
+    left -= kBlk;
+    measure();
+  }
+  __device__ __forceinline__ void measure() {
+    bytes = full;
+    if (left < kBlk) bytes = left > 0 ? (uint32_t)(left - 1) * stride + last : 0u;
   }
 };
 // Keys and values of one key head, staged tile after tile: running (scalar) addresses instead of products per tile.
@@ -220,6 +261,20 @@ __device__ __forceinline__ bf16x8 read_col_both(uint32_t lo_addr) { return read_
 __device__ __forceinline__ bf16x8 global_frag(const uint16_t* row, bool valid, int col, int width) {
   if (!valid || col >= width) return zero8();
   return __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(row + col));
+}
+
+// Makes the compiler have operands ready here.  Otherwise it waits for them where they are first used, in every round of a loop,
+// and for all loads, among them those into LDS that are meant to stay in flight.
+template <int M, int N>
+__device__ __forceinline__ void arrived(bf16x8 (&v)[M][N]) {
+#pragma unroll
+  for (int m = 0; m < M; m++)
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+      u32x4 u = __builtin_bit_cast(u32x4, v[m][n]);
+      asm volatile("" : "+v"(u));
+      v[m][n] = __builtin_bit_cast(bf16x8, u);
+    }
 }
 
 __device__ __forceinline__ int sample_length(const gc_diff_attention& a, int b) {
@@ -324,6 +379,41 @@ __device__ __forceinline__ void store_share(const DiffParams& P, size_t row, int
       for (int e = 0; e < 4; e++)
         *reinterpret_cast<f32x4*>(P.part + (row * 2 + m) * (VC * 32) + cb * 32 + 8 * e + 4 * h) =
             f32x4{acc[m][cb][4 * e], acc[m][cb][4 * e + 1], acc[m][cb][4 * e + 2], acc[m][cb][4 * e + 3]};
+}
+
+// The same between the waves of a workgroup, through LDS (p: this lane's first of kShareItems rows of 64 items)
+template <int VC> constexpr int kShareItems = 8 * VC + 1;
+template <int VC>
+__device__ __forceinline__ void lend_share(f32x4* p, const f32x16 (&acc)[2][VC], const float (&mrun)[2], const float (&lsum)[2]) {
+#pragma unroll
+  for (int m = 0; m < 2; m++)
+#pragma unroll
+    for (int cb = 0; cb < VC; cb++)
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        p[((m * VC + cb) * 4 + e) * 64] = f32x4{acc[m][cb][4 * e], acc[m][cb][4 * e + 1], acc[m][cb][4 * e + 2], acc[m][cb][4 * e + 3]};
+  p[8 * VC * 64] = f32x4{mrun[0], lsum[0], mrun[1], lsum[1]};
+}
+template <int VC>
+__device__ __forceinline__ void take_share(const f32x4* p, f32x16 (&acc)[2][VC], float (&mrun)[2], float (&lsum)[2], float c2) {
+  const f32x4 ml = p[8 * VC * 64];
+#pragma unroll
+  for (int m = 0; m < 2; m++) {
+    const float mn = fmaxf(mrun[m], ml[2 * m]), top = mn == -INFINITY ? 0.f : mn;
+    const float own = __builtin_amdgcn_exp2f((mrun[m] - top) * c2), other = __builtin_amdgcn_exp2f((ml[2 * m] - top) * c2);
+    mrun[m] = mn;
+    lsum[m] = lsum[m] * own + ml[2 * m + 1] * other;
+#pragma unroll
+    for (int cb = 0; cb < VC; cb++) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const f32x4 v = p[((m * VC + cb) * 4 + e) * 64];
+#pragma unroll
+        for (int x = 0; x < 4; x++) acc[m][cb][4 * e + x] = acc[m][cb][4 * e + x] * own + v[x] * other;
+      }
+      if (VC > 4) __builtin_amdgcn_sched_barrier(0);       // (few values at once: the accumulators fill the registers)
+    }
+  }
 }
 
 // A finished row: out = O1 - lam O2, and for a backward pass O2 and the log2-sums
@@ -506,6 +596,226 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_fwd_kerne
   store_row<F::VC>(P, acc, mrun, lsum, b, i, head, h);
 }
 
+// The forms whose registers hold two waves per SIMD: 8 waves, of which four and four take turns on the matrix units.  Two waves of a SIMD
+// left alone fall into step, and the matrix unit waits while both form exponentials: its share of the cycles and the vector unit's added
+// up to the whole.  Here waves 0-3 work on the first 32 keys of every tile, waves 4-7 on the second, for the same 128 rows, and a barrier
+// after every phase keeps one half multiplying (a block's probabilities with its values, then the next block's scores) while the other
+// half forms exponentials; the multiplying waves go first where both could issue.  The two shares are joined at the end.  Tiles go through
+// a ring of five: two are in use, the others have landed or are on their way.  N 4096, batch 32, one head of 64/128: 436 us with two
+// independent workgroups of 4 waves per CU, 411 so (752 TFLOP/s, matrix unit busy 55 % of the cycles at the 1.84 GHz that power leaves);
+// N 4096, 8 heads of one sample, where every CU has one workgroup: 126 and 97; 2048, 16 heads: 68 and 55.
+template <int DK, int DV>
+struct TurnsCfg {
+  static constexpr int NW = 8, KB = kBlk * DK * 2, VB = kBlk * DV * 2, STAGE = 2 * KB + VB, LOADS = STAGE / 1024 / NW;
+  static constexpr int RING = 5 * STAGE;
+  static constexpr int SHARES = 4 * 64 * 16 * kShareItems<DV / 32>, LDS = RING > SHARES ? RING : SHARES;
+};
+template <int DK, int DV>
+__global__ __launch_bounds__(512, 2) void diff_fwd_turns_kernel(const DiffParams P) {
+  typedef Cfg<DK, DV> F;
+  typedef TurnsCfg<DK, DV> X;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const gc_diff_attention& a = P.a;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), late = wave >> 2, h = lane >> 5;
+  const WorkId id = work_id(P, (uint32_t)a.B * a.HK, (uint32_t)P.G);
+  const int split = id.share, tile = id.tile, bh = id.bh, b = bh / a.HK, hk = bh - b * a.HK;
+  const int R = P.G * a.NQ, len = sample_length(a, b);
+  const int r0 = tile * kRows, w0 = r0 + (wave & 3) * 32, r = w0 + (lane & 31);
+  const bool valid = r < R;
+  const int rc = valid ? r : R - 1, g = (int)fd_div((uint32_t)rc, P.div_nq), i = rc - g * a.NQ, head = hk * P.G + g;
+  const int lim = visible(a, i, len);
+  // most and fewest visible keys of this wave's rows, most of the workgroup's
+  int kend = len, wmin = len, wmax = len;
+  if (a.causal) {
+    const int e = (r0 + kRows < R ? r0 + kRows : R) - 1, ge = (int)fd_div((uint32_t)e, P.div_nq), gs = (int)fd_div((uint32_t)r0, P.div_nq);
+    kend = gs == ge ? visible(a, e - ge * a.NQ, len) : len;
+    const int first = w0 < R ? w0 : R - 1, last = w0 + 31 < R ? w0 + 31 : R - 1;
+    const int gf = (int)fd_div((uint32_t)first, P.div_nq), gl = (int)fd_div((uint32_t)last, P.div_nq);
+    wmin = gf == gl ? visible(a, first - gf * a.NQ, len) : visible(a, 0, len);
+    wmax = gf == gl ? visible(a, last - gl * a.NQ, len) : len;
+  }
+  wmin = __builtin_amdgcn_readfirstlane(wmin);
+  wmax = __builtin_amdgcn_readfirstlane(wmax);
+
+  const uint16_t* qrow = static_cast<const uint16_t*>(a.q) + b * a.q_stride[0] + i * a.q_stride[1] + head * a.q_stride[2];
+  bf16x8 qf[2][F::KS];
+#pragma unroll
+  for (int m = 0; m < 2; m++)
+#pragma unroll
+    for (int ks = 0; ks < F::KS; ks++) qf[m][ks] = global_frag(qrow + m * a.q_stride[3], valid, ks * 16 + 8 * h, a.d);
+
+  f32x16 acc[2][F::VC];
+  float mrun[2] = {-INFINITY, -INFINITY}, lsum[2] = {0.f, 0.f}, base[2] = {0.f, 0.f};
+  bool careful = true;                                     // (of the whole wave) no maximum yet, or scores too large for the short way
+#pragma unroll
+  for (int m = 0; m < 2; m++)
+#pragma unroll
+    for (int cb = 0; cb < F::VC; cb++) acc[m][cb] = zero16();
+
+  const uint32_t base0 = lds_offset(smem);
+  const uint32_t kaddr = base0 + late * 32 * F::KROW + row_addr<F::KROW, kRowWise>(lane);
+  const uint32_t vaddr = base0 + 2 * F::KB + late * 32 * F::VROW + col_addr<F::VROW, kTransposed>(lane, 0);
+  const int nblk = (kend + kBlk - 1) / kBlk;
+  const int blk0 = split * P.blocks_per_split, T = max(0, min(nblk, blk0 + P.blocks_per_split) - blk0);
+  // a wave fetches rows of one map of the keys and of the values; behind the last row: loads of no rows, which read nothing
+  TileStream<F::KROW, kRowWise, 4> tk;
+  TileStream<F::VROW, kTransposed, 8> tv;
+  const uint32_t kst = (uint32_t)(a.k_stride[1] * 2), vst = (uint32_t)(a.v_stride[1] * 2);
+  const int first = blk0 * kBlk;
+  tk.init(wave & 3, lane, reinterpret_cast<const char*>(static_cast<const uint16_t*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[2] + late * a.k_stride[3]) + first * (int64_t)kst,
+          len - first, kst, a.d);
+  tv.init(wave, lane, reinterpret_cast<const char*>(static_cast<const uint16_t*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[2]) + first * (int64_t)vst, len - first, vst, a.dv);
+  auto after = [](uint32_t st) { return st + X::STAGE == X::RING ? 0u : st + X::STAGE; };
+  uint32_t ask = 0;
+  constexpr int PIECES = tk.NI + tv.NI;
+  auto fetch = [&](int n) {                                // pieces of the next tile, in order
+    if (n < tk.NI) tk.piece(n < tk.NI ? n : 0, wave & 3, base0 + ask + late * F::KB);
+    else if (n < PIECES) tv.piece(n < PIECES && n >= tk.NI ? n - tk.NI : 0, wave, base0 + ask + 2 * F::KB);
+    if (n == PIECES - 1) {
+      ask = after(ask);
+      tk.next();
+      tv.next();
+    }
+  };
+  auto turn = [&]() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  float sum[2];
+  auto exponentials = [&](f32x16 (&s)[2]) {
+#pragma unroll
+    for (int m = 0; m < 2; m++) {
+      sum[m] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 16; e++) {
+        s[m][e] = __builtin_amdgcn_exp2f(s[m][e] * P.c2 - base[m]);
+        sum[m] += s[m][e];
+      }
+    }
+  };
+
+  auto scores = [&](f32x16 (&s)[2], const bf16x8 (&k)[2], int ks) {
+#pragma unroll
+    for (int m = 0; m < 2; m++) s[m] = mfma(k[m], qf[m][ks], ks == 0 ? zero16() : s[m]);
+  };
+  auto keys = [&](bf16x8 (&k)[2], uint32_t ka, int ks) {
+#pragma unroll
+    for (int m = 0; m < 2; m++) k[m] = read_row((ka ^ (ks << 5)) + m * F::KB);
+  };
+  auto value = [&](bf16x8& v, uint32_t va, int n) {
+    const uint32_t x = (va ^ ((n % F::VC) << 6)) + (n / F::VC) * 16 * F::VROW;
+    v = read_col(x, x + 8 * F::VROW);
+  };
+  arrived(qf);
+#pragma unroll
+  for (int x = 0; x < 4; x++)
+#pragma unroll
+    for (int n = 0; n < PIECES; n++) fetch(n);
+  wait_loads<3 * X::LOADS>();
+  turn();
+  if (late) turn();
+  f32x16 s[2];
+  {
+    bf16x8 k[F::KS][2];
+#pragma unroll
+    for (int ks = 0; ks < F::KS; ks++) keys(k[ks], kaddr, ks);
+#pragma unroll
+    for (int ks = 0; ks < F::KS; ks++) scores(s, k[ks], ks);
+  }
+  wait_loads<2 * X::LOADS>();
+  turn();
+  // In every round everyone asks for the tile four on; letting the youngest two stay in flight puts the tile that the other half reads
+  // in two phases in place.
+  const int own = min(T, max(0, (wmax - blk0 * kBlk - late * 32 + kBlk - 1) / kBlk));      // rounds in which this wave sees keys
+  uint32_t here = 0;                                       // stage of this round's tile
+  int t = 0;
+  for (; t < own; t++) {
+    const int j0 = (blk0 + t) * kBlk + late * 32;
+    if (j0 + 32 > wmin) hide(s, lim - j0 - 4 * h);
+    // Exponentials against the maxima so far, without looking for new ones: the sum of a lane's 16 exponentials, wanted anyway,
+    // tells whether one of them passed 2^8 (it is then above 2^8 ... 2^12, or infinite).  Then, and while a row has no maximum
+    // yet, the scores are formed again and take the careful way.
+    bool again = careful;
+    if (!again) {
+      exponentials(s);
+      again = __builtin_amdgcn_ballot_w64(fmaxf(sum[0], sum[1]) > 16.f * kLazyExp) != 0;
+    }
+    if (again) {
+      if (!careful) {
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+#pragma unroll
+          for (int ks = 0; ks < F::KS; ks++) {
+            s[m] = mfma(read_row(((kaddr + here) ^ (ks << 5)) + m * F::KB), qf[m][ks], ks == 0 ? zero16() : s[m]);
+            __builtin_amdgcn_sched_barrier(0);             // (one operand at a time: rare, and the registers are taken)
+          }
+        if (j0 + 32 > wmin) hide(s, lim - j0 - 4 * h);
+      }
+      softmax_step<F::VC>(s, acc, mrun, lsum, base, P.c2, P.lazy);
+      exponentials(s);
+      careful = __builtin_amdgcn_ballot_w64(mrun[0] == -INFINITY || mrun[1] == -INFINITY ||
+                                            fmaxf(fabsf(mrun[0]), fabsf(mrun[1])) * P.c2 > kLargeScore) != 0;
+    }
+      bf16x8 pb[2][2];
+#pragma unroll
+    for (int m = 0; m < 2; m++) {
+      lsum[m] += sum[m];
+      pb[m][0] = pack8(s[m], 0);
+      pb[m][1] = pack8(s[m], 8);
+    }
+    // This block's products, then the next block's scores (of whatever lies there behind the last block: nobody looks at them), two matrix
+    // instructions at a time.  An operand is read from LDS three of these steps before its turn, the first ones in this phase already;
+    // the loads are asked for in between.
+    constexpr int NV = 2 * F::VC, AHEAD = 3;
+    const uint32_t va = vaddr + here, ka = kaddr + after(here);
+    bf16x8 v[NV], k[F::KS][2];
+#pragma unroll
+    for (int n = 0; n < AHEAD; n++) value(v[n], va, n);
+    arrived(pb);                                           // (and not put off into the other phase)
+    turn();
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int q = 0; q < NV + F::KS; q++) {
+      if (q < NV) {
+        acc[0][q % F::VC] = mfma(v[q], pb[0][q / F::VC], acc[0][q % F::VC]);
+        acc[1][q % F::VC] = mfma(v[q], pb[1][q / F::VC], acc[1][q % F::VC]);
+      } else {
+        scores(s, k[q - NV], q - NV);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (q + AHEAD < NV) value(v[q + AHEAD < NV ? q + AHEAD : 0], va, q + AHEAD);
+      else if (q + AHEAD < NV + F::KS) keys(k[q + AHEAD < NV + F::KS ? q + AHEAD - NV : 0], ka, q + AHEAD - NV);
+      if (q & 1) fetch(q / 2);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_s_setprio(0);
+    wait_loads<2 * X::LOADS>();
+    turn();
+    here = after(here);
+  }
+  for (; t < T; t++) {
+    turn();
+#pragma unroll
+    for (int n = 0; n < PIECES; n++) fetch(n);
+    wait_loads<2 * X::LOADS>();
+    turn();
+  }
+  if (!late) turn();
+
+  wait_loads<0>();                                         // (nothing is still writing LDS)
+  lsum[0] = half_sum(lsum[0]);
+  lsum[1] = half_sum(lsum[1]);
+  f32x4* const lds = reinterpret_cast<f32x4*>(smem) + (wave & 3) * kShareItems<F::VC> * 64 + lane;
+  __syncthreads();
+  if (late) lend_share<F::VC>(lds, acc, mrun, lsum);
+  __syncthreads();
+  if (late || !valid) return;
+  take_share<F::VC>(lds, acc, mrun, lsum, P.c2);
+  if (P.nsplit > 1) store_share<F::VC>(P, ((size_t)split * a.B * a.HK + bh) * R + r, h, acc, mrun, lsum);
+  else store_row<F::VC>(P, acc, mrun, lsum, b, i, head, h);
+}
+
 // At most 32 rows per key head (single queries and short runs of them against long keys): bound by reading the keys and values once.
 // Every wave walks a share of the keys of its own in tiles of 32, staged privately (no barriers; the loads of the next tile are in
 // flight while one is worked on), so that a CU keeps 64 KiB of loads under way; the waves' shares become one in LDS (4 x 65536 keys, 16
@@ -518,10 +828,6 @@ struct FewCfg {
   static constexpr int NW = DV > 128 ? 2 : 4;              // waves
   static constexpr int KB = 32 * DK * 2, VB = 32 * DV * 2, STAGE = 2 * KB + VB, LOADS = STAGE / 1024;
 };
-template <int N>
-__device__ __forceinline__ void wait_loads() {             // all but the N youngest loads of this wave have landed
-  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
-}
 __device__ __forceinline__ bf16x8 pack8_rest(const f32x16& v, int r0, bf16x8 hi) {
   const u32x4 b = __builtin_bit_cast(u32x4, hi);
   f32x16 d;
@@ -563,6 +869,7 @@ __global__ __launch_bounds__((FewCfg<DK, DV>::NW * 64), 1) void diff_few_rows_ke
   const int t0 = (share * X::NW + wave) * P.blocks_per_split, t1 = min((wmax + 31) / 32, t0 + P.blocks_per_split);
   KeyTiles<F::KROW, F::VROW, kRowWise, kTransposed, 32, 1> tiles;
   tiles.init(a, b, hk, t0 * 32, len, 0, lane);
+  arrived(qf);
   if (t0 < t1) tiles.next(base0);
   for (int t = t0; t < t1; t++) {
     // (behind the last tile: loads of no rows, which read nothing; the count of loads in flight stays the same)
@@ -610,44 +917,13 @@ __global__ __launch_bounds__((FewCfg<DK, DV>::NW * 64), 1) void diff_few_rows_ke
   lsum[0] = half_sum(lsum[0]);
   lsum[1] = half_sum(lsum[1]);
   // The waves' shares become one, by halves, through the LDS that held the tiles
-  f32x4* const half = reinterpret_cast<f32x4*>(smem) + lane;
-  constexpr int ITEMS = 8 * F::VC + 1;
+  f32x4* const lds = reinterpret_cast<f32x4*>(smem) + lane;
 #pragma unroll
   for (int n = X::NW / 2; n > 0; n /= 2) {
     __syncthreads();
-    if (wave >= n && wave < 2 * n && valid) {
-      f32x4* p = half + (wave - n) * ITEMS * 64;
-#pragma unroll
-      for (int m = 0; m < 2; m++)
-#pragma unroll
-        for (int cb = 0; cb < F::VC; cb++)
-#pragma unroll
-          for (int e = 0; e < 4; e++)
-            p[((m * F::VC + cb) * 4 + e) * 64] = f32x4{acc[m][cb][4 * e], acc[m][cb][4 * e + 1], acc[m][cb][4 * e + 2], acc[m][cb][4 * e + 3]};
-      p[8 * F::VC * 64] = f32x4{mrun[0], lsum[0], mrun[1], lsum[1]};
-    }
+    if (wave >= n && wave < 2 * n && valid) lend_share<F::VC>(lds + (wave - n) * kShareItems<F::VC> * 64, acc, mrun, lsum);
     __syncthreads();
-    if (wave < n && valid) {
-      const f32x4* p = half + wave * ITEMS * 64;
-      const f32x4 ml = p[8 * F::VC * 64];
-#pragma unroll
-      for (int m = 0; m < 2; m++) {
-        const float mn = fmaxf(mrun[m], ml[2 * m]), top = mn == -INFINITY ? 0.f : mn;
-        const float own = __builtin_amdgcn_exp2f((mrun[m] - top) * P.c2), other = __builtin_amdgcn_exp2f((ml[2 * m] - top) * P.c2);
-        mrun[m] = mn;
-        lsum[m] = lsum[m] * own + ml[2 * m + 1] * other;
-#pragma unroll
-        for (int cb = 0; cb < F::VC; cb++) {
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const f32x4 v = p[((m * F::VC + cb) * 4 + e) * 64];
-#pragma unroll
-            for (int x = 0; x < 4; x++) acc[m][cb][4 * e + x] = acc[m][cb][4 * e + x] * own + v[x] * other;
-          }
-          if (F::VC > 4) __builtin_amdgcn_sched_barrier(0);      // (few values at once: the accumulators fill the registers)
-        }
-      }
-    }
+    if (wave < n && valid) take_share<F::VC>(lds + wave * kShareItems<F::VC> * 64, acc, mrun, lsum, P.c2);
   }
   if (wave > 0 || !valid) return;
   if (P.nsplit > 1) store_share<F::VC>(P, ((size_t)share * a.B * a.HK + bh) * R + r, h, acc, mrun, lsum);
@@ -1295,12 +1571,10 @@ int check_desc(const gc_diff_attention* a, bool backward) {
 }
 
 // Whether and how far the keys of a row are split.
-// Shares of a walk of `steps` blocks by `groups` workgroups: as many as give every CU one workgroup, at least 4 blocks each (forward, N
-// 1024, one head: 35 us unsplit, 20 in 4 shares of 4, 26 in 2), or two workgroups per CU where these still have `least` blocks each and
-// the registers hold two.  Two at a time walk only 1.2 times as fast as one, and their results are twice the work to add: N 4096, one
-// head forward 40 us in 16 shares of 4, 35 in 8 of 8; 8192, 4 heads 250 us unsplit, 214 in two shares.  Backward (with the forward, N
-// 3000, 8 heads): 335 us in one share, 307 in two; N 4096, one head: 142 in 16 shares of 4, 124 in 8; 4 x 1024, 8 heads: 170 in two
-// shares of 8, 146 in one.
+// Shares of a backward walk of `steps` blocks by `groups` workgroups: as many as give every CU one workgroup, at least 4 blocks each, or two
+// workgroups per CU where these still have `least` blocks each and the registers hold two.  Two at a time walk only 1.2 times as fast as
+// one, and their results are twice the work to add.  With the forward pass, us: N 3000, 8 heads 335 in one share, 307 in two; N 4096, one
+// head 142 in 16 shares of 4, 124 in 8; 4 x 1024, 8 heads 170 in two shares of 8, 146 in one.
 int64_t shares_of(const gc_diff_attention* a, int64_t groups, int64_t steps, int64_t least) {
   if (groups <= 0) return 1;
   const int64_t cus = device_cu_count();
@@ -1336,11 +1610,12 @@ void plan_forward(const gc_diff_attention* a, DiffParams& P) {
     P.blocks_per_split = (int)((tiles32 + n * nw - 1) / (n * nw));
     return;
   }
-  // The join costs about three blocks' time and one more for every 28 workgroups whose rows it reads (N 1024, 4 heads, 16 blocks: 36 us
-  // unsplit, 27 in 4 shares; 16 heads: 38 and 41; N 512, 8 blocks, 1 and 16 heads: 21 and 22 unsplit, 18 and 27 in two shares).
+  // As many shares as give every CU one workgroup, where that saves more blocks of a walk than the join costs: about 5 blocks' time and
+  // one more for every 15 workgroups whose rows it reads, in the widest form, whose blocks take three times as long, 3 and one for 28
+  // (64/128: N 4096, one head 68 us unsplit, 34 in 8 shares; 4 heads 77 and 67 in two; N 1024, 8 heads 27 and 36 in 4; 128/256: 61, 46).
   const int64_t nblk = ((int64_t)a->NK + kBlk - 1) / kBlk, groups = heads * P.tiles;
-  n = shares_of(a, groups, nblk, 8);
-  if (n > 1 && nblk - nblk / n < 3 + groups * n / 28) n = 1;
+  n = groups > 0 ? std::min(cus / groups, nblk / 4) : 1;
+  if (n > 1 && nblk - nblk / n < (form < 2 ? 5 + groups * n / 15 : 3 + groups * n / 28)) n = 1;
   if (n > 256) n = 256;
   if (n < 1) n = 1;
   P.blocks_per_split = (int)((nblk + n - 1) / n);
@@ -1391,6 +1666,13 @@ int launch_fwd(const DiffParams& P, hipStream_t s) {
   constexpr int lds = 2 * (2 * F::KB + F::VB);
   if (int e = ensure_dynamic_smem(reinterpret_cast<const void*>(diff_fwd_kernel<DK, DV>), lds)) return e;
   hipLaunchKernelGGL((diff_fwd_kernel<DK, DV>), dim3((unsigned)P.a.B * P.a.HK * P.tiles * P.nsplit), dim3(kThreads), lds, s, P);
+  return check_hip(hipGetLastError(), "diff_fwd launch");
+}
+template <int DK, int DV>
+int launch_turns(const DiffParams& P, hipStream_t s) {
+  typedef TurnsCfg<DK, DV> X;
+  if (int e = ensure_dynamic_smem(reinterpret_cast<const void*>(diff_fwd_turns_kernel<DK, DV>), X::LDS)) return e;
+  hipLaunchKernelGGL((diff_fwd_turns_kernel<DK, DV>), dim3((unsigned)P.a.B * P.a.HK * P.tiles * P.nsplit), dim3(X::NW * 64), X::LDS, s, P);
   return check_hip(hipGetLastError(), "diff_fwd launch");
 }
 template <int DK, int DV>
@@ -1454,7 +1736,7 @@ extern "C" int gc_diff_attention_fwd(const gc_diff_attention* desc, void* worksp
     ProfScope ps(P.few ? "gc::diff_few_rows_kernel" : "gc::diff_fwd_kernel", 4.0 * desc->B * desc->H * (double)desc->NQ * desc->NK * (desc->d + desc->dv), s);
     int e;
     if (P.few) e = form == 0 ? launch_few<32, 64>(P, s) : (form == 1 ? launch_few<64, 128>(P, s) : launch_few<128, 256>(P, s));
-    else e = form == 0 ? launch_fwd<32, 64>(P, s) : (form == 1 ? launch_fwd<64, 128>(P, s) : launch_fwd<128, 256>(P, s));
+    else e = form == 0 ? launch_turns<32, 64>(P, s) : (form == 1 ? launch_turns<64, 128>(P, s) : launch_fwd<128, 256>(P, s));
     if (e) return e;
   }
   if (P.nsplit > 1) {
