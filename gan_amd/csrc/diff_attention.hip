@@ -1290,6 +1290,221 @@ __global__ __launch_bounds__(kThreads) void diff_sum_kernel(const float* part, i
   *reinterpret_cast<u32x2*>(out + i) = cvt_bf16x4(t);
 }
 
+// The dQ kernel with the halves of a workgroup taking turns, as in the forward kernel: in one phase a block's dQ products, the next block's
+// scores and its dP, in the other the exponentials and score gradients between them.  Three matrix instructions at a time, so that the one
+// chain that dP is does not wait for itself.  For grids of up to a workgroup per CU, which it fills with two waves per SIMD (dQ and the rest
+// of both passes, N 2048, 16 heads on 4: 259 us with the kernel above, 247 with this one; 1500, 16 heads 173 and 163; 4 x 1024, 8 heads,
+// causal 133 and 127).  Larger grids it does no good (batch 32, N 4096: 442 and 459 us), small ones that are split further neither (1024,
+// 4 heads: 85 and 87).
+template <int DK, int DV>
+__global__ __launch_bounds__(512, 2) void diff_bwd_dq_turns_kernel(const DiffParams P) {
+  typedef Cfg<DK, DV> F;
+  typedef TurnsCfg<DK, DV> X;
+  static_assert(2 * F::KC + F::KS == F::VS, "dP's steps go beside the others");
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const gc_diff_attention& a = P.a;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), late = wave >> 2, h = lane >> 5;
+  const WorkId id = work_id(P, (uint32_t)a.B * a.H, 1);
+  const int share = id.share, tile = id.tile, bh = id.bh, b = bh / a.H, head = bh - b * a.H, hk = head / P.G;
+  const int len = sample_length(a, b), r0 = tile * kRows, w0 = r0 + (wave & 3) * 32, r = w0 + (lane & 31);
+  const bool valid = r < a.NQ;
+  const int i = valid ? r : a.NQ - 1, lim = visible(a, i, len);
+  const int kend = visible(a, min(r0 + kRows, a.NQ) - 1, len);
+  const int wmin = __builtin_amdgcn_readfirstlane(visible(a, min(w0, a.NQ - 1), len));
+  const int wmax = __builtin_amdgcn_readfirstlane(visible(a, min(w0 + 31, a.NQ - 1), len));
+
+  const uint16_t* qrow = static_cast<const uint16_t*>(a.q) + b * a.q_stride[0] + i * a.q_stride[1] + head * a.q_stride[2];
+  const uint16_t* grow = static_cast<const uint16_t*>(a.dout) + (((size_t)b * a.NQ + i) * a.H + head) * a.dv;
+  bf16x8 qf[2][F::KS], gf[1][F::VS];
+#pragma unroll
+  for (int m = 0; m < 2; m++)
+#pragma unroll
+    for (int ks = 0; ks < F::KS; ks++) qf[m][ks] = global_frag(qrow + m * a.q_stride[3], valid, ks * 16 + 8 * h, a.d);
+#pragma unroll
+  for (int ks = 0; ks < F::VS; ks++) gf[0][ks] = global_frag(grow, valid, ks * 16 + 8 * h, a.dv);
+  // (every other row's dP with its sign turned, as in the kernel above)
+  const float turned = (r & 1) ? -1.f : 1.f;
+  if (r & 1)
+#pragma unroll
+    for (int ks = 0; ks < F::VS; ks++) gf[0][ks] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, gf[0][ks]) ^ 0x80008000u);
+  float L[2], D[2];
+#pragma unroll
+  for (int m = 0; m < 2; m++) {
+    const size_t o = ((size_t)(b * a.H + head) * 2 + m) * a.NQ + i;
+    L[m] = a.lse[o];
+    D[m] = P.delta[o];
+  }
+  asm volatile("" : "+v"(L[0]), "+v"(L[1]), "+v"(D[0]), "+v"(D[1]));      // (as arrived() does)
+  arrived(qf);
+  arrived(gf);
+
+  f32x16 acc[2][F::KC];
+#pragma unroll
+  for (int m = 0; m < 2; m++)
+#pragma unroll
+    for (int cb = 0; cb < F::KC; cb++) acc[m][cb] = zero16();
+  float left = 0.f;                                        // sum_j p2 (dP - delta2), its sign turned in odd rows
+  const float gap = turned * (D[0] - D[1]);
+  f32x16 start;
+#pragma unroll
+  for (int e = 0; e < 16; e++) start[e] = -turned * D[0];
+
+  const uint32_t base0 = lds_offset(smem);
+  const uint32_t kra = base0 + late * 32 * F::KROW + row_addr<F::KROW, kBothWays>(lane);
+  const uint32_t kca = base0 + late * 32 * F::KROW + col_addr<F::KROW, kBothWays>(lane, 0);
+  const uint32_t vra = base0 + 2 * F::KB + late * 32 * F::VROW + row_addr<F::VROW, kRowWise>(lane);
+  const int blk0 = share * P.blocks_per_split, T = max(0, min((kend + kBlk - 1) / kBlk, blk0 + P.blocks_per_split) - blk0);
+  TileStream<F::KROW, kBothWays, 4> tk;
+  TileStream<F::VROW, kRowWise, 8> tv;
+  const uint32_t kst = (uint32_t)(a.k_stride[1] * 2), vst = (uint32_t)(a.v_stride[1] * 2);
+  const int first = blk0 * kBlk;
+  tk.init(wave & 3, lane, reinterpret_cast<const char*>(static_cast<const uint16_t*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[2] + late * a.k_stride[3]) + first * (int64_t)kst,
+          len - first, kst, a.d);
+  tv.init(wave, lane, reinterpret_cast<const char*>(static_cast<const uint16_t*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[2]) + first * (int64_t)vst, len - first, vst, a.dv);
+  auto after = [](uint32_t st) { return st + X::STAGE == X::RING ? 0u : st + X::STAGE; };
+  uint32_t ask = 0;
+  constexpr int PIECES = tk.NI + tv.NI;
+  auto fetch = [&](int n) {                                // pieces of the next tile, in order
+    if (n < tk.NI) tk.piece(n < tk.NI ? n : 0, wave & 3, base0 + ask + late * F::KB);
+    else if (n < PIECES) tv.piece(n < PIECES && n >= tk.NI ? n - tk.NI : 0, wave, base0 + ask + 2 * F::KB);
+    if (n == PIECES - 1) {
+      ask = after(ask);
+      tk.next();
+      tv.next();
+    }
+  };
+  auto turn = [&]() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // operands of step n: 2 KC steps of dQ (half a block, a column block), then KS of the scores; one of dP's beside each
+  struct Operands { bf16x8 k[2], v; };
+  auto operands = [&](Operands& o, uint32_t here, uint32_t next, int n) {
+#pragma unroll
+    for (int m = 0; m < 2; m++)
+      o.k[m] = n < 2 * F::KC ? read_col_both<F::KROW>(((kca + here) ^ ((n % F::KC) << 6)) + m * F::KB + (n / F::KC) * 16 * F::KROW)
+                             : read_row(((kra + next) ^ ((n - 2 * F::KC) << 5)) + m * F::KB);
+    o.v = read_row((vra + next) ^ (n << 5));
+  };
+
+#pragma unroll
+  for (int x = 0; x < 4; x++)
+#pragma unroll
+    for (int n = 0; n < PIECES; n++) fetch(n);
+  wait_loads<2 * X::LOADS>();
+  turn();
+  if (late) turn();
+  f32x16 s[2], dp = start;                                 // dP - delta1
+#pragma unroll
+  for (int n = 0; n < F::VS; n++) {
+    Operands o;
+    operands(o, 0, 0, n);
+    if (n >= 2 * F::KC)
+#pragma unroll
+      for (int m = 0; m < 2; m++) s[m] = mfma(o.k[m], qf[m][n < 2 * F::KC ? 0 : n - 2 * F::KC], n == 2 * F::KC ? zero16() : s[m]);
+    dp = mfma(o.v, gf[0][n], dp);
+  }
+  wait_loads<X::LOADS>();
+  turn();
+  // In every round everyone asks for the tile four on; letting only this youngest one stay in flight puts the tile whose first operands
+  // the other half reads in the next phase in place.
+  const int own = min(T, max(0, (wmax - blk0 * kBlk - late * 32 + kBlk - 1) / kBlk));      // rounds in which this wave sees keys
+  uint32_t here = 0;                                       // stage of this round's tile
+  int t = 0;
+  for (; t < own; t++) {
+    const int j0 = (blk0 + t) * kBlk + late * 32;
+    if (j0 + 32 > wmin) hide(s, lim - j0 - 4 * h);
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+      s[0][e] = __builtin_amdgcn_exp2f(s[0][e] * P.c2 - L[0]) * dp[e];
+      s[1][e] = __builtin_amdgcn_exp2f(s[1][e] * P.c2 - L[1]) * (dp[e] + gap);
+      left += s[1][e];
+    }
+    bf16x8 d[2][2];
+#pragma unroll
+    for (int m = 0; m < 2; m++) {
+      d[m][0] = pack8(s[m], 0);
+      d[m][1] = pack8(s[m], 8);
+    }
+    constexpr int AHEAD = 2;
+    const uint32_t next = after(here);
+    Operands o[F::VS];
+#pragma unroll
+    for (int n = 0; n < AHEAD; n++) operands(o[n], here, next, n);
+    arrived(d);                                            // (and not put off into the other phase)
+    turn();
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int n = 0; n < F::VS; n++) {
+      if (n < 2 * F::KC) {
+#pragma unroll
+        for (int m = 0; m < 2; m++) acc[m][n % F::KC] = mfma(o[n].k[m], d[m][n / F::KC], acc[m][n % F::KC]);
+      } else {
+#pragma unroll
+        for (int m = 0; m < 2; m++) s[m] = mfma(o[n].k[m], qf[m][n - 2 * F::KC], n == 2 * F::KC ? zero16() : s[m]);
+      }
+      dp = mfma(o[n].v, gf[0][n], n == 0 ? start : dp);
+      __builtin_amdgcn_sched_barrier(0);
+      if (n + AHEAD < F::VS) operands(o[n + AHEAD < F::VS ? n + AHEAD : 0], here, next, n + AHEAD);
+      if (n >= 2) fetch(n - 2);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_s_setprio(0);
+    wait_loads<X::LOADS>();
+    turn();
+    here = next;
+  }
+  for (; t < T; t++) {
+    turn();
+#pragma unroll
+    for (int n = 0; n < PIECES; n++) fetch(n);
+    wait_loads<X::LOADS>();
+    turn();
+  }
+  if (!late) turn();
+
+  wait_loads<0>();                                         // (nothing is still writing LDS)
+  __syncthreads();
+  f32x4* const lent = reinterpret_cast<f32x4*>(smem) + (wave & 3) * (8 * F::KC) * 64 + lane;
+  float* const red = reinterpret_cast<float*>(smem + 4 * 8 * F::KC * 64 * 16);
+  if (late)
+#pragma unroll
+    for (int x = 0; x < 8 * F::KC; x++) {
+      const f32x16& v = acc[x / (4 * F::KC)][x / 4 % F::KC];
+      lent[x * 64] = f32x4{v[4 * (x % 4)], v[4 * (x % 4) + 1], v[4 * (x % 4) + 2], v[4 * (x % 4) + 3]};
+    }
+  float tl = valid ? turned * left + (h == 0 && share == 0 && !late ? D[1] : 0.f) : 0.f;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) tl += __shfl_xor(tl, o, 64);
+  if (lane == 0) red[wave] = tl;
+  __syncthreads();
+  if (tid == 0) {
+    float sum = red[0];
+    for (int w = 1; w < 8; w++) sum += red[w];
+    P.lampart[((size_t)bh * P.tiles + tile) * P.nsplit + share] = sum;
+  }
+  if (late || !valid) return;
+  const float lam = a.lam[head], f[2] = {turned * a.scale, -turned * lam * a.scale};
+  const size_t row = (((size_t)b * a.NQ + i) * a.H + head) * 2 * a.d;
+  uint16_t* dst = static_cast<uint16_t*>(a.dq) + row;
+  float* part = P.part + (size_t)share * a.B * a.NQ * a.H * 2 * a.d + row;
+#pragma unroll
+  for (int m = 0; m < 2; m++)
+#pragma unroll
+    for (int cb = 0; cb < F::KC; cb++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const int c = cb * 32 + 8 * e + 4 * h;
+        if (c >= a.d) continue;
+        f32x4 v = lent[((m * F::KC + cb) * 4 + e) * 64];
+#pragma unroll
+        for (int x = 0; x < 4; x++) v[x] = (acc[m][cb][4 * e + x] + v[x]) * f[m];
+        if (P.nsplit > 1) *reinterpret_cast<f32x4*>(part + m * a.d + c) = v;
+        else *reinterpret_cast<u32x2*>(dst + m * a.d + c) = cvt_bf16x4(v);
+      }
+}
+
 // Owner: 128 keys of a key head; walks the queries of every head that shares them.  Produces dK and dV.  OUT: 1 dK, 2 dV, 3 both
 // (both accumulators of the widest form do not fit the register file: it runs as two launches).  VLDS: the owned values, an operand of
 // dP, stay in LDS instead of registers, and the queries are staged 32 rows at a time to make room: with 64 keys' worth of accumulators
@@ -1634,7 +1849,7 @@ size_t forward_bytes(const DiffParams& P, int DV) {
 // many, 1446 with twice as many; 2048, where that leaves 8 blocks a share: 215 and 250), and 6 blocks are enough for a share where the grid
 // has room (6 x 777, 6 heads on 2 of 32/64: 32 us in 3 shares, 23 in 6).
 struct BackwardPlan {
-  int dq_tiles, dq_shares, dq_blocks, dkv_tiles, dkv_shares;
+  int dq_tiles, dq_shares, dq_blocks, dq_turns, dkv_tiles, dkv_shares;
   size_t delta, rows4, lampart, part;                      // floats
 };
 BackwardPlan plan_backward(const gc_diff_attention* a) {
@@ -1642,7 +1857,9 @@ BackwardPlan plan_backward(const gc_diff_attention* a) {
   const int64_t cus = device_cu_count(), nkb = ((int64_t)a->NK + kBlk - 1) / kBlk, nqb = ((int64_t)a->NQ + kBlk - 1) / kBlk, G = a->H / a->HK;
   p.dq_tiles = (a->NQ + kRows - 1) / kRows;
   p.dkv_tiles = (a->NK + kRows - 1) / kRows;
-  int64_t n = shares_of(a, (int64_t)a->B * a->H * p.dq_tiles, nkb, 10);
+  const int64_t dq_groups = (int64_t)a->B * a->H * p.dq_tiles;
+  p.dq_turns = form_of(a) < 2 && dq_groups <= cus && 4 * dq_groups > cus;
+  int64_t n = p.dq_turns ? std::max<int64_t>(1, std::min(cus / dq_groups, nkb / 4)) : shares_of(a, dq_groups, nkb, 10);
   p.dq_blocks = (int)((nkb + n - 1) / n);
   p.dq_shares = (int)((nkb + p.dq_blocks - 1) / p.dq_blocks);
   const int64_t groups = (int64_t)a->B * a->HK * p.dkv_tiles, steps = G * nqb;
@@ -1695,6 +1912,13 @@ int launch_sum(const float* part, int shares, void* out0, size_t n0, void* out1,
   hipLaunchKernelGGL(diff_sum_kernel, dim3((unsigned)(((n0 + n1) / 4 + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, part, shares, (uint16_t*)out0, n0,
                      (uint16_t*)out1, n1);
   return check_hip(hipGetLastError(), "diff_sum launch");
+}
+template <int DK, int DV>
+int launch_dq_turns(const DiffParams& P, hipStream_t s) {
+  typedef TurnsCfg<DK, DV> X;
+  if (int e = ensure_dynamic_smem(reinterpret_cast<const void*>(diff_bwd_dq_turns_kernel<DK, DV>), X::RING)) return e;
+  hipLaunchKernelGGL((diff_bwd_dq_turns_kernel<DK, DV>), dim3((unsigned)P.a.B * P.a.H * P.tiles * P.nsplit), dim3(X::NW * 64), X::RING, s, P);
+  return check_hip(hipGetLastError(), "diff_bwd_dq launch");
 }
 template <int DK, int DV, int OUT>
 int launch_dkv(const DiffParams& P, hipStream_t s) {
@@ -1789,7 +2013,9 @@ extern "C" int gc_diff_attention_bwd(const gc_diff_attention* desc, void* worksp
   P.blocks_per_split = plan.dq_blocks;
   {
     ProfScope ps("gc::diff_bwd_dq_kernel", pairs * (8.0 * desc->d + 2.0 * desc->dv), s);
-    const int e = form == 0 ? launch_dq<32, 64>(P, s) : (form == 1 ? launch_dq<64, 128>(P, s) : launch_dq<128, 256>(P, s));
+    int e;
+    if (plan.dq_turns) e = form == 0 ? launch_dq_turns<32, 64>(P, s) : launch_dq_turns<64, 128>(P, s);
+    else e = form == 0 ? launch_dq<32, 64>(P, s) : (form == 1 ? launch_dq<64, 128>(P, s) : launch_dq<128, 256>(P, s));
     if (e) return e;
   }
   if (P.nsplit > 1)

@@ -476,6 +476,11 @@ ATTENTION_CASES = [
     (70, 1, 300, 4, 4, 32, 64, False, None, 1.0),
     (64, 2, 260, 8, 4, 64, 128, True, None, 1.0),
     (2, 5, 700, 2, 1, 64, 128, True, (700, 33), 1.0),
+    # grids of a quarter to one workgroup per CU in the backward pass: one share, several, shares without a visible key, odd widths
+    (5, 200, 300, 8, 4, 64, 128, True, (300, 0, 1, 33, 170), 1.0),
+    (9, 130, 700, 4, 2, 32, 64, False, (700, 31, 32, 33, 64, 65, 0, 1, 640), 1.0),
+    (3, 90, 90, 24, 24, 40, 80, True, None, 2.0),
+    (3, 129, 1100, 12, 3, 64, 128, True, (1100, 500, 64), 1.0),
 ]
 
 
