@@ -1806,12 +1806,11 @@ void plan_forward(const gc_diff_attention* a, DiffParams& P) {
   P.c2 = a->scale * 1.44269504088896340736f;
   P.lazy = kLazy / P.c2;
   const int form = form_of(a);
-  // Up to 32 rows: the kernel for few rows, measured beside the general one with its shares (one query, us).  64 wide: it is ahead from 256
-  // keys on (1 head 8 and 10, 64 heads x 16384 keys 53 and 73, 512 x 4096 106 and 134).  128 wide: level or ahead as long as it runs at
-  // once, on one CU per head (1 x 256 keys 11.5 and 12.5, 256 x 1024 32 and 38, 16 heads of interleaved keys x 65536 117 and 143;
-  // 512 heads x 256 30 and 21).  256 wide: only ahead in short walks (64 x 512 19 and 35, 1 x 256 17 and 21; 1 x 4096 25 and 23,
-  // 1 x 16384 40 and 32).
-  P.few = R <= 32 && a->NK >= 256 && (form == 0 || heads <= cus) && (form < 2 || a->NK <= 512);
+  // Up to 32 rows: the kernel for few rows, measured beside the general one with its shares (one query, us).  64 wide it is ahead from 64
+  // keys on (1 head x 256 keys 8 and 10, 512 x 64 10 and 13, 64 x 16384 52 and 69), 128 wide ahead or level (1 x 256 12 and 13, 64 x 1024
+  // 18 and 26, 512 x 256 29 and 33, 64 x 4096 32 and 31, 16 heads of interleaved keys x 65536 110 and 121), 256 wide ahead in walks of 256
+  // to 512 keys that run at once (64 x 512 20 and 35, 1 x 256 17 and 22; 1 x 128 19 and 16, 1 x 16384 40 and 32, 512 x 256 53 and 48).
+  P.few = R <= 32 && (form < 2 ? a->NK >= 64 : a->NK >= 256 && a->NK <= 512 && heads <= cus);
   int64_t n = 1;
   if (P.few) {
     // one workgroup per CU (two of the narrow form, whose stages are half as large), every wave a share of at least two tiles
