@@ -18,7 +18,8 @@
 // written once.  Rows of up to 512 channels belong to 2^k lanes of one wave (sums by lane exchange, no LDS); wider rows to a
 // workgroup.  A thread keeps its channels for all its rows, so the parameters are read once per workgroup and the sums S
 // live in registers; they leave as one partial row per workgroup and are added in a fixed order (no atomics).  Statistics
-// and sums are fp32; y enters the second norm before it is rounded to its storage type.
+// and sums are fp32; y enters the second norm before it is rounded to its storage type.  64 x 4096 rows of 128 bf16, both parts: forward
+// 61 us, backward 92 (4.4 TB/s both; a large copy reaches 4.9) and 11 for the parameters; 16384 rows of 4096 forward 113 (4.7 TB/s).
 #include <mutex>
 
 #include "common.h"

@@ -10,7 +10,8 @@
 // out cos and sin of their P pairs once into LDS and then streams all heads (and, where the samples share positions, several
 // samples) of those tokens with 16-byte accesses.  An angle is formed in turns (w / 2 pi per unit of position, fp64), its
 // whole turns dropped in fp64, and only the fraction is rounded to fp32: a position of a million in the fastest pair would
-// otherwise lose 17 of 24 bits.
+// otherwise lose 17 of 24 bits.  64 x 4096 tokens, 8 heads of 32 fp32: 114 us (4.7 TB/s; a large copy reaches 4.9), of bf16 44; 2 x 16384
+// tokens, 40 heads of 128 bf16, positions of their own: 141 (4.75 TB/s).  Element by element, where 16-byte accesses do not fit: 159 and 62.
 #include "common.h"
 
 namespace gc {
