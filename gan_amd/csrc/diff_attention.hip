@@ -115,10 +115,10 @@ __device__ __forceinline__ void tile_ready() {
 // data; tile_ready() waits for the loads.
 typedef uint32_t u32x4s __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void load_to_lds16(u32x4s rsrc, uint32_t voff, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "memory", "m0");
 }
 __device__ __forceinline__ void load_to_lds4(u32x4s rsrc, uint32_t voff, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "memory", "m0");
 }
 // Raw buffer of `bytes` bytes at p (uniform): loads at or past its end return zeros
 __device__ __forceinline__ u32x4s buffer_at(const void* p, uint32_t bytes) {
@@ -725,10 +725,10 @@ __global__ __launch_bounds__(512, 2) void diff_fwd_turns_kernel(const DiffParams
   }
   wait_loads<2 * X::LOADS>();
   turn();
-  // In every round everyone asks for the tile four on; letting the youngest two stay in flight puts the tile that the other half reads
+  // In every step everyone asks for the tile four on; letting the youngest two stay in flight puts the tile that the other half reads
   // in two phases in place.
-  const int own = min(T, max(0, (wmax - blk0 * kBlk - late * 32 + kBlk - 1) / kBlk));      // rounds in which this wave sees keys
-  uint32_t here = 0;                                       // stage of this round's tile
+  const int own = min(T, max(0, (wmax - blk0 * kBlk - late * 32 + kBlk - 1) / kBlk));      // steps in which this wave sees keys
+  uint32_t here = 0;                                       // stage of this step's tile
   int t = 0;
   for (; t < own; t++) {
     const int j0 = (blk0 + t) * kBlk + late * 32;
@@ -1204,12 +1204,14 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dq_ke
       // the exponentials (N 4096, batch 32: 476 against 438 us; in the forward kernel the same gained nothing, 433 against 437)
       __builtin_amdgcn_s_setprio(0);
       if (j0 + 32 > wmin) hide(s, lim - j0 - 4 * h);
+      float here_left = 0.f;                               // (16 of its addends at a time: fewer roundings at its full size)
 #pragma unroll
       for (int e = 0; e < 16; e++) {
         s[0][e] = __builtin_amdgcn_exp2f(s[0][e] * P.c2 - L[0]) * dp[e];
         s[1][e] = __builtin_amdgcn_exp2f(s[1][e] * P.c2 - L[1]) * (dp[e] + gap);
-        left += s[1][e];
+        here_left += s[1][e];
       }
+      left += here_left;
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int t = 0; t < 2; t++) {
@@ -1257,10 +1259,10 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dq_ke
 
 // dlam[head] = -(the workgroups' shares, added in a fixed order); one workgroup per head
 __global__ __launch_bounds__(kThreads) void diff_dlam_kernel(const DiffParams P) {
-  __shared__ float red[kThreads];
+  __shared__ double red[kThreads];
   const int head = blockIdx.x;
   const int64_t per = (int64_t)P.tiles * P.nsplit, n = P.a.B * per;
-  float s = 0.f;
+  double s = 0.0;                                          // (sums of either sign, of which little may be left)
   for (int64_t i = threadIdx.x; i < n; i += kThreads) {
     const int64_t b = i / per, t = i - b * per;
     s += P.lampart[(b * P.a.H + head) * per + t];
@@ -1268,9 +1270,9 @@ __global__ __launch_bounds__(kThreads) void diff_dlam_kernel(const DiffParams P)
   red[threadIdx.x] = s;
   __syncthreads();
   if (threadIdx.x == 0) {
-    float t = 0.f;
+    double t = 0.0;
     for (int i = 0; i < kThreads; i++) t += red[i];
-    P.a.dlam[head] = -t;
+    P.a.dlam[head] = (float)-t;
   }
 }
 
@@ -1409,20 +1411,22 @@ __global__ __launch_bounds__(512, 2) void diff_bwd_dq_turns_kernel(const DiffPar
   }
   wait_loads<X::LOADS>();
   turn();
-  // In every round everyone asks for the tile four on; letting only this youngest one stay in flight puts the tile whose first operands
+  // In every step everyone asks for the tile four on; letting only this youngest one stay in flight puts the tile whose first operands
   // the other half reads in the next phase in place.
-  const int own = min(T, max(0, (wmax - blk0 * kBlk - late * 32 + kBlk - 1) / kBlk));      // rounds in which this wave sees keys
-  uint32_t here = 0;                                       // stage of this round's tile
+  const int own = min(T, max(0, (wmax - blk0 * kBlk - late * 32 + kBlk - 1) / kBlk));      // steps in which this wave sees keys
+  uint32_t here = 0;                                       // stage of this step's tile
   int t = 0;
   for (; t < own; t++) {
     const int j0 = (blk0 + t) * kBlk + late * 32;
     if (j0 + 32 > wmin) hide(s, lim - j0 - 4 * h);
+    float here_left = 0.f;                                 // (16 of its addends at a time: fewer roundings at its full size)
 #pragma unroll
     for (int e = 0; e < 16; e++) {
       s[0][e] = __builtin_amdgcn_exp2f(s[0][e] * P.c2 - L[0]) * dp[e];
       s[1][e] = __builtin_amdgcn_exp2f(s[1][e] * P.c2 - L[1]) * (dp[e] + gap);
-      left += s[1][e];
+      here_left += s[1][e];
     }
+    left += here_left;
     bf16x8 d[2][2];
 #pragma unroll
     for (int m = 0; m < 2; m++) {
