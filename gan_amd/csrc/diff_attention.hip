@@ -1575,6 +1575,7 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dkv_k
   // the staged queries: running (scalar) addresses, set anew for every head of the group
   const char *q0 = nullptr, *q1 = nullptr, *go = nullptr;
   const float* four = nullptr;
+  float weight = 0.f;
   int left = 0;
   auto seek = [&](int g, int blk) {
     const int head = hk * P.G + g;
@@ -1584,6 +1585,7 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dkv_k
     go = reinterpret_cast<const char*>(static_cast<const uint16_t*>(a.dout) + ((size_t)b * a.NQ * a.H + head) * a.dv) + row * gst;
     four = P.rows4 + ((size_t)(b * a.H + head) * 4 + wave) * a.NQ + row;
     left = a.NQ - (int)row;
+    weight = a.lam[head];
   };
   auto fetch = [&](uint32_t st) {
     lq.load(q0, left, qst, a.d, st);
@@ -1609,8 +1611,8 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_bwd_dkv_k
     fetch(base0);
   }
   for (int step = step0; step < step1; step++) {
-    const float sgn = a.lam[hk * P.G + g] > 0.f ? -1.f : 1.f;      // (asked for in front of the next step's loads, which it would wait for)
-    tile_ready();
+    tile_ready();                                          // (and a new head's weight with it)
+    const float sgn = weight > 0.f ? -1.f : 1.f;
     const int i_blk = blk * ROWS;
     const bool more = step + 1 < step1;
     if (++blk == nblk) {
