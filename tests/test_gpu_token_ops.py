@@ -608,6 +608,35 @@ def test_differential_attention_gradients_against_differences(F):
     assert abs(diff - along) < 2.0 ** -7 * float(gq.double().norm()) * 4 + 1e-6 * abs(diff), (diff, along)
 
 
+def test_differential_attention_of_a_cache_past_32_bits(F):
+    """Keys and values of more than 4 GiB each: all but the last key are zeros, the last one's score in the first map (128 above the others')
+    leaves e^-128 x 2^21 to them, the second map is uniform, so the result is the last value (and 2^-21 of it), rounded once, and the last
+    value's gradient the sum of the incoming ones."""
+    NK, H, d, dv = (1 << 21) + 70, 8, 64, 128
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GiB")
+    k = torch.zeros(1, NK, H, 2, d, dtype=torch.bfloat16, device="cuda")
+    v = torch.zeros(1, NK, H, dv, dtype=torch.bfloat16, device="cuda")
+    assert k.numel() * 2 > 1 << 32 and v.numel() * 2 > 1 << 32
+    g = torch.Generator(device="cuda").manual_seed(8)
+    last = torch.randn(H, dv, generator=g, device="cuda").bfloat16()
+    k[0, -1, :, 0], v[0, -1] = 4.0, last
+    k.requires_grad_(True), v.requires_grad_(True)
+    lam = torch.full((H,), 0.5, device="cuda")
+    for NQ in (1, 40):                                     # the kernel for few rows, and the general one
+        q = torch.full((1, NQ, H, 2, d), 4.0, dtype=torch.bfloat16, device="cuda")
+        out = F.differential_attention(q, k, v, lam)
+        assert float((out[0].float() - last.float()).abs().max()) <= 2.0 ** -8 * float(last.float().abs().max())
+        dout = torch.randn(out.shape, generator=g, device="cuda").bfloat16()
+        gk, gv = torch.autograd.grad(out, (k, v), dout)
+        want = dout[0].double().sum(0)
+        # each addend's probability and the sum are rounded to bf16
+        assert bool(((gv[0, -1].double() - want).abs() <= 2.0 ** -8 * (want.abs() + dout[0].double().abs().sum(0)) + 1e-6).all())
+        assert float(gv[0, :-1].abs().max()) <= 2.0 ** -20 * float(dout.float().abs().sum(1).max())
+        assert bool(torch.isfinite(gk[0, -64:]).all()) and float(gk[0, :64].abs().max()) <= 1e-3
+        del out, gk, gv
+
+
 def test_differential_attention_weight_gradient_of_many_rows(F):
     """dlam is one sum over 131072 rows of either sign: a rounding that always goes one way would add up.  A row's term, dO . O2, is a
     difference of sums of fp32 values no larger than S = |delta1| + |delta2| + sum_j p2 |dP|, each step of them off by half of 2^-23 of S
