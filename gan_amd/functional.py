@@ -250,7 +250,7 @@ def differential_attention(q, k, v, lam, *, scale=None, causal=False, key_length
     [B, NK, HK, 2, d] (index 3: the two maps), v [B, NK, HK, dv], bf16; lam: [H], fp32 or bf16.  Returns [B, NQ, H, dv].  d: a multiple
     of 8 up to 128, dv: up to 256; H a multiple of HK (head h reads keys h // (H // HK)).  scale: d ** -0.5 by default, positive.
     key_lengths [B] (integers, clamped to 0 .. NK): keys from there on are not read at all.  causal: query i sees keys
-    j <= i + length - NQ, i.e. the queries are the last NQ positions of a sample; values at keys hidden this way must be finite.
+    j <= i + length - NQ, i.e. the queries are the last NQ positions of a sample; values (and, for the gradients, keys) hidden this way must be finite.
     A query without a visible key gives zeros and sends no gradient.  Single queries against long keys are split over the
     keys.  Deterministic; first-order gradients for q, k, v and lam."""
     return token_ops.differential_attention(q, k, v, lam, scale, causal, key_lengths)

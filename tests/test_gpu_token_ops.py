@@ -577,6 +577,28 @@ def test_differential_attention_never_reads_behind_a_length(F):
     _check("mean", out[0, 0, 0], vv[0, :, 0].double().mean(0), 2.0 ** -8 * 1.06 * vv[0, :, 0].double().abs().mean(0).cpu(), torch.bfloat16)
 
 
+@pytest.mark.parametrize("slope", ["rising", "falling", "steps", "one"])
+@pytest.mark.parametrize("B,NQ,H,HK,d,dv,causal", [(1, 5, 2, 1, 64, 128, False), (2, 150, 2, 1, 64, 128, True), (2, 150, 2, 2, 32, 64, False), (9, 130, 8, 4, 64, 128, True),
+                                                   (1, 140, 1, 1, 128, 256, True)])
+def test_differential_attention_of_steep_scores(F, B, NQ, H, HK, d, dv, causal, slope):
+    """Scores that run over a range of 300 along the keys, in a different direction in each map: the running maximum moves in every block, in
+    none, now and then, or once.  fp32 scores of that size are off by 300 x 2^-23 at most, which the bounds' room beside a bf16 step covers."""
+    NK = 600
+    q, k, v, lam, dout = _attention_inputs((B, NQ, NK, H, HK, d, dv, causal, None, 0.05))
+    j = torch.arange(NK, dtype=torch.float64)
+    f = {"rising": j / 2, "falling": (NK - j) / 2, "steps": (j // 97) * 50, "one": 300.0 * (j == 431)}[slope]
+    q[..., 0] = 8.0
+    k[..., 0, 0] = (f * d ** 0.5 / 8).to(torch.bfloat16)[None, :, None]
+    k[..., 1, 0] = (f.flip(0) * d ** 0.5 / 8).to(torch.bfloat16)[None, :, None]
+    leaves = [t.cuda().requires_grad_(True) for t in (q, k, v, lam)]
+    out = F.differential_attention(*leaves, causal=causal)
+    want, eo, gr, er = _attention_reference(q, k, v, lam, d ** -0.5, causal, None, dout)
+    _check("out", out, want, eo, torch.bfloat16)
+    grads = torch.autograd.grad(out, leaves, dout.cuda())
+    for n, got in zip(("v", "lam", "q", "k"), (grads[2], grads[3], grads[0], grads[1])):
+        _check("d " + n, got, gr[n], er[n] + 1e-30, got.dtype)
+
+
 def test_differential_attention_gradients_against_differences(F):
     """The output is linear in lam and in v: differences over whole steps are exact but for the stored roundings (2^-8 of the two
     outputs and of the probabilities)."""
