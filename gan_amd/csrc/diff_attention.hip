@@ -603,7 +603,8 @@ __global__ __launch_bounds__(kThreads, (Cfg<DK, DV>::WAVES)) void diff_fwd_kerne
 // half forms exponentials; the multiplying waves go first where both could issue.  The two shares are joined at the end.  Tiles go through
 // a ring of five: two are in use, the others have landed or are on their way.  N 4096, batch 32, one head of 64/128: 436 us with two
 // independent workgroups of 4 waves per CU, 411 so (752 TFLOP/s, matrix unit busy 55 % of the cycles at the 1.84 GHz that power leaves);
-// N 4096, 8 heads of one sample, where every CU has one workgroup: 126 and 97; 2048, 16 heads: 68 and 55.
+// N 4096, 8 heads of one sample, where every CU has one workgroup: 126 and 97; 2048, 16 heads: 68 and 55.  It starts later and ends with the
+// joining of the halves, so that short walks are left to the four waves (takes_turns).
 template <int DK, int DV>
 struct TurnsCfg {
   static constexpr int NW = 8, KB = kBlk * DK * 2, VB = kBlk * DV * 2, STAGE = 2 * KB + VB, LOADS = STAGE / 1024 / NW;
@@ -1847,6 +1848,16 @@ void plan_forward(const gc_diff_attention* a, DiffParams& P) {
   P.nsplit = (int)((nblk + P.blocks_per_split - 1) / P.blocks_per_split);
   if (P.nsplit < 1) P.nsplit = 1;
 }
+// Which forward kernel, by the length of a workgroup's walk: halves that take turns start and join slower than four waves, and walk faster,
+// above all where a CU has one workgroup.  Measured, us by turns and by four waves, 8 heads of 64/128, N x N:
+//   at most one workgroup per CU   N 128: 16 and 12,  256: 18.3 and 16.3,  512: 23.1 and 24.5,  1024: 33 and 39,  2048: 55 and 76
+//   8 per CU                       N 128: 119 and 68, 256: 126 and 81,  512: 161 and 124,  1024: 242 and 212,  2048: 415 and 409 (causal 266
+//                                  and 258; 4 per CU 209 and 210, causal 139 and 157),  4096 (4 per CU): 381 and 403, causal 217 and 246
+//   32/64, whose blocks are half as long, 4 to 8 per CU: 1024: 163 and 139, 2048: 280 and 266, 4096: 263 and 260, causal 152 and 165
+bool takes_turns(const DiffParams& P, int form) {
+  const int64_t groups = (int64_t)P.a.B * P.a.HK * P.tiles * P.nsplit;
+  return form < 2 && P.blocks_per_split >= (groups <= device_cu_count() ? 8 : (form == 0 ? 64 : 32));
+}
 size_t forward_bytes(const DiffParams& P, int DV) {
   if (P.nsplit <= 1) return 0;
   const size_t rows = (size_t)P.nsplit * P.a.B * P.a.HK * P.G * P.a.NQ;
@@ -1969,7 +1980,8 @@ extern "C" int gc_diff_attention_fwd(const gc_diff_attention* desc, void* worksp
     ProfScope ps(P.few ? "gc::diff_few_rows_kernel" : "gc::diff_fwd_kernel", 4.0 * desc->B * desc->H * (double)desc->NQ * desc->NK * (desc->d + desc->dv), s);
     int e;
     if (P.few) e = form == 0 ? launch_few<32, 64>(P, s) : (form == 1 ? launch_few<64, 128>(P, s) : launch_few<128, 256>(P, s));
-    else e = form == 0 ? launch_turns<32, 64>(P, s) : (form == 1 ? launch_turns<64, 128>(P, s) : launch_fwd<128, 256>(P, s));
+    else if (takes_turns(P, form)) e = form == 0 ? launch_turns<32, 64>(P, s) : launch_turns<64, 128>(P, s);
+    else e = form == 0 ? launch_fwd<32, 64>(P, s) : (form == 1 ? launch_fwd<64, 128>(P, s) : launch_fwd<128, 256>(P, s));
     if (e) return e;
   }
   if (P.nsplit > 1) {

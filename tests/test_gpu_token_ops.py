@@ -577,6 +577,43 @@ def test_differential_attention_never_reads_behind_a_length(F):
     _check("mean", out[0, 0, 0], vv[0, :, 0].double().mean(0), 2.0 ** -8 * 1.06 * vv[0, :, 0].double().abs().mean(0).cpu(), torch.bfloat16)
 
 
+# Both forward kernels on either side of each of the rule's limits: eight blocks of keys where every CU has a workgroup at most, 32 (64 in the
+# narrow form) where more have to share one, and shares of four blocks and of eight.
+WALK_CASES = [
+    (2, 100, 448, 2, 1, 64, 128, True, (448, 384), 1.0),
+    (2, 100, 449, 2, 1, 64, 128, True, (449, 63), 1.0),
+    (3, 70, 512, 4, 4, 32, 64, False, (0, 1, 512), 1.0),
+    (2, 40, 449, 2, 2, 40, 72, True, None, 2.0),
+    (33, 40, 700, 8, 8, 64, 128, True, None, 1.0),
+    (33, 40, 1984, 8, 8, 64, 128, False, None, 1.0),
+    (33, 40, 1985, 8, 8, 64, 128, True, tuple((1985, 0, 1, 33, 700)[i % 5] for i in range(33)), 1.0),
+    (33, 33, 4032, 8, 8, 32, 64, False, None, 1.0),
+    (33, 33, 4033, 8, 8, 32, 64, True, None, 1.0),
+    (1, 200, 2048, 1, 1, 64, 128, True, None, 1.0),
+    (1, 130, 8000, 2, 1, 64, 128, True, (7000,), 1.0),
+]
+
+
+@pytest.mark.parametrize("case", WALK_CASES, ids=lambda c: "x".join(map(str, c[:7])) + ("-causal" if c[7] else "") + ("-lengths" if c[8] else ""))
+def test_differential_attention_of_short_and_long_walks(F, case):
+    test_differential_attention_against_the_definition(F, case)
+
+
+@pytest.mark.parametrize("B,NK,d,dv", [(3, 200, 32, 64), (3, 700, 64, 128), (3, 700, 32, 64), (140, 2000, 64, 128)])
+def test_differential_attention_walks_never_read_behind_a_length(F, B, NK, d, dv):
+    """As above, in a walk of every kernel that takes many rows."""
+    ln = torch.tensor([(0, 65, NK - 70)[i % 3] for i in range(B)], device="cuda")
+    q, k, v, lam, _ = (t.cuda() for t in _attention_inputs((B, 70, NK, 2, 2, d, dv, False, None, 1.0)))
+    hidden = torch.arange(NK, device="cuda")[None] >= ln[:, None]
+    kn, vn = k.clone(), v.clone()
+    kn[hidden], vn[hidden] = float("nan"), float("inf")
+    with torch.no_grad():
+        for causal in (False, True):
+            out = F.differential_attention(q, kn, vn, lam, causal=causal, key_lengths=ln)
+            assert torch.equal(out, F.differential_attention(q, k, v, lam, causal=causal, key_lengths=ln))
+            assert float(out[0].abs().max()) == 0.0
+
+
 @pytest.mark.parametrize("slope", ["rising", "falling", "steps", "one"])
 @pytest.mark.parametrize("B,NQ,H,HK,d,dv,causal", [(1, 5, 2, 1, 64, 128, False), (2, 150, 2, 1, 64, 128, True), (2, 150, 2, 2, 32, 64, False), (9, 130, 8, 4, 64, 128, True),
                                                    (1, 140, 1, 1, 128, 256, True)])
