@@ -1300,7 +1300,8 @@ __global__ __launch_bounds__(kThreads) void diff_sum_kernel(const float* part, i
 // chain that dP is does not wait for itself.  For grids of up to a workgroup per CU, which it fills with two waves per SIMD (dQ and the rest
 // of both passes, N 2048, 16 heads on 4: 259 us with the kernel above, 247 with this one; 1500, 16 heads 173 and 163; 4 x 1024, 8 heads,
 // causal 133 and 127).  Larger grids it does no good (batch 32, N 4096: 442 and 459 us), small ones that are split further neither (1024,
-// 4 heads: 85 and 87).
+// 4 heads: 85 and 87), nor walks of fewer than 12 blocks (both passes, 8 heads of 64/128, us with the kernel above and with this one: 32 x 128
+// rows of 128 keys 58 and 63, of 320 88 and 94, of 704 153 and 152; 1536 x 1536, two shares of 12, 132 and 128).
 template <int DK, int DV>
 __global__ __launch_bounds__(512, 2) void diff_bwd_dq_turns_kernel(const DiffParams P) {
   typedef Cfg<DK, DV> F;
@@ -1878,8 +1879,9 @@ BackwardPlan plan_backward(const gc_diff_attention* a) {
   p.dq_tiles = (a->NQ + kRows - 1) / kRows;
   p.dkv_tiles = (a->NK + kRows - 1) / kRows;
   const int64_t dq_groups = (int64_t)a->B * a->H * p.dq_tiles;
-  p.dq_turns = form_of(a) < 2 && dq_groups <= cus && 4 * dq_groups > cus;
-  int64_t n = p.dq_turns ? std::max<int64_t>(1, std::min(cus / dq_groups, nkb / 4)) : shares_of(a, dq_groups, nkb, 10);
+  int64_t n = dq_groups > 0 ? std::max<int64_t>(1, std::min(cus / dq_groups, nkb / 4)) : 1;
+  p.dq_turns = form_of(a) < 2 && dq_groups <= cus && 4 * dq_groups > cus && nkb / n >= 12;
+  if (!p.dq_turns) n = shares_of(a, dq_groups, nkb, 10);
   p.dq_blocks = (int)((nkb + n - 1) / n);
   p.dq_shares = (int)((nkb + p.dq_blocks - 1) / p.dq_blocks);
   const int64_t groups = (int64_t)a->B * a->HK * p.dkv_tiles, steps = G * nqb;

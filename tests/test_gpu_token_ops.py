@@ -591,6 +591,12 @@ WALK_CASES = [
     (33, 33, 4033, 8, 8, 32, 64, True, None, 1.0),
     (1, 200, 2048, 1, 1, 64, 128, True, None, 1.0),
     (1, 130, 8000, 2, 1, 64, 128, True, (7000,), 1.0),
+    # dQ: grids of a quarter to one workgroup per CU, on either side of walks of 12 blocks, whole and in shares
+    (9, 130, 704, 8, 4, 64, 128, True, (704, 0, 1, 33, 700, 64, 65, 640, 641), 1.0),
+    (9, 130, 705, 8, 4, 64, 128, True, (705, 0, 1, 33, 700, 64, 65, 640, 641), 1.0),
+    (9, 130, 1600, 4, 2, 32, 64, False, (1600, 31, 32, 33, 64, 65, 0, 1, 1540), 1.0),
+    (6, 90, 800, 24, 24, 40, 80, True, None, 2.0),
+    (3, 129, 2400, 12, 3, 64, 128, True, (2400, 500, 64), 1.0),
 ]
 
 
@@ -617,13 +623,12 @@ def test_differential_attention_walks_never_read_behind_a_length(F, B, NK, d, dv
 @pytest.mark.parametrize("slope", ["rising", "falling", "steps", "one"])
 @pytest.mark.parametrize("B,NQ,H,HK,d,dv,causal", [(1, 5, 2, 1, 64, 128, False), (2, 150, 2, 1, 64, 128, True), (2, 150, 2, 2, 32, 64, False), (9, 130, 8, 4, 64, 128, True),
                                                    (1, 140, 1, 1, 128, 256, True)])
-def test_differential_attention_of_steep_scores(F, B, NQ, H, HK, d, dv, causal, slope):
+def test_differential_attention_of_steep_scores(F, B, NQ, H, HK, d, dv, causal, slope, NK=600):
     """Scores that run over a range of 300 along the keys, in a different direction in each map: the running maximum moves in every block, in
     none, now and then, or once.  fp32 scores of that size are off by 300 x 2^-23 at most, which the bounds' room beside a bf16 step covers."""
-    NK = 600
     q, k, v, lam, dout = _attention_inputs((B, NQ, NK, H, HK, d, dv, causal, None, 0.05))
     j = torch.arange(NK, dtype=torch.float64)
-    f = {"rising": j / 2, "falling": (NK - j) / 2, "steps": (j // 97) * 50, "one": 300.0 * (j == 431)}[slope]
+    f = {"rising": j * (300 / NK), "falling": (NK - j) * (300 / NK), "steps": (j // 97) * (30000 / NK), "one": 300.0 * (j == 431)}[slope]
     q[..., 0] = 8.0
     k[..., 0, 0] = (f * d ** 0.5 / 8).to(torch.bfloat16)[None, :, None]
     k[..., 1, 0] = (f.flip(0) * d ** 0.5 / 8).to(torch.bfloat16)[None, :, None]
@@ -634,6 +639,12 @@ def test_differential_attention_of_steep_scores(F, B, NQ, H, HK, d, dv, causal, 
     grads = torch.autograd.grad(out, leaves, dout.cuda())
     for n, got in zip(("v", "lam", "q", "k"), (grads[2], grads[3], grads[0], grads[1])):
         _check("d " + n, got, gr[n], er[n] + 1e-30, got.dtype)
+
+
+@pytest.mark.parametrize("slope", ["rising", "falling", "steps", "one"])
+@pytest.mark.parametrize("B,NQ,H,HK,d,dv", [(9, 130, 8, 4, 64, 128), (9, 130, 8, 8, 32, 64), (33, 33, 8, 8, 64, 128)])
+def test_differential_attention_of_steep_scores_in_long_walks(F, B, NQ, H, HK, d, dv, slope):
+    test_differential_attention_of_steep_scores(F, B, NQ, H, HK, d, dv, True, slope, NK=2000 if B == 33 else 800)
 
 
 def test_differential_attention_gradients_against_differences(F):
